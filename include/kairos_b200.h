@@ -220,6 +220,73 @@ int kairos_rope_kv(const void* QKV_f16, const void* cos_table, const void* sin_t
                    int pos0, void* Q_out, void* K_cache, void* V_cache, int B, int S, int H, int Hkv, int D,
                    int max_len, kairos_stream_t stream);
 
+/* ---- decoding over a paged key-value cache ------------------------------------------------------
+ * No counterpart in the reference, whose runs keep HuggingFace's contiguous fp16 cache.  A cache is a pool of
+ * pages; a sequence owns a list of them (a row of the page table), so a batch of sequences of different lengths
+ * shares one pool.  One layer's pool, as the operators see it: */
+enum {
+    KAIROS_DTYPE_F16 = 0,
+    KAIROS_DTYPE_BF16 = 1,
+    KAIROS_DTYPE_F32 = 2,
+    KAIROS_DTYPE_I8 = 3,  /* cache only: value = code * scale, scale = max|row| / 127 */
+    KAIROS_DTYPE_E4M3 = 4 /* cache only: value = code * scale, scale = max|row| / 448 */
+};
+typedef struct {
+    void* k;        /* [pages, kv_heads, page_size, head_dim], elements of `dtype`, 16-byte aligned */
+    void* v;
+    float* k_scale; /* [pages, kv_heads, page_size], one per row of an I8 / E4M3 cache; null otherwise */
+    float* v_scale;
+    int pages, kv_heads, page_size, head_dim; /* page_size 16, 32, 64, 128 or 256; head_dim 64, 128 or 256 */
+    int dtype;
+} kairos_kv_layer;
+/* Rotary positions.  Pair i of the first `rot` channels of a head (channels i and i + rot / 2 in layout 0, "half";
+ * 2 i and 2 i + 1 in layout 1, "interleaved") is turned by position * f_i and multiplied by `magnitude`; the
+ * channels behind `rot` pass unchanged.  f_i is given as a binary fraction of a full turn:
+ * steps[i] = round(f_i / (2 pi) * 2^64), uint64 in device memory.  position * step modulo 2^64 IS the angle, so a
+ * position of any size (negative ones included) has an angle that is exact to 2^-32 turns: no table, no far-position
+ * error. */
+typedef struct {
+    const void* steps; /* uint64 [rot / 2] */
+    float magnitude;
+    int rot;    /* even, <= head dim */
+    int layout; /* 0 half, 1 interleaved */
+} kairos_rotary_plan;
+/* Y[b,s,h,:] = turned X[b,s,h,:]; X and Y are F16 / BF16 / F32 with element strides {b, s, h} and a dense last
+ * dimension (D <= 512); Y may be X.  positions: int64 with element strides {b, s} (0 broadcasts).  transpose != 0
+ * turns the other way with the same magnitude: the transposed operator, i.e. the gradient of X from that of Y.
+ * Rows that are 16-byte aligned with D % 16 == 0 and rot % 16 == 0 move in 16-byte accesses, others element-wise. */
+int kairos_rotary(const void* X, const long long* x_strides, void* Y, const long long* y_strides, const void* positions,
+                  const long long* pos_strides, const kairos_rotary_plan* plan, int dtype, int transpose, int B, int S,
+                  int H, int D, kairos_stream_t stream);
+/* The attention input of T tokens in one pass: of each row of QKV [T, (H + 2 kv_heads) * D] (F16 / BF16, row stride in
+ * elements, a multiple of 8) the q heads are turned into Q_out [T, H, D], the k heads are turned and the v heads copied into the
+ * cache at slots[t] = page * page_size + offset (int64).  A 16-bit cache has QKV's type; rows of an I8 / E4M3 cache
+ * are quantized from the fp32 rotated values (code = nearest-even of row / scale).  A row with an infinity or NaN
+ * gets scale NaN.  slots[t] < 0 marks padding: nothing is stored for it (its q row is).  slots[t] past the pool is
+ * not stored either and raises the device status word (KAIROS_ERR_ARG).  Slots must be distinct.
+ * rot % 16 == 0. */
+int kairos_rope_paged_kv(const void* QKV, long long row_stride, const void* positions, const void* slots,
+                         const kairos_rotary_plan* plan, const kairos_kv_layer* kv, void* Q_out, int T, int H, int dtype,
+                         kairos_stream_t stream);
+/* K_out / V_out [T, kv_heads, D] (F16, BF16 or F32) = what the cache holds at slots[t], code * scale rounded once;
+ * zeros where slots[t] < 0, and past the pool (which raises the status word). */
+int kairos_paged_kv_read(const kairos_kv_layer* kv, const void* slots, void* K_out, void* V_out, int T, int dtype,
+                         kairos_stream_t stream);
+/* Attention of one new token per sequence: O[b,h,:] = sum_j softmax_j(scale * Q[b,h,:] . K[j,:]) V[j,:] over the
+ * sequence's lens[b] positions, position j at offset j % page_size of page page_table[b, j / page_size].
+ * Q [B, H, D] F16 / BF16 with element strides {b, h} (multiples of 8); O dense [B, H, D] of the same type; a 16-bit cache has Q's
+ * type.  H % kv_heads == 0 (head h reads kv head h / (H / kv_heads)).  LSE [B, H] fp32 (natural logarithm of the
+ * softmax's denominator) when not null.  lens[b] <= 0: O = 0, LSE = -inf.  Entries of the table behind the end are
+ * not read.  A page outside the pool is left out of the sum, lens[b] is cut to table_width * page_size, and both
+ * raise the status word (KAIROS_ERR_ARG).  Scores, softmax sums and outputs are accumulated in fp32.
+ * `workspace` of kairos_paged_attention_workspace_bytes() is scratch of this call alone (contents need no
+ * initialisation): calls that may overlap need workspaces of their own. */
+size_t kairos_paged_attention_workspace_bytes(const kairos_kv_layer* kv, int B, int H, int table_width);
+int kairos_paged_attention(const void* Q, const long long* q_strides, const kairos_kv_layer* kv, const void* page_table,
+                           long long table_stride, int table_width, const void* lens, void* O, void* LSE_or_null, int B,
+                           int H, float scale, int dtype, void* workspace, size_t workspace_bytes,
+                           kairos_stream_t stream);
+
 /* ---- interval LUT: M -> kernel id  (kernels/csrc/kairos_kernel/lut/lut.h:8-43) ---- */
 typedef struct kairos_lut kairos_lut;
 kairos_lut* kairos_lut_create(void);

@@ -47,6 +47,12 @@ SIGNATURES = {
     'kairos_add_rms_norm': (c_int, [c_void_p] * 4 + [c_int, c_int, ctypes.c_float, c_void_p]),
     'kairos_silu_mul_quant': (c_int, [c_void_p] * 4 + [c_int, c_int, c_void_p]),
     'kairos_rope_kv': (c_int, [c_void_p] * 4 + [c_int] + [c_void_p] * 3 + [c_int] * 6 + [c_void_p]),
+    'kairos_rotary': (c_int, [c_void_p] * 7 + [c_int] * 6 + [c_void_p]),
+    'kairos_rope_paged_kv': (c_int, [c_void_p, ctypes.c_longlong] + [c_void_p] * 5 + [c_int] * 3 + [c_void_p]),
+    'kairos_paged_kv_read': (c_int, [c_void_p] * 4 + [c_int] * 2 + [c_void_p]),
+    'kairos_paged_attention_workspace_bytes': (c_size_t, [c_void_p] + [c_int] * 3),
+    'kairos_paged_attention': (c_int, [c_void_p] * 4 + [ctypes.c_longlong, c_int] + [c_void_p] * 3 +
+                               [c_int, c_int, ctypes.c_float, c_int, c_void_p, c_size_t, c_void_p]),
     'kairos_peer_allreduce_signal_bytes': (c_int, []),
     'kairos_peer_allreduce_f16': (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, ctypes.c_longlong, c_void_p]),
     'kairos_add_rms_norm_peer': (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int,
@@ -71,6 +77,19 @@ SIGNATURES = {
     'kairos_layer_prefetch': (c_int, [c_void_p, c_int, c_void_p]),
     'kairos_switched_linear_host': (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
 }
+
+
+
+class KvLayer(ctypes.Structure):
+    """``kairos_kv_layer``: one layer of a paged cache."""
+    _fields_ = [('k', c_void_p), ('v', c_void_p), ('k_scale', c_void_p), ('v_scale', c_void_p), ('pages', c_int),
+                ('kv_heads', c_int), ('page_size', c_int), ('head_dim', c_int), ('dtype', c_int)]
+
+
+class RotaryPlan(ctypes.Structure):
+    """``kairos_rotary_plan``."""
+    _fields_ = [('steps', c_void_p), ('magnitude', ctypes.c_float), ('rot', c_int), ('layout', c_int)]
+
 
 if not os.path.exists(LIB_PATH):
     raise ImportError(

@@ -59,8 +59,13 @@ int* device_status_word() {
     std::lock_guard<std::mutex> lk(mu);
     if (!words[dev]) {
         int* w = nullptr;
-        if (cudaHostAlloc(reinterpret_cast<void**>(&w), sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) !=
-            cudaSuccess) {
+        // the first call on a device may come while one of its streams is capturing: the word is no part of the graph
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        const cudaError_t e =
+            cudaHostAlloc(reinterpret_cast<void**>(&w), sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess) {
             cudaGetLastError();
             return nullptr;
         }

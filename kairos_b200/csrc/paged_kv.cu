@@ -1,0 +1,288 @@
+// Writing a paged key-value cache (rotary positions, quantization and the scatter in one pass over the fused QKV
+// activation) and reading it back.  Both are HBM-bound: an activation is read once and a cache row written once.
+#include <cfloat>
+#include <type_traits>
+
+#include "paged_kv.cuh"
+
+namespace kairos {
+
+// Largest magnitude of a row held by `lanes` consecutive threads (a power of two, aligned), 16 values each;
+// NaN if the row has an infinity or a NaN.
+__device__ __forceinline__ float row_amax(const float (&a)[8], const float (&b)[8], int lanes) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, fmaxf(fabsf(a[i]), fabsf(b[i])));
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bad |= !(fabsf(a[i]) <= FLT_MAX) | !(fabsf(b[i]) <= FLT_MAX);
+    if (bad) m = __int_as_float(0x7f800000);
+    for (int o = lanes >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m <= FLT_MAX ? m : __int_as_float(0x7fffffff);
+}
+
+struct CodesI8 {
+    static constexpr float kTop = 127.f;
+    static __device__ __forceinline__ uint2 encode(const float (&x)[8], float scale, float inv) {
+        uint32_t q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = (uint32_t)max(-127, min(127, rint_div(x[i], scale, inv)));
+        uint2 out;
+        out.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+        out.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
+        return out;
+    }
+    static __device__ __forceinline__ void decode(const uint2& v, float (&f)[8]) {
+        const uint32_t w[2] = {v.x, v.y};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = (float)(int)(signed char)(w[i >> 2] >> (8 * (i & 3)));
+    }
+};
+struct CodesE4M3 {
+    static constexpr float kTop = 448.f;
+    static __device__ __forceinline__ uint2 encode(const float (&x)[8], float scale, float) {
+        uint32_t p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            p[i] = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x[2 * i], scale), __fdiv_rn(x[2 * i + 1], scale)),
+                                            __NV_SATFINITE, __NV_E4M3);
+        return make_uint2(p[0] | (p[1] << 16), p[2] | (p[3] << 16));
+    }
+    static __device__ __forceinline__ void decode(const uint2& v, float (&f)[8]) {
+        const uint32_t w[2] = {v.x, v.y};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i >> 1] >> (16 * (i & 1))), __NV_E4M3);
+            const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&h));
+            f[2 * i] = t.x;
+            f[2 * i + 1] = t.y;
+        }
+    }
+};
+
+struct WriteShape {
+    long long row_stride;
+    int T, H, rot, layout, tokens_per_block;
+    float magnitude;
+};
+
+// Codes = void: the cache holds the activation's own type.  One block takes `tokens_per_block` tokens: their angles go
+// to shared memory once, then every thread moves cells of 16 elements; the D / 16 threads of a row are neighbours in
+// one warp, so the row's maximum is a few shuffles.
+template <typename T, typename Codes, int D>
+__global__ void __launch_bounds__(256) rope_paged_kv_kernel(const T* __restrict__ QKV, const long long* __restrict__ positions,
+                                                            const long long* __restrict__ slots,
+                                                            const unsigned long long* __restrict__ steps, const KvView kv,
+                                                            T* __restrict__ Q, const WriteShape p, int* status) {
+    constexpr int kLanes = D / 16;
+    __shared__ __align__(16) float cs[kTablePairs], sn[kTablePairs];
+    chain_release();
+    chain_wait();
+    const int t0 = blockIdx.x * p.tokens_per_block;
+    const int here = min(p.tokens_per_block, p.T - t0);
+    const int pairs = p.rot >> 1;
+    for (int i = threadIdx.x; i < here * pairs; i += 256) {
+        const int t = i / pairs, pair = i - t * pairs;
+        float c, s;
+        turn_of(__ldcg(positions + t0 + t), __ldg(steps + pair), p.magnitude, &c, &s);
+        cs[i] = c;
+        sn[i] = s;
+    }
+    __syncthreads();
+    const int heads = p.H + 2 * kv.heads;
+    const int total = here * heads * kLanes;
+    const long long capacity = (long long)kv.pages << kv.page_shift;
+    for (int base = 0; base < total; base += 256) {        // whole warps stay together for the shuffles
+        const int i = base + threadIdx.x;
+        const bool live = i < total;
+        const int row = (live ? i : 0) / kLanes, j = i % kLanes;
+        const int t = row / heads, head = row - t * heads;
+        const T* x = QKV + (size_t)(t0 + t) * p.row_stride + (size_t)head * D;
+        const Cell cell = cell_of(j, p.rot, p.layout);
+        float a[8], b[8];
+        load8(x + cell.first, a);
+        load8(x + cell.second, b);
+        if (cell.pair >= 0 && head < p.H + kv.heads) turn_cell(a, b, cs + t * pairs, sn + t * pairs, cell.pair, p.layout);
+        float amax = 0.f;
+        if constexpr (!std::is_void<Codes>::value) amax = row_amax(a, b, kLanes);
+        if (!live) continue;
+        if (head < p.H) {
+            T* q = Q + ((size_t)(t0 + t) * p.H + head) * D;
+            store8(q + cell.first, a);
+            store8(q + cell.second, b);
+            continue;
+        }
+        const long long slot = __ldcg(slots + t0 + t);
+        if (slot < 0) continue;                            // padding
+        if (slot >= capacity) {
+            *status = KAIROS_ERR_ARG;
+            continue;
+        }
+        const bool is_v = head >= p.H + kv.heads;
+        const size_t r = pool_row(kv, slot, head - p.H - (is_v ? kv.heads : 0));
+        if constexpr (std::is_void<Codes>::value) {
+            T* y = static_cast<T*>(is_v ? kv.v : kv.k) + r * D;
+            store8(y + cell.first, a);
+            store8(y + cell.second, b);
+        } else {
+            float scale = __fdiv_rn(amax, Codes::kTop);
+            uint2 qa = make_uint2(0, 0), qb = qa;
+            if (scale > 0.f) {                             // false for a row of zeros and for NaN: codes 0
+                const float inv = __frcp_rn(scale);
+                qa = Codes::encode(a, scale, inv);
+                qb = Codes::encode(b, scale, inv);
+            }
+            uint8_t* y = static_cast<uint8_t*>(is_v ? kv.v : kv.k) + r * D;
+            *reinterpret_cast<uint2*>(y + cell.first) = qa;
+            *reinterpret_cast<uint2*>(y + cell.second) = qb;
+            if (j == 0) (is_v ? kv.vs : kv.ks)[r] = scale;
+        }
+    }
+}
+
+// One thread brings the same eight channels of a K row and of its V row.
+template <typename C, typename Codes, typename T>
+__global__ void __launch_bounds__(256) paged_kv_read_kernel(const KvView kv, const long long* __restrict__ slots,
+                                                            T* __restrict__ K, T* __restrict__ V, long long total,
+                                                            int* status) {
+    chain_release();
+    chain_wait();
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const int chunks = kv.dim >> 3;
+    const int c = (int)(i % chunks);
+    const long long row = i / chunks;
+    const int head = (int)(row % kv.heads);
+    const long long slot = __ldcg(slots + row / kv.heads);
+    float k[8] = {}, v[8] = {};
+    if (slot >= 0 && slot < ((long long)kv.pages << kv.page_shift)) {
+        const size_t r = pool_row(kv, slot, head);
+        if constexpr (std::is_void<Codes>::value) {
+            load8(static_cast<const C*>(kv.k) + r * kv.dim + 8 * c, k);
+            load8(static_cast<const C*>(kv.v) + r * kv.dim + 8 * c, v);
+        } else {
+            const uint2 kc = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(kv.k) + r * kv.dim) + c);
+            const uint2 vc = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(kv.v) + r * kv.dim) + c);
+            const float ks = __ldcg(kv.ks + r), vs = __ldcg(kv.vs + r);
+            Codes::decode(kc, k);
+            Codes::decode(vc, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                k[e] *= ks;
+                v[e] *= vs;
+            }
+        }
+    } else if (slot >= 0) {
+        *status = KAIROS_ERR_ARG;
+    }
+    store8(K + row * kv.dim + 8 * c, k);
+    store8(V + row * kv.dim + 8 * c, v);
+}
+
+template <typename T, typename Codes, int D>
+static int run_write(const void* QKV, const void* positions, const void* slots, const void* steps, const KvView& kv, void* Q,
+                     WriteShape p, int* status, cudaStream_t st) {
+    const int cells = (p.H + 2 * kv.heads) * (D / 16);
+    int tb = cells >= 256 ? 1 : (256 + cells - 1) / cells;
+    if (p.rot) tb = min(tb, kTablePairs / (p.rot / 2));
+    p.tokens_per_block = max(1, tb);
+    const cudaError_t e = launch_chained(
+        rope_paged_kv_kernel<T, Codes, D>, dim3((unsigned)((p.T + p.tokens_per_block - 1) / p.tokens_per_block)), dim3(256), 0,
+        st, static_cast<const T*>(QKV), static_cast<const long long*>(positions), static_cast<const long long*>(slots),
+        static_cast<const unsigned long long*>(steps), kv, static_cast<T*>(Q), p, status);
+    if (e != cudaSuccess) return note_cuda_error(e);
+    return launch_status();
+}
+
+template <typename T, typename Codes>
+static int pick_write(const void* QKV, const void* positions, const void* slots, const void* steps, const KvView& kv, void* Q,
+                      const WriteShape& p, int* status, cudaStream_t st) {
+    if (kv.dim == 64) return run_write<T, Codes, 64>(QKV, positions, slots, steps, kv, Q, p, status, st);
+    if (kv.dim == 128) return run_write<T, Codes, 128>(QKV, positions, slots, steps, kv, Q, p, status, st);
+    return run_write<T, Codes, 256>(QKV, positions, slots, steps, kv, Q, p, status, st);
+}
+
+template <typename C, typename Codes, typename T>
+static int run_read(const KvView& kv, const void* slots, void* K, void* V, long long T_, int* status, cudaStream_t st) {
+    const long long total = T_ * kv.heads * (kv.dim / 8);
+    const long long blocks = (total + 255) / 256;
+    if (blocks > 0x7fffffffLL) return KAIROS_ERR_SHAPE;
+    const cudaError_t e = launch_chained(paged_kv_read_kernel<C, Codes, T>, dim3((unsigned)blocks), dim3(256), 0, st, kv,
+                                         static_cast<const long long*>(slots), static_cast<T*>(K), static_cast<T*>(V), total,
+                                         status);
+    if (e != cudaSuccess) return note_cuda_error(e);
+    return launch_status();
+}
+
+template <typename T>
+static int pick_read(int dtype, const KvView& kv, const void* slots, void* K, void* V, long long n, int* status,
+                     cudaStream_t st) {
+    switch (dtype) {
+        case KAIROS_DTYPE_F16: return run_read<__half, void, T>(kv, slots, K, V, n, status, st);
+        case KAIROS_DTYPE_BF16: return run_read<__nv_bfloat16, void, T>(kv, slots, K, V, n, status, st);
+        case KAIROS_DTYPE_I8: return run_read<uint8_t, CodesI8, T>(kv, slots, K, V, n, status, st);
+        default: return run_read<uint8_t, CodesE4M3, T>(kv, slots, K, V, n, status, st);
+    }
+}
+
+int* device_status_word();   // api.cu
+
+}  // namespace kairos
+
+extern "C" int kairos_rope_paged_kv(const void* QKV, long long row_stride, const void* positions, const void* slots,
+                                    const kairos_rotary_plan* plan, const kairos_kv_layer* layer, void* Q_out, int T, int H,
+                                    int dtype, kairos_stream_t stream) {
+    using namespace kairos;
+    KvView kv;
+    const int rc = kv_view(layer, &kv);
+    if (rc != KAIROS_OK) return rc;
+    if (T < 0 || H <= 0 || row_stride % 8 != 0 || row_stride < (long long)(H + 2LL * kv.heads) * kv.dim) return KAIROS_ERR_SHAPE;
+    if ((H + 2LL * kv.heads) * kv.dim > (1 << 24)) return KAIROS_ERR_SHAPE;
+    if (!rotary_plan_ok(plan, kv.dim) || plan->rot % 16 != 0) {
+        set_last_error("rope_paged_kv: the rotated part is a multiple of 16 channels, at most the head");
+        return KAIROS_ERR_ARG;
+    }
+    const bool coded = layer->dtype == KAIROS_DTYPE_I8 || layer->dtype == KAIROS_DTYPE_E4M3;
+    if ((dtype != KAIROS_DTYPE_F16 && dtype != KAIROS_DTYPE_BF16) || (!coded && layer->dtype != dtype)) {
+        set_last_error("rope_paged_kv: activations are fp16 or bf16, and a 16-bit cache has their type");
+        return KAIROS_ERR_ARG;
+    }
+    if (T == 0) return KAIROS_OK;
+    if (!QKV || !Q_out || !positions || !slots || ((uintptr_t)QKV & 15) || ((uintptr_t)Q_out & 15) ||
+        ((uintptr_t)positions & 7) || ((uintptr_t)slots & 7))
+        return KAIROS_ERR_ALIGN;
+    int* status = device_status_word();
+    if (!status) return KAIROS_ERR_CUDA;
+    WriteShape p = {};
+    p.row_stride = row_stride;
+    p.T = T; p.H = H; p.rot = plan->rot; p.layout = plan->layout; p.magnitude = plan->magnitude;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const void* s = plan->steps;
+    if (dtype == KAIROS_DTYPE_F16) {
+        if (layer->dtype == KAIROS_DTYPE_I8) return pick_write<__half, CodesI8>(QKV, positions, slots, s, kv, Q_out, p, status, st);
+        if (layer->dtype == KAIROS_DTYPE_E4M3) return pick_write<__half, CodesE4M3>(QKV, positions, slots, s, kv, Q_out, p, status, st);
+        return pick_write<__half, void>(QKV, positions, slots, s, kv, Q_out, p, status, st);
+    }
+    if (layer->dtype == KAIROS_DTYPE_I8) return pick_write<__nv_bfloat16, CodesI8>(QKV, positions, slots, s, kv, Q_out, p, status, st);
+    if (layer->dtype == KAIROS_DTYPE_E4M3) return pick_write<__nv_bfloat16, CodesE4M3>(QKV, positions, slots, s, kv, Q_out, p, status, st);
+    return pick_write<__nv_bfloat16, void>(QKV, positions, slots, s, kv, Q_out, p, status, st);
+}
+
+extern "C" int kairos_paged_kv_read(const kairos_kv_layer* layer, const void* slots, void* K_out, void* V_out, int T, int dtype,
+                                    kairos_stream_t stream) {
+    using namespace kairos;
+    KvView kv;
+    const int rc = kv_view(layer, &kv);
+    if (rc != KAIROS_OK) return rc;
+    if (T < 0) return KAIROS_ERR_SHAPE;
+    if (dtype != KAIROS_DTYPE_F16 && dtype != KAIROS_DTYPE_BF16 && dtype != KAIROS_DTYPE_F32) return KAIROS_ERR_ARG;
+    if (T == 0) return KAIROS_OK;
+    if (!K_out || !V_out || !slots || ((uintptr_t)K_out & 15) || ((uintptr_t)V_out & 15) || ((uintptr_t)slots & 7))
+        return KAIROS_ERR_ALIGN;
+    int* status = device_status_word();
+    if (!status) return KAIROS_ERR_CUDA;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (dtype == KAIROS_DTYPE_F16) return pick_read<__half>(layer->dtype, kv, slots, K_out, V_out, T, status, st);
+    if (dtype == KAIROS_DTYPE_BF16) return pick_read<__nv_bfloat16>(layer->dtype, kv, slots, K_out, V_out, T, status, st);
+    return pick_read<float>(layer->dtype, kv, slots, K_out, V_out, T, status, st);
+}

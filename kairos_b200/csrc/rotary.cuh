@@ -1,0 +1,125 @@
+// Rotary positions: what the stand-alone operator and the cache write share.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace kairos {
+
+// Eight consecutive elements of a row as fp32, in one or two 16-byte accesses.
+__device__ __forceinline__ void load8(const __half* p, float (&f)[8]) {
+    const uint4 v = __ldcg(reinterpret_cast<const uint4*>(p));
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 t = __half22float2(h[i]);
+        f[2 * i] = t.x;
+        f[2 * i + 1] = t.y;
+    }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&f)[8]) {
+    const uint4 v = __ldcg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
+    const float4 a = __ldcg(reinterpret_cast<const float4*>(p)), b = __ldcg(reinterpret_cast<const float4*>(p) + 1);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+__device__ __forceinline__ void store8(__half* p, const float (&f)[8]) {
+    uint4 v;
+    __half2* h = reinterpret_cast<__half2*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = v;
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&f)[8]) {
+    uint4 v;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = v;
+}
+__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+}
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+
+// cos and sin of position * step, step being a binary fraction of a full turn (2^64 = one turn).  The product
+// modulo 2^64 is the angle without any rounding, however far the position; its upper 32 bits, read as a signed
+// number, are half turns in [-1, 1), which is what sincospif takes.  What is dropped is below 2^-32 turns
+// (1.5e-9 rad), under the 2^-24 of the fp32 result.
+__device__ __forceinline__ void turn_of(long long position, unsigned long long step, float magnitude, float* c, float* s) {
+    const unsigned long long a = (unsigned long long)position * step;
+    float sn, cs;
+    sincospif(__int2float_rn((int)(a >> 32)) * 4.656612873077393e-10f, &sn, &cs);   // 2^-31
+    *c = cs * magnitude;
+    *s = sn * magnitude;
+}
+
+// Both members of a pair; sums and products in fp32.
+__device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s) {
+    const float x = a;
+    a = __fmaf_rn(x, c, -(b * s));
+    b = __fmaf_rn(b, c, x * s);
+}
+
+// A row (one head of one token) moves as cells of 16 elements, two chunks of 8, one cell per thread.  In the half
+// layout the two chunks of a rotating cell are partners rot / 2 apart; in the interleaved layout and behind `rot` they
+// are neighbours.  Cell j of a row: its two element offsets, and the first of its eight pairs (-1: passes unchanged).
+struct Cell {
+    int first, second, pair;
+};
+__device__ __forceinline__ Cell cell_of(int j, int rot, int layout) {
+    const int turning = rot >> 4;
+    Cell c;
+    if (layout == 0 && j < turning) {
+        c.first = 8 * j;
+        c.second = 8 * j + (rot >> 1);
+    } else {
+        c.first = 16 * j;
+        c.second = 16 * j + 8;
+    }
+    c.pair = j < turning ? 8 * j : -1;
+    return c;
+}
+// Turns the cell's eight pairs by the table entries cs / sn (fp32 cos and sin, indexed by pair).
+__device__ __forceinline__ void turn_cell(float (&a)[8], float (&b)[8], const float* cs, const float* sn, int pair,
+                                          int layout) {
+    float c[8], s[8];
+    *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(cs + pair);
+    *reinterpret_cast<float4*>(c + 4) = *reinterpret_cast<const float4*>(cs + pair + 4);
+    *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(sn + pair);
+    *reinterpret_cast<float4*>(s + 4) = *reinterpret_cast<const float4*>(sn + pair + 4);
+    if (layout == 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) turn_pair(a[i], b[i], c[i], s[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            turn_pair(a[2 * i], a[2 * i + 1], c[i], s[i]);
+            turn_pair(b[2 * i], b[2 * i + 1], c[4 + i], s[4 + i]);
+        }
+    }
+}
+
+constexpr int kTablePairs = 2048;   // pairs whose cos and sin a block keeps: 16 KB of shared memory
+
+inline bool rotary_plan_ok(const kairos_rotary_plan* p, int D) {
+    return p && p->rot >= 0 && p->rot <= D && (p->rot & 1) == 0 && (p->layout == 0 || p->layout == 1) &&
+           (p->rot == 0 || (p->steps && ((uintptr_t)p->steps & 7) == 0));
+}
+
+}  // namespace kairos

@@ -8,6 +8,8 @@ torch's current stream (the reference's GEMV/GEMM launch on the legacy default s
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from ._lib import check, lib
@@ -277,3 +279,135 @@ def silu_mul_quant(gate_up, want_f16=False, blocked=False):
         check(fn(_chk(gate_up, torch.float16, 'gate_up'), None if y is None else y.data_ptr(), xq.data_ptr(),
                  sx.data_ptr(), m, i2 // 2, stream_ptr()), 'silu_mul_quant')
     return xq, sx, y
+
+
+# ---- decoding over a paged key-value cache ----------------------------------------------------------
+_FLOATS = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_HALVES = (torch.float16, torch.bfloat16)
+_Three, _Two = ctypes.c_longlong * 3, ctypes.c_longlong * 2
+
+
+def _index(t, dtype, device, name):
+    if t.dtype != dtype or t.device != device or not t.is_contiguous():
+        raise ValueError(f'{name}: expected a contiguous tensor of {dtype} on {device}, got {t.dtype} on {t.device}')
+    return t.data_ptr()
+
+
+def _same_device(device, other, name):
+    if not device.type == 'cuda' or other != device:
+        raise ValueError(f'{name} is on {other}, the activations are on {device}: expected one CUDA device')
+
+
+def _head_strides(t):
+    """Element strides of (batch, sequence, head) of [.., H, D]; a dimension of one element has none."""
+    s = [0 if n == 1 else st for n, st in zip(t.shape[:-1], t.stride()[:-1])]
+    return _Three(0, *s) if t.dim() == 3 else _Three(*s)
+
+
+def rotary(x, positions, rotary, transpose=False, out=None):
+    """Heads [T, H, D] or [B, S, H, D] (fp16, bf16 or fp32; dense last dimension, any other strides) turned by their
+    int64 positions, [T] or broadcastable to [B, S], with the plan of a :class:`Rotary`.  ``transpose`` turns back with the same
+    magnitude: the gradient of x from that of the result.  ``out`` may be x."""
+    if x.dtype not in _FLOATS or x.dim() not in (3, 4) or x.shape[-1] != rotary.head_dim or x.stride(-1) != 1:
+        raise ValueError(f'x: expected fp16, bf16 or fp32 [.., heads, {rotary.head_dim}] with a dense last dimension, '
+                         f'got {x.dtype} {tuple(x.shape)}')
+    _same_device(x.device, rotary.steps.device, 'rotary')
+    if positions.dtype != torch.int64 or positions.device != x.device:
+        raise ValueError(f'positions: expected int64 on {x.device}, got {positions.dtype} on {positions.device}')
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1:
+        raise ValueError('out: expected the shape, type and device of x and a dense last dimension')
+    at = positions.expand(x.shape[:-2])
+    b, s = (1, x.shape[0]) if x.dim() == 3 else x.shape[:2]
+    ps = _Two(0, at.stride(0)) if x.dim() == 3 else _Two(*at.stride())
+    with _on(x.device):
+        check(lib.kairos_rotary(x.data_ptr(), _head_strides(x), out.data_ptr(), _head_strides(out), at.data_ptr(), ps,
+                                rotary.plan_ptr, _FLOATS[x.dtype], 1 if transpose else 0, b, s, x.shape[-2], x.shape[-1],
+                                stream_ptr()), 'rotary')
+    return out
+
+
+def rope_paged_kv(qkv, positions, slots, rotary, cache, layer=0, q_out=None):
+    """One pass over the fused activation qkv [T, (H + 2 kv_heads) * D] (fp16 / bf16, rows may be strided): returns the
+    turned q heads [T, H, D], and stores the turned k heads and the v heads at ``slots`` [T] of the cache's `layer`, in
+    the cache's type (int8 / e4m3 rows are quantized from fp32).  positions and slots are int64 [T]; a negative slot is
+    padding and stores nothing; slots must be distinct."""
+    d, hkv = cache.head_dim, cache.kv_heads
+    if qkv.dtype not in _HALVES or qkv.dim() != 2 or qkv.shape[1] % d or (qkv.shape[1] and qkv.stride(1) != 1):
+        raise ValueError(f'qkv: expected fp16 or bf16 [tokens, heads * {d}] with dense rows, got {qkv.dtype} {tuple(qkv.shape)}')
+    t, h = qkv.shape[0], qkv.shape[1] // d - 2 * hkv
+    if h <= 0 or rotary.head_dim != d:
+        raise ValueError(f'qkv has {qkv.shape[1] // d} heads of {d}: the cache holds {hkv} kv heads, the rotary plan turns '
+                         f'heads of {rotary.head_dim}')
+    dev = qkv.device
+    _same_device(dev, cache.device, 'cache')
+    _same_device(dev, rotary.steps.device, 'rotary')
+    if positions.numel() != t or slots.numel() != t:
+        raise ValueError(f'positions and slots: expected {t} each, got {positions.numel()} and {slots.numel()}')
+    if q_out is None:
+        q_out = torch.empty((t, h, d), dtype=qkv.dtype, device=dev)
+    elif q_out.shape != (t, h, d) or q_out.dtype != qkv.dtype or q_out.device != dev or not q_out.is_contiguous():
+        raise ValueError(f'q_out: expected a contiguous {qkv.dtype} [{t}, {h}, {d}] on {dev}')
+    with _on(dev):
+        check(lib.kairos_rope_paged_kv(qkv.data_ptr(), qkv.stride(0) if t > 1 else qkv.shape[1],
+                                       _index(positions, torch.int64, dev, 'positions'),
+                                       _index(slots, torch.int64, dev, 'slots'), rotary.plan_ptr,
+                                       cache.layer_ptrs[layer], q_out.data_ptr(), t, h, _FLOATS[qkv.dtype], stream_ptr()),
+              'rope_paged_kv')
+    return q_out
+
+
+def paged_kv_read(cache, slots, layer=0, dtype=torch.float16, out=None):
+    """(k, v), each [T, kv_heads, D] of `dtype` (fp16, bf16 or fp32): what the cache's `layer` holds at ``slots`` (int64
+    [T]), quantized rows as the values they stand for; zeros where the slot is negative.  ``out``: the two tensors to
+    fill."""
+    if dtype not in _FLOATS:
+        raise ValueError(f'dtype: expected fp16, bf16 or fp32, got {dtype}')
+    dev = cache.device
+    _same_device(slots.device, dev, 'cache')
+    shape = (slots.numel(), cache.kv_heads, cache.head_dim)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
+    for o in out:
+        if o.shape != shape or o.dtype != dtype or o.device != dev or not o.is_contiguous():
+            raise ValueError(f'out: expected two contiguous {dtype} {shape} on {dev}')
+    with _on(dev):
+        check(lib.kairos_paged_kv_read(cache.layer_ptrs[layer], _index(slots, torch.int64, dev, 'slots'), out[0].data_ptr(),
+                                       out[1].data_ptr(), shape[0], _FLOATS[dtype], stream_ptr()), 'paged_kv_read')
+    return out
+
+
+def paged_attention(q, cache, page_table, lens, layer=0, scale=None, out=None, return_lse=False):
+    """Attention of one new token per sequence: q [B, H, D] (fp16 / bf16, strided batch and heads) over the first
+    ``lens[b]`` positions of sequence b, whose pages are row b of ``page_table``.  page_table is int32 [B, W] (entries
+    behind the end are not read), lens int32 [B]; scale defaults to 1 / sqrt(D).  Returns o [B, H, D], with
+    ``return_lse`` also the fp32 [B, H] logarithm of the softmax's denominator.  An empty sequence gives zeros and
+    -inf."""
+    dev, d = q.device, cache.head_dim
+    if q.dtype not in _HALVES or q.dim() != 3 or q.shape[2] != d or q.stride(2) != 1:
+        raise ValueError(f'q: expected fp16 or bf16 [batch, heads, {d}] with a dense last dimension, got {q.dtype} {tuple(q.shape)}')
+    _same_device(dev, cache.device, 'cache')
+    b, h, _ = q.shape
+    if page_table.dim() != 2 or page_table.shape[0] != b or page_table.dtype != torch.int32 or \
+            page_table.device != dev or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError(f'page_table: expected int32 [{b}, pages] with dense rows on {dev}, got {page_table.dtype} '
+                         f'{tuple(page_table.shape)} on {page_table.device}')
+    if lens.numel() != b:
+        raise ValueError(f'lens: expected {b}, got {lens.numel()}')
+    if out is None:
+        out = torch.empty((b, h, d), dtype=q.dtype, device=dev)
+    elif out.shape != (b, h, d) or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError(f'out: expected a contiguous {q.dtype} [{b}, {h}, {d}] on {dev}')
+    lse = torch.empty((b, h), dtype=torch.float32, device=dev) if return_lse else None
+    width, kv = page_table.shape[1], cache.layer_ptrs[layer]
+    with _on(dev):
+        need = lib.kairos_paged_attention_workspace_bytes(kv, b, h, width)
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None    # this call's own: see the header
+        check(lib.kairos_paged_attention(q.data_ptr(), _Two(q.stride(0) if b > 1 else 0, q.stride(1) if h > 1 else 0), kv,
+                                         page_table.data_ptr(), page_table.stride(0) if b > 1 else width, width,
+                                         _index(lens, torch.int32, dev, 'lens'), out.data_ptr(),
+                                         None if lse is None else lse.data_ptr(), b, h,
+                                         d ** -0.5 if scale is None else float(scale), _FLOATS[q.dtype],
+                                         None if ws is None else ws.data_ptr(), need, stream_ptr()), 'paged_attention')
+    return (out, lse) if return_lse else out
