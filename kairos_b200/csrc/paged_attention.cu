@@ -27,15 +27,13 @@ namespace kairos {
 int* device_status_word();   // api.cu
 
 constexpr int kWarps = 4;
-constexpr int kSub = 16;                    // positions per warp stage
-constexpr int kTile = kSub * kWarps;        // positions per scheduling tile
 constexpr float kLift = 14.f;               // weights are kept times 2^14: fp16's smallest step is then 2^-38 of the largest weight
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnShape {
     long long qb, qh, table_stride;
     int B, H, group, blocks_per_kv;         // head blocks (of 8 or 16 query heads) per kv head
-    int table_width, workers, min_tiles;
+    int table_width, workers, joins;        // joins == 0: no pair is ever cut
     float scale_log2;
 };
 
@@ -44,38 +42,59 @@ __device__ __forceinline__ int seq_len(const int* lens, int b, int most) { retur
 
 struct Cut {
     unsigned total, run;                    // tiles of all pairs, tiles per worker
-    int b, pair, tile;                      // where tile `x` lies: sequence, pair (kv head, head block) and tile of it
+    int b, pair, tile;                      // where flat tile `x` lies: sequence, pair (kv head, head block) and tile of it
     int tiles;                              // tiles of that sequence
     unsigned pair_first;                    // flat index of that pair's first tile
 };
 
-// Block-wide (128 threads): scan of the sequences' tile counts, then the place of flat tile x (x < total).  `x` is
-// computed from the totals by `at`.
-template <typename At>
-__device__ __forceinline__ bool locate(const int* lens, const AttnShape& p, int pairs, int most, At at, Cut* out) {
-    __shared__ unsigned warp_sum[kWarps];
+// Tiles that a block may take over what an even cut gives it before cutting pays: a join costs about as long as a block
+// needs for so many tiles.
+constexpr unsigned kSpare = 6;
+
+// Block-wide (128 threads).  Scans the sequences' tile counts and finds, for this block, the flat tile x:
+//   kMain: where worker blockIdx.x begins; returns false where it has no work.  If every pair is short -- no more than
+//     kSpare tiles over the even run -- and there are no more pairs than workers, a worker takes one whole pair (run = 0);
+//   !kMain: the boundary behind worker blockIdx.x's run; returns false where there is none.
+template <int kTile, bool kMain>
+__device__ __forceinline__ bool locate(const int* lens, const AttnShape& p, int pairs, int most, Cut* out) {
+    __shared__ unsigned warp_sum[kWarps], warp_top[kWarps];
     __shared__ Cut found;
     const int tid = threadIdx.x, per = (p.B + 127) >> 7;
     const int first = tid * per, last = min(p.B, first + per);
-    unsigned mine = 0;
-    for (int b = first; b < last; ++b) mine += (unsigned)(seq_len(lens, b, most) + kTile - 1) / kTile;
+    unsigned mine = 0, top = 0;
+    for (int b = first; b < last; ++b) {
+        const unsigned n = (unsigned)(seq_len(lens, b, most) + kTile - 1) / kTile;
+        mine += n;
+        top = max(top, n);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
     unsigned upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
         if ((tid & 31) >= o) upto += v;
     }
-    if ((tid & 31) == 31) warp_sum[tid >> 5] = upto;
+    if ((tid & 31) == 31) warp_sum[tid >> 5] = upto, warp_top[tid >> 5] = top;
     __syncthreads();
     unsigned total = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
         if (w < (tid >> 5)) upto += warp_sum[w];
         total += warp_sum[w];
+        top = max(top, warp_top[w]);
     }
     total *= pairs;
-    const unsigned run = max((unsigned)p.min_tiles, (total + p.workers - 1) / p.workers);
-    const unsigned x = at(run);
+    const unsigned run = (total + p.workers - 1) / p.workers;
+    const bool whole = !p.joins || (top <= run + kSpare && (long long)p.B * pairs <= p.workers);
+    if (whole) {
+        if (!kMain) return false;
+        const int b = blockIdx.x / pairs;
+        if (b >= p.B) return false;
+        const int n = (seq_len(lens, b, most) + kTile - 1) / kTile;
+        *out = Cut{total, 0, b, (int)(blockIdx.x - b * pairs), 0, n, 0};
+        return n > 0;
+    }
+    const unsigned x = (blockIdx.x + (kMain ? 0 : 1)) * run;
     if (x >= total) return false;           // the same for every thread
     unsigned before = upto - mine;
     if (x >= before * pairs && x < upto * pairs) {
@@ -105,6 +124,9 @@ struct Partials {
 // ---- instructions -------------------------------------------------------------------------------------------
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -148,6 +170,15 @@ __device__ __forceinline__ void split(__nv_bfloat16, float x, float y, uint32_t*
     *lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
+__device__ __forceinline__ void put4(__half* to, const float4& v, float f) {
+    __half2 h[2] = {__floats2half2_rn(v.x * f, v.y * f), __floats2half2_rn(v.z * f, v.w * f)};
+    *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(h);
+}
+__device__ __forceinline__ void put4(__nv_bfloat16* to, const float4& v, float f) {
+    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v.x * f, v.y * f), __floats2bfloat162_rn(v.z * f, v.w * f)};
+    *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(h);
+}
+
 // Codes as fp16 pairs, exactly.  bytes 0, 1 -> first, 2, 3 -> second.
 struct WidenI8 {      // 1024 + (code + 128) has the shifted code in its low byte
     static __device__ __forceinline__ void run(uint32_t w, uint32_t* first, uint32_t* second) {
@@ -176,42 +207,42 @@ __device__ __forceinline__ uint32_t place(int r, int c) {
     else return r * ROWB + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
-template <int ROWB, bool kCoded>
+// A warp's ring.  A stage holds 16 positions, 32 where rows are short: the work per stage that does not depend on its
+// size (page look-up, maximum over lanes, rescaling) is then spread over more of them.
+template <int D, bool kCoded>
 struct Ring {
-    static constexpr int kRows = kSub * ROWB;
+    static constexpr int kRowBytes = kCoded ? D : 2 * D;
+    static constexpr int kChunks = kRowBytes / 16;
+    static constexpr int kSub = kCoded || kRowBytes < 256 ? 32 : 16;
+    static constexpr int kTile = kSub * kWarps;                                // positions per scheduling tile
+    static constexpr int kRows = kSub * kRowBytes;
     static constexpr int kStage = 2 * kRows + (kCoded ? 2 * kSub * 4 : 0);
-    // stages a warp: 24 KB and more in flight per warp, and two to four blocks of four warps on an SM
-    static constexpr int kStages = ROWB >= 256 ? 3 : ROWB == 128 ? 4 : 6;
+    static constexpr int kStages = kRowBytes >= 128 ? 3 : 4;
     static constexpr int kBytes = kWarps * kStages * kStage;
+    static constexpr int kBlocksPerSm = kBytes > 112 * 1024 ? 1 : kBytes > 74 * 1024 ? 2 : 3;
+};
+
+// One worker's part of one pair.
+struct Segment {
+    int b, pair, tile, tiles, take, len;
 };
 
 // QT: type of q and o; Widen: void for a cache of type QT, else how codes become fp16; kHalves: 1 (up to 8 query heads in
 // a block) or 2 (16).
 template <typename QT, typename Widen, int D, int kHalves>
-struct Attn {
-    static constexpr bool kCoded = !std::is_void<Widen>::value;
-    using MT = typename std::conditional<kCoded, __half, QT>::type;
-    static constexpr int kRowBytes = kCoded ? D : 2 * D;
-    static constexpr int kChunks = kRowBytes / 16;
-    using R = Ring<kRowBytes, kCoded>;
-    static constexpr int kHeads = 8 * kHalves;
-    static constexpr int kPadRow = D + 8;      // floats: rows of the joining buffer fall on different banks
-    static constexpr int kJoin = kWarps * kHeads * (kPadRow + 2) * 4;
-    static constexpr int kSmem = R::kBytes > kJoin ? R::kBytes : kJoin;
-    static constexpr int kBlocksPerSm = kSmem > 112 * 1024 ? 1 : kSmem > 74 * 1024 ? 2 : kSmem > 54 * 1024 ? 3 : 4;
-};
-
-template <typename QT, typename Widen, int D, int kHalves>
-__global__ void __launch_bounds__(128, (Attn<QT, Widen, D, kHalves>::kBlocksPerSm))
+__global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value>::kBlocksPerSm))
     paged_attention_kernel(const QT* __restrict__ Q, const KvView kv, const int* __restrict__ table, const int* __restrict__ lens,
                            QT* __restrict__ O, float* __restrict__ LSE, float* __restrict__ ws, const AttnShape p, int* status) {
-    using A = Attn<QT, Widen, D, kHalves>;
-    using MT = typename A::MT;
-    using R = typename A::R;
-    constexpr int kTilesN = D / 8;
+    constexpr bool kCoded = !std::is_void<Widen>::value;
+    using MT = typename std::conditional<kCoded, __half, QT>::type;
+    using R = Ring<D, kCoded>;
+    constexpr int kHeads = 8 * kHalves, kSteps = R::kSub / 16, kCols = R::kSub / 8, kTilesN = D / 8, kTile = R::kTile;
+    static_assert(kHeads * D * 4 <= R::kStage, "a warp's output rows fit one stage of its ring");
     extern __shared__ __align__(128) uint8_t smem[];
-    chain_release();
+    __shared__ float jm[kWarps][kHeads], jl[kWarps][kHeads];
+    __shared__ uint32_t jslot[kWarps];
     chain_wait();
+    chain_release();        // what reads this kernel's results waits for all of it; its set-up may begin
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int pairs = kv.heads * p.blocks_per_kv, most = p.table_width << kv.page_shift;
     // sequences without positions have no tile: their rows are written here
@@ -225,72 +256,99 @@ __global__ void __launch_bounds__(128, (Attn<QT, Widen, D, kHalves>::kBlocksPerS
             for (int i = threadIdx.x; i < p.H; i += 128) LSE[(size_t)b * p.H + i] = -INFINITY;
     }
     Cut cut;
-    if (!locate(lens, p, pairs, most, [](unsigned run) { return blockIdx.x * run; }, &cut)) return;
-    const unsigned begin = blockIdx.x * cut.run, end = min(begin + cut.run, cut.total);
-    int b = cut.b, pair = cut.pair, tile = cut.tile, len = seq_len(lens, b, most), tiles = cut.tiles;
+    if (!locate<kTile, true>(lens, p, pairs, most, &cut)) return;
+    // flat tiles still to take: a run of the even cut, or (run == 0) one whole pair
+    unsigned left = cut.run ? min(cut.run, cut.total - blockIdx.x * cut.run) : (unsigned)cut.tiles;
+    Segment seg = {cut.b, cut.pair, cut.tile, cut.tiles, min((int)left, cut.tiles - cut.tile), seq_len(lens, cut.b, most)};
+    bool first_segment = true;
 
     uint8_t* ring = smem + warp * (R::kStages * R::kStage);
     const uint32_t ring_u = smem_u32(ring);
-    for (unsigned x = begin; x < end;) {
-        const int take = min((int)(end - x), tiles - tile);
-        const int head = pair / p.blocks_per_kv, block = pair - head * p.blocks_per_kv;
-        const int q0 = head * p.group + block * A::kHeads;                     // first query head of the block
-        const int rows = min(A::kHeads, p.group - block * A::kHeads);
-        const int k0 = tile * kTile + warp * kSub, k1 = min((tile + take) * kTile, len);   // this warp: k0, k0 + 64, ...
-        const int count = k0 < k1 ? (k1 - k0 + kTile - 1) / kTile : 0;
-        const int* pages = table + (size_t)b * p.table_stride;
-        unsigned bad = 0;                                                      // one bit per stage: page outside the pool
+    const int page_mask = (1 << kv.page_shift) - 1;
+    int slot = 0;                               // ring slot of the next stage to read
+    unsigned bad = 0;                           // per 16 positions of a slot: page outside the pool
+    int k0, k1, count, head;                    // this warp's positions: k0 .. k0 + kSub - 1, then kTile further, below k1
+    const int* pages;
+    int ahead[kSteps];                          // pages of the next stage to request
+    uint32_t qa[D / 16][2 * kHalves];
+    float unit[kHalves];                        // score = product * unit (* scale of the key)
 
-        auto page_of = [&](int i) { return i < count ? __ldcg(pages + ((k0 + i * kTile) >> kv.page_shift)) : 0; };
-        auto issue = [&](int i, int page) {
-            if (i < count) {
-                const int key = k0 + i * kTile, real = min(kSub, k1 - key);
-                const int st = i % R::kStages;
-                const bool ok = (unsigned)page < (unsigned)kv.pages;
-                bad = (bad & ~(1u << st)) | ((ok ? 0u : 1u) << st);
-                if (!ok) *status = KAIROS_ERR_ARG;
-                const size_t row = ((((size_t)(ok ? page : 0)) * kv.heads + head) << kv.page_shift) + (key & ((1 << kv.page_shift) - 1));
-                const uint8_t* ks = static_cast<const uint8_t*>(kv.k) + row * A::kRowBytes;
-                const uint8_t* vs = static_cast<const uint8_t*>(kv.v) + row * A::kRowBytes;
-                const uint32_t dst = ring_u + st * R::kStage;
+    auto look = [&](int i) {
 #pragma unroll
-                for (int n = 0; n < A::kChunks / 2; ++n) {
-                    const int c = lane + 32 * n, r = c / A::kChunks;
-                    cp16(dst + place<A::kRowBytes>(r, c % A::kChunks), ks + c * 16, ok && r < real);
-                }
+        for (int h = 0; h < kSteps; ++h) {
+            const int key = k0 + i * kTile + 16 * h;
+            if (h == 0 || kv.page_shift < 5) ahead[h] = key < k1 ? __ldcg(pages + (key >> kv.page_shift)) : 0;
+            else ahead[h] = ahead[0];
+        }
+    };
+    auto request = [&](int i, int st) {         // stage i of the segment into slot st, from the pages in `ahead`
+        if (i < count) {
+            const uint32_t dst = ring_u + st * R::kStage;
 #pragma unroll
-                for (int n = 0; n < A::kChunks / 2; ++n) {
-                    const int c = lane + 32 * n, r = c / A::kChunks;
-                    cp16(dst + R::kRows + place<A::kRowBytes>(r, c % A::kChunks), vs + c * 16, ok && r < real);
+            for (int h = 0; h < kSteps; ++h) {
+                const int key = k0 + i * kTile + 16 * h, real = k1 - key;
+                const bool ok = (unsigned)ahead[h] < (unsigned)kv.pages;
+                const unsigned bit = 1u << (st * kSteps + h);
+                bad &= ~bit;
+                if (!ok && real > 0) {
+                    bad |= bit;
+                    *status = KAIROS_ERR_ARG;
                 }
-                if constexpr (A::kCoded) {      // lanes 0..3: scales of K, 4..7: of V
-                    if (lane < 8) cp16(dst + 2 * R::kRows + lane * 16, (lane < 4 ? kv.ks : kv.vs) + row + (lane & 3) * 4, ok);
+                const size_t row = (((size_t)(unsigned)(ok ? ahead[h] : 0) * kv.heads + head) << kv.page_shift) + (key & page_mask);
+                const uint8_t* ks = static_cast<const uint8_t*>(kv.k) + row * R::kRowBytes + lane * 16;
+                const uint8_t* vs = static_cast<const uint8_t*>(kv.v) + row * R::kRowBytes + lane * 16;
+                if (ok && real >= 16) {
+#pragma unroll
+                    for (int n = 0; n < R::kChunks / 2; ++n) {
+                        const int c = lane + 32 * n;
+                        cp16(dst + place<R::kRowBytes>(16 * h + c / R::kChunks, c % R::kChunks), ks + 512 * n);
+                        cp16(dst + R::kRows + place<R::kRowBytes>(16 * h + c / R::kChunks, c % R::kChunks), vs + 512 * n);
+                    }
+                } else {                        // rows behind the end, or of no page, are zeros: 0 * weight stays 0
+#pragma unroll
+                    for (int n = 0; n < R::kChunks / 2; ++n) {
+                        const int c = lane + 32 * n, r = c / R::kChunks;
+                        cp16(dst + place<R::kRowBytes>(16 * h + r, c % R::kChunks), ks + 512 * n, ok && r < real);
+                        cp16(dst + R::kRows + place<R::kRowBytes>(16 * h + r, c % R::kChunks), vs + 512 * n, ok && r < real);
+                    }
+                }
+                if constexpr (kCoded) {         // lanes 0..3: scales of K, 4..7: of V
+                    if (lane < 8)
+                        cp16(dst + 2 * R::kRows + (lane >> 2) * (R::kSub * 4) + h * 64 + (lane & 3) * 16,
+                             (lane < 4 ? kv.ks : kv.vs) + row + (lane & 3) * 4, ok && real > 0);
                 }
             }
-            cp_commit();
-        };
-
-        int ahead = page_of(0);
+        }
+        cp_commit();
+    };
+    // Puts a segment's first stages and its queries under way.
+    auto start = [&](const Segment& sg) {
+        head = sg.pair / p.blocks_per_kv;
+        const int block = sg.pair - head * p.blocks_per_kv;
+        const int rows = min(kHeads, p.group - block * kHeads);
+        k0 = sg.tile * kTile + warp * R::kSub;
+        k1 = min((sg.tile + sg.take) * kTile, sg.len);
+        count = k0 < k1 ? (k1 - k0 + kTile - 1) / kTile : 0;
+        pages = table + (size_t)sg.b * p.table_stride;
+        look(0);
+        int st = slot;
 #pragma unroll
         for (int i = 0; i < R::kStages - 1; ++i) {
-            const int page = ahead;
-            ahead = page_of(i + 1);
-            issue(i, page);
+            request(i, st);
+            look(i + 1);
+            st = st + 1 == R::kStages ? 0 : st + 1;
         }
-
         // q as the first operand: rows g (and g + 8) of the block.  For a coded cache the channels of a step are permuted
         // as the code words lie: a thread's four channels are 4 t .. 4 t + 3.
-        uint32_t qa[D / 16][2 * kHalves];
-        float unit[kHalves];                   // score = product * unit (* scale of the key)
 #pragma unroll
         for (int r = 0; r < kHalves; ++r) {
             unit[r] = p.scale_log2;
             const bool real = g + 8 * r < rows;
-            const QT* q = Q + (size_t)b * p.qb + (size_t)(q0 + (real ? g + 8 * r : 0)) * p.qh;
+            const QT* q = Q + (size_t)sg.b * p.qb + (size_t)(head * p.group + block * kHeads + (real ? g + 8 * r : 0)) * p.qh;
 #pragma unroll
             for (int s = 0; s < D / 16; ++s) {
                 uint32_t lo, hi;
-                if constexpr (A::kCoded) {
+                if constexpr (kCoded) {
                     const uint2 w = __ldcg(reinterpret_cast<const uint2*>(q + 16 * s + 4 * t));
                     lo = w.x, hi = w.y;
                 } else {
@@ -300,8 +358,13 @@ __global__ void __launch_bounds__(128, (Attn<QT, Widen, D, kHalves>::kBlocksPerS
                 qa[s][r] = real ? lo : 0u;
                 qa[s][kHalves + r] = real ? hi : 0u;
             }
-            if constexpr (A::kCoded && std::is_same<QT, __nv_bfloat16>::value) {
-                // bf16 rows become fp16 by a power of two of their own: exact to 2^-38 of the row's largest value
+        }
+    };
+    // bf16 rows become fp16 by a power of two of their own: exact to 2^-38 of the row's largest value.
+    auto settle = [&]() {
+        if constexpr (kCoded && std::is_same<QT, __nv_bfloat16>::value) {
+#pragma unroll
+            for (int r = 0; r < kHalves; ++r) {
                 float top = 0.f;
 #pragma unroll
                 for (int s = 0; s < D / 16; ++s)
@@ -325,9 +388,13 @@ __global__ void __launch_bounds__(128, (Attn<QT, Widen, D, kHalves>::kBlocksPerS
                     }
             }
         }
+    };
 
+    start(seg);
+    for (;;) {
+        settle();
         float o[kTilesN][4] = {};
-        float m[kHalves], l[kHalves], vtop = 7.888609052210118e-31f;           // 2^-100
+        float m[kHalves], l[kHalves], vtop = 7.888609052210118e-31f, vinv = 1.2676506002282294e30f;      // 2^-100, 2^100
 #pragma unroll
         for (int r = 0; r < kHalves; ++r) m[r] = -INFINITY, l[r] = 0.f;
 
@@ -335,87 +402,94 @@ __global__ void __launch_bounds__(128, (Attn<QT, Widen, D, kHalves>::kBlocksPerS
         for (int i = 0; i < count; ++i) {
             cp_wait<R::kStages - 2>();
             __syncwarp();                       // every lane's copies have landed; the stage before has been read
-            {
-                const int page = ahead;
-                ahead = page_of(i + R::kStages);
-                issue(i + R::kStages - 1, page);
-            }
-            const int st = i % R::kStages;
-            const uint32_t ku = ring_u + st * R::kStage, vu = ku + R::kRows;
-            const uint8_t* stage = ring + st * R::kStage;
-            const int real = (bad >> st) & 1u ? 0 : min(kSub, k1 - (k0 + i * kTile));
+            request(i + R::kStages - 1, slot == 0 ? R::kStages - 1 : slot - 1);
+            look(i + R::kStages);
+            const uint32_t ku = ring_u + slot * R::kStage, vu = ku + R::kRows;
+            const uint8_t* stage = ring + slot * R::kStage;
+            const int real = k1 - (k0 + i * kTile);
+            const unsigned gone = (bad >> (slot * kSteps)) & ((1u << kSteps) - 1);
+            const bool full = real >= R::kSub && gone == 0;     // the same in all lanes
+            slot = slot + 1 == R::kStages ? 0 : slot + 1;
 
-            // scores of 16 positions: columns 2 t, 2 t + 1 of two 8-wide tiles
-            float s[2][4] = {};
-            if constexpr (!A::kCoded) {
+            // scores: columns 2 t, 2 t + 1 of tiles of 8 positions
+            float s[kCols][4] = {};
+            if constexpr (!kCoded) {
 #pragma unroll
-                for (int c = 0; c < D / 16; ++c) {
-                    uint32_t w[4];
-                    ldsm4(ku + place<A::kRowBytes>((lane & 7) + ((lane >> 4) << 3), 2 * c + ((lane >> 3) & 1)), w);
+                for (int c = 0; c < D / 16; ++c)
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
-                        mma(MT(), s[n], qa[c][0], kHalves == 2 ? qa[c][1] : 0u, qa[c][kHalves], kHalves == 2 ? qa[c][3] : 0u,
-                            w[2 * n], w[2 * n + 1]);
-                }
+                    for (int h = 0; h < kSteps; ++h) {
+                        uint32_t w[4];
+                        ldsm4(ku + place<R::kRowBytes>(16 * h + (lane & 7) + ((lane >> 4) << 3), 2 * c + ((lane >> 3) & 1)), w);
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+                            mma(MT(), s[2 * h + n], qa[c][0], kHalves == 2 ? qa[c][1] : 0u, qa[c][kHalves],
+                                kHalves == 2 ? qa[c][3] : 0u, w[2 * n], w[2 * n + 1]);
+                    }
             } else {
 #pragma unroll
-                for (int c = 0; c < D / 16; c += 2) {
-                    uint32_t w[4];              // two steps of 16 channels x two tiles of 8 positions
-                    ldsm4(ku + place<A::kRowBytes>((lane & 7) + (((lane >> 3) & 1) << 3), c + (lane >> 4)), w);
+                for (int c = 0; c < D / 16; c += 2)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int h = 0; h < kSteps; ++h) {
+                        uint32_t w[4];          // two steps of 16 channels x two tiles of 8 positions
+                        ldsm4(ku + place<R::kRowBytes>(16 * h + (lane & 7) + (((lane >> 3) & 1) << 3), c + (lane >> 4)), w);
 #pragma unroll
-                        for (int n = 0; n < 2; ++n) {
-                            uint32_t b0, b1;
-                            Widen::run(w[2 * h + n], &b0, &b1);
-                            mma(MT(), s[n], qa[c + h][0], kHalves == 2 ? qa[c + h][1] : 0u, qa[c + h][kHalves],
-                                kHalves == 2 ? qa[c + h][3] : 0u, b0, b1);
-                        }
-                }
+                        for (int d = 0; d < 2; ++d)
+#pragma unroll
+                            for (int n = 0; n < 2; ++n) {
+                                uint32_t b0, b1;
+                                Widen::run(w[2 * d + n], &b0, &b1);
+                                mma(MT(), s[2 * h + n], qa[c + d][0], kHalves == 2 ? qa[c + d][1] : 0u, qa[c + d][kHalves],
+                                    kHalves == 2 ? qa[c + d][3] : 0u, b0, b1);
+                            }
+                    }
             }
-            float vs[2][2];                     // scale of V over the largest scale so far
+            float vs[kCols][2];                 // scale of V over the largest scale so far
             float grow = 1.f;
-            float ks[2][2];
-            if constexpr (A::kCoded) {
+            if constexpr (kCoded) {
                 const float* sc = reinterpret_cast<const float*>(stage + 2 * R::kRows);
                 float top = 0.f;
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
+                for (int n = 0; n < kCols; ++n) {
                     const float2 k2 = *reinterpret_cast<const float2*>(sc + 8 * n + 2 * t);
-                    const float2 v2 = *reinterpret_cast<const float2*>(sc + kSub + 8 * n + 2 * t);
-                    ks[n][0] = k2.x, ks[n][1] = k2.y, vs[n][0] = v2.x, vs[n][1] = v2.y;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        if (8 * n + 2 * t + e >= real) vs[n][e] = 0.f;         // may be anything, NaN too
-                        top = fmaxf(top, fabsf(vs[n][e]));
-                    }
+                    const float2 v2 = *reinterpret_cast<const float2*>(sc + R::kSub + 8 * n + 2 * t);
+                    vs[n][0] = v2.x, vs[n][1] = v2.y;
+                    s[n][0] *= k2.x, s[n][1] *= k2.y;
+                    if constexpr (kHalves == 2) s[n][2] *= k2.x, s[n][3] *= k2.y;
                 }
+                if (!full) {                    // scales behind the end may be anything, NaN too
+#pragma unroll
+                    for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (8 * n + 2 * t + e >= real || ((gone >> (n >> 1)) & 1u)) vs[n][e] = 0.f;
+                }
+#pragma unroll
+                for (int n = 0; n < kCols; ++n) top = fmaxf(top, fmaxf(fabsf(vs[n][0]), fabsf(vs[n][1])));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 if (top > vtop) {               // the same in all lanes
                     grow = __fdividef(vtop, top);
                     vtop = top;
+                    vinv = __frcp_rn(top);
                 }
-                const float inv = __frcp_rn(vtop);
-#pragma unroll
-                for (int n = 0; n < 2; ++n) vs[n][0] *= inv, vs[n][1] *= inv;
             }
-            uint32_t pa[2][2 * kHalves];        // [tile][half]: weights, [tile][kHalves + half]: their remainders
+            uint32_t pa[kCols][2 * kHalves];    // [tile][half]: weights, [tile][kHalves + half]: their remainders
             float keep[kHalves];
             bool moved = grow != 1.f;
 #pragma unroll
             for (int r = 0; r < kHalves; ++r) {
                 float top = -INFINITY;
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int n = 0; n < kCols; ++n) s[n][2 * r] *= unit[r], s[n][2 * r + 1] *= unit[r];
+                if (!full) {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float v = s[n][2 * r + e] * unit[r];
-                        if constexpr (A::kCoded) v *= ks[n][e];
-                        v = 8 * n + 2 * t + e < real ? v : -INFINITY;
-                        s[n][2 * r + e] = v;
-                        top = fmaxf(top, v);
-                    }
+                    for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (8 * n + 2 * t + e >= real || ((gone >> (n >> 1)) & 1u)) s[n][2 * r + e] = -INFINITY;
+                }
+#pragma unroll
+                for (int n = 0; n < kCols; ++n) top = fmaxf(top, fmaxf(s[n][2 * r], s[n][2 * r + 1]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 top = fmaxf(top, m[r]);
@@ -423,108 +497,128 @@ __global__ void __launch_bounds__(128, (Attn<QT, Widen, D, kHalves>::kBlocksPerS
                 keep[r] = exp2_fast(m[r] - safe);
                 moved |= top != m[r];
                 m[r] = top;
-                float w[2][2];
+                const float base = safe - kLift;
+                float sum = 0.f;
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) w[n][e] = exp2_fast(s[n][2 * r + e] - safe + kLift);
-                l[r] = __fmaf_rn(l[r], keep[r], (w[0][0] + w[0][1]) + (w[1][0] + w[1][1]));
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    if constexpr (A::kCoded) w[n][0] *= vs[n][0], w[n][1] *= vs[n][1];
-                    split(MT(), w[n][0], w[n][1], &pa[n][r], &pa[n][kHalves + r]);
+                for (int n = 0; n < kCols; ++n) {
+                    float w0 = exp2_fast(s[n][2 * r] - base), w1 = exp2_fast(s[n][2 * r + 1] - base);
+                    sum += w0 + w1;
+                    if constexpr (kCoded) w0 *= vs[n][0] * vinv, w1 *= vs[n][1] * vinv;
+                    split(MT(), w0, w1, &pa[n][r], &pa[n][kHalves + r]);
                 }
+                l[r] = __fmaf_rn(l[r], keep[r], sum);
             }
             if (__any_sync(0xffffffffu, moved)) {
                 const float f0 = keep[0] * grow, f1 = (kHalves == 2 ? keep[kHalves - 1] : keep[0]) * grow;
 #pragma unroll
                 for (int j = 0; j < kTilesN; ++j) o[j][0] *= f0, o[j][1] *= f0, o[j][2] *= f1, o[j][3] *= f1;
             }
-            // o += weights . V.  kHalves == 1: rows 8..15 are the remainders of rows 0..7; 2: a second product
-            auto weigh = [&](float (&acc)[4], uint32_t b0, uint32_t b1) {
-                if constexpr (kHalves == 1) {
-                    mma(MT(), acc, pa[0][0], pa[0][1], pa[1][0], pa[1][1], b0, b1);
-                } else {
-                    mma(MT(), acc, pa[0][0], pa[0][1], pa[1][0], pa[1][1], b0, b1);
-                    mma(MT(), acc, pa[0][2], pa[0][3], pa[1][2], pa[1][3], b0, b1);
-                }
+            // o += weights . V of step h.  kHalves == 1: rows 8..15 are the remainders of rows 0..7; 2: a second product
+            auto weigh = [&](int h, float (&acc)[4], uint32_t b0, uint32_t b1) {
+                const uint32_t(&x)[2 * kHalves] = pa[2 * h];
+                const uint32_t(&y)[2 * kHalves] = pa[2 * h + 1];
+                mma(MT(), acc, x[0], x[1], y[0], y[1], b0, b1);
+                if constexpr (kHalves == 2) mma(MT(), acc, x[2], x[3], y[2], y[3], b0, b1);
             };
-            if constexpr (!A::kCoded) {
 #pragma unroll
-                for (int c = 0; c < D / 16; ++c) {
-                    uint32_t w[4];
-                    ldsm4t(vu + place<A::kRowBytes>(lane & 15, 2 * c + (lane >> 4)), w);
-                    weigh(o[2 * c], w[0], w[1]);
-                    weigh(o[2 * c + 1], w[2], w[3]);
-                }
-            } else {
-                // column n of tile j is channel n * D / 8 + j: a thread's bytes of a row are D / 8 neighbours
-                constexpr int kWords = D / 32 < 4 ? D / 32 : 4;        // words per access: 2 (8 bytes) or 4 (16 bytes)
+            for (int h = 0; h < kSteps; ++h) {
+                if constexpr (!kCoded) {
 #pragma unroll
-                for (int c = 0; c < D / 8 / (4 * kWords); ++c) {
-                    uint32_t x[4][kWords];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int key = 2 * t + (k & 1) + ((k >> 1) << 3), byte = g * (D / 8) + c * 16;
-                        const uint8_t* from = stage + R::kRows + place<A::kRowBytes>(key, byte >> 4) + (byte & 15);
-                        if constexpr (kWords == 4) *reinterpret_cast<uint4*>(x[k]) = *reinterpret_cast<const uint4*>(from);
-                        else *reinterpret_cast<uint2*>(x[k]) = *reinterpret_cast<const uint2*>(from);
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t w[4];
+                        ldsm4t(vu + place<R::kRowBytes>(16 * h + (lane & 15), 2 * c + (lane >> 4)), w);
+                        weigh(h, o[2 * c], w[0], w[1]);
+                        weigh(h, o[2 * c + 1], w[2], w[3]);
                     }
+                } else {
+                    // column n of tile j is channel n * D / 8 + j: a thread's bytes of a row are D / 8 neighbours
+                    constexpr int kWords = D / 32 < 4 ? D / 32 : 4;    // words per access: 2 (8 bytes) or 4 (16 bytes)
 #pragma unroll
-                    for (int w = 0; w < kWords; ++w) {
-                        uint32_t lo[4], hi[4];                          // tiles 4 w .. 4 w + 3: positions 2 t, 2 t + 1 and 8 further
-                        Widen::run(__byte_perm(x[0][w], x[1][w], 0x5140), &lo[0], &lo[1]);
-                        Widen::run(__byte_perm(x[0][w], x[1][w], 0x7362), &lo[2], &lo[3]);
-                        Widen::run(__byte_perm(x[2][w], x[3][w], 0x5140), &hi[0], &hi[1]);
-                        Widen::run(__byte_perm(x[2][w], x[3][w], 0x7362), &hi[2], &hi[3]);
+                    for (int c = 0; c < D / 8 / (4 * kWords); ++c) {
+                        uint32_t x[4][kWords];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) weigh(o[(c * kWords + w) * 4 + e], lo[e], hi[e]);
+                        for (int k = 0; k < 4; ++k) {
+                            const int key = 16 * h + 2 * t + (k & 1) + ((k >> 1) << 3), byte = g * (D / 8) + c * 16;
+                            const uint8_t* from = stage + R::kRows + place<R::kRowBytes>(key, byte >> 4) + (byte & 15);
+                            if constexpr (kWords == 4) *reinterpret_cast<uint4*>(x[k]) = *reinterpret_cast<const uint4*>(from);
+                            else *reinterpret_cast<uint2*>(x[k]) = *reinterpret_cast<const uint2*>(from);
+                        }
+#pragma unroll
+                        for (int w = 0; w < kWords; ++w) {
+                            uint32_t lo[4], hi[4];      // tiles 4 w .. 4 w + 3: positions 2 t, 2 t + 1 and 8 further
+                            Widen::run(__byte_perm(x[0][w], x[1][w], 0x5140), &lo[0], &lo[1]);
+                            Widen::run(__byte_perm(x[0][w], x[1][w], 0x7362), &lo[2], &lo[3]);
+                            Widen::run(__byte_perm(x[2][w], x[3][w], 0x5140), &hi[0], &hi[1]);
+                            Widen::run(__byte_perm(x[2][w], x[3][w], 0x7362), &hi[2], &hi[3]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) weigh(h, o[(c * kWords + w) * 4 + e], lo[e], hi[e]);
+                        }
                     }
                 }
             }
         }
-        cp_wait<0>();
 
-        // ---- the four warps' parts of the segment become one ------------------------------------------------
-        __syncthreads();                        // all rings are read
-        float* jo = reinterpret_cast<float*>(smem);                            // [warp][head][kPadRow]
-        float* jm = jo + kWarps * A::kHeads * A::kPadRow;                      // [warp][head] maximum, then sum
-        float* jl = jm + kWarps * A::kHeads;
+        // ---- the next segment's first stages are requested before this one's parts are joined ----------------
+        const Segment done = seg;
+        const bool first = first_segment;
+        left -= done.take;
+        const uint32_t free_slot = slot == 0 ? R::kStages - 1 : slot - 1;      // the one slot that start() leaves alone
+        __syncwarp();                           // every lane has read the last stage
+        if (left) {
+            if (++seg.pair == pairs) {
+                seg.pair = 0;
+                do seg.len = seq_len(lens, ++seg.b, most); while (seg.len == 0);
+                seg.tiles = (seg.len + kTile - 1) / kTile;
+            }
+            seg.tile = 0;
+            seg.take = min((int)left, seg.tiles);
+            first_segment = false;
+            start(seg);
+        }
+
+        // ---- the four warps' parts become one: each leaves its rows in a slot of its ring.  Column c of row r lies at
+        // c ^ 8 (r % 8) ^ 4 (c / 32 % 8): the lanes of a store fall on different banks
+        auto at = [](int r, int c) { return r * D + (c ^ ((r & 7) << 3) ^ (((c >> 5) & 7) << 2)); };
+        float* mine = reinterpret_cast<float*>(ring + free_slot * R::kStage);
+        if (lane == 0) jslot[warp] = (uint32_t)(warp * R::kStages + free_slot) * R::kStage;
 #pragma unroll
         for (int r = 0; r < kHalves; ++r) {
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            const int row = warp * A::kHeads + g + 8 * r;
-            if (t == 0) jm[row] = m[r], jl[row] = l[r];
-            float* to = jo + row * A::kPadRow;
+            const int row = g + 8 * r;
+            if (t == 0) jm[warp][row] = m[r], jl[warp][row] = l[r];
+            auto value = [&](int j, int e) { return kHalves == 1 ? o[j][e] + o[j][2 + e] : o[j][2 * r + e]; };
+            if constexpr (kCoded) {
 #pragma unroll
-            for (int j = 0; j < kTilesN; ++j) {
-                float x = o[j][2 * r], y = o[j][2 * r + 1];
-                if constexpr (kHalves == 1) x += o[j][2], y += o[j][3];
-                if constexpr (A::kCoded) {
-                    to[2 * t * (D / 8) + j] = x * vtop;
-                    to[(2 * t + 1) * (D / 8) + j] = y * vtop;
-                } else {
-                    *reinterpret_cast<float2*>(to + 8 * j + 2 * t) = make_float2(x, y);
-                }
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int j = 0; j < kTilesN; j += 4)
+                        *reinterpret_cast<float4*>(mine + at(row, (2 * t + e) * (D / 8) + j)) =
+                            make_float4(value(j, e) * vtop, value(j + 1, e) * vtop, value(j + 2, e) * vtop, value(j + 3, e) * vtop);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kTilesN; ++j)
+                    *reinterpret_cast<float2*>(mine + at(row, 8 * j + 2 * t)) = make_float2(value(j, 0), value(j, 1));
             }
         }
         __syncthreads();
-        const bool whole = take == tiles;
-        const unsigned slot = 2 * blockIdx.x + (x == begin ? 0 : 1);
+        const int dhead = done.pair / p.blocks_per_kv, dblock = done.pair - dhead * p.blocks_per_kv;
+        const int q0 = dhead * p.group + dblock * kHeads, rows = min(kHeads, p.group - dblock * kHeads);
+        const bool whole = done.take == done.tiles;
+        const unsigned part = 2 * blockIdx.x + (first ? 0 : 1);
         for (int i = threadIdx.x; i < rows * (D / 4); i += 128) {
-            const int row = i / (D / 4), c = i - row * (D / 4);
+            const int row = i / (D / 4), c = 4 * (i - row * (D / 4));
             float top = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, jm[w * A::kHeads + row]);
+            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, jm[w][row]);
             const float safe = top == -INFINITY ? 0.f : top;
             float sum = 0.f;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const float f = exp2_fast(jm[w * A::kHeads + row] - safe);
-                const float4 v = *reinterpret_cast<const float4*>(jo + (w * A::kHeads + row) * A::kPadRow + 4 * c);
-                sum = __fmaf_rn(f, jl[w * A::kHeads + row], sum);
+                const float f = exp2_fast(jm[w][row] - safe);
+                const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + jslot[w]) + at(row, c));
+                sum = __fmaf_rn(f, jl[w][row], sum);
                 acc.x = __fmaf_rn(f, v.x, acc.x);
                 acc.y = __fmaf_rn(f, v.y, acc.y);
                 acc.z = __fmaf_rn(f, v.z, acc.z);
@@ -532,43 +626,35 @@ __global__ void __launch_bounds__(128, (Attn<QT, Widen, D, kHalves>::kBlocksPerS
             }
             if (whole) {
                 const float inv = __fdiv_rn(1.f, sum);
-                const size_t at = (size_t)b * p.H + q0 + row;
-                QT* to = O + at * D + 4 * c;
-                put(to, acc.x * inv);
-                put(to + 1, acc.y * inv);
-                put(to + 2, acc.z * inv);
-                put(to + 3, acc.w * inv);
-                if (LSE && c == 0) LSE[at] = (top + __log2f(sum) - kLift) * kLn2;
+                const size_t to = (size_t)done.b * p.H + q0 + row;
+                put4(O + to * D + c, acc, inv);
+                if (LSE && c == 0) LSE[to] = (top + __log2f(sum) - kLift) * kLn2;
             } else {
-                *reinterpret_cast<float4*>(Partials<A::kHeads, D>::o(ws, slot) + row * D + 4 * c) = acc;
-                if (c == 0) *reinterpret_cast<float2*>(Partials<A::kHeads, D>::ml(ws, slot) + 2 * row) = make_float2(top, sum);
+                *reinterpret_cast<float4*>(Partials<kHeads, D>::o(ws, part) + row * D + c) = acc;
+                if (c == 0) *reinterpret_cast<float2*>(Partials<kHeads, D>::ml(ws, part) + 2 * row) = make_float2(top, sum);
             }
         }
-        __syncthreads();                        // the buffer is a ring again
-
-        x += take;
-        tile = 0;
-        if (x < end && ++pair == pairs) {
-            pair = 0;
-            do len = seq_len(lens, ++b, most); while (len == 0);
-            tiles = (len + kTile - 1) / kTile;
-        }
+        if (!left) break;
+        __syncthreads();                        // the slots belong to the rings again
     }
 }
 
 // Block w looks at the boundary between the runs of workers w and w + 1.  Where a pair lies across it and no earlier
 // boundary, its partial results (workers w, w + 1, ... up to the one that holds its last tile) are joined here; the
 // channels are spread over gridDim.y.
-template <typename QT, int D, int kHeads>
+template <typename QT, int D, int kHeads, int kTile>
 __global__ void __launch_bounds__(128) paged_attention_join_kernel(const KvView kv, const int* __restrict__ lens, QT* __restrict__ O,
                                                                    float* __restrict__ LSE, float* __restrict__ ws,
                                                                    const AttnShape p) {
     using P = Partials<kHeads, D>;
-    chain_release();
-    chain_wait();
+    // The lengths were there before the kernel whose parts are joined began (it lets this one start only after its own
+    // wait), so the place is found while that kernel still runs.
     const int pairs = kv.heads * p.blocks_per_kv;
     Cut cut;
-    if (!locate(lens, p, pairs, p.table_width << kv.page_shift, [](unsigned run) { return (blockIdx.x + 1) * run; }, &cut)) return;
+    const bool some = locate<kTile, false>(lens, p, pairs, p.table_width << kv.page_shift, &cut);
+    chain_wait();
+    chain_release();
+    if (!some) return;
     const unsigned x = (blockIdx.x + 1) * cut.run, first = cut.pair_first;
     if (first >= x || first < x - cut.run) return;      // a pair begins here, or lay across an earlier boundary already
     const unsigned last = (first + cut.tiles - 1) / cut.run;
@@ -595,11 +681,7 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const KvView 
         }
         const float inv = __fdiv_rn(1.f, sum);
         const size_t at = (size_t)cut.b * p.H + head * p.group + block * kHeads + row;
-        QT* to = O + at * D + 4 * c;
-        put(to, acc.x * inv);
-        put(to + 1, acc.y * inv);
-        put(to + 2, acc.z * inv);
-        put(to + 3, acc.w * inv);
+        put4(O + at * D + 4 * c, acc, inv);
         if (LSE && c == 0) LSE[at] = (top + __log2f(sum) - kLift) * kLn2;
     }
 }
@@ -619,20 +701,9 @@ static int sm_count() {
 
 struct Plan {
     int heads_per_block, blocks_per_kv, workers;
-    long long most_tiles;      // were every sequence as long as the table allows
     bool joins;
     size_t bytes;
 };
-
-// Blocks per SM of the variant that serves (cache type, head dim, head block): what its shared memory leaves room for.
-static int blocks_per_sm(const KvView& kv, bool coded, int heads) {
-    const bool wide = heads == 16;
-#define KAIROS_OCC(D) \
-    (coded ? (wide ? Attn<__half, WidenI8, D, 2>::kBlocksPerSm : Attn<__half, WidenI8, D, 1>::kBlocksPerSm) \
-           : (wide ? Attn<__half, void, D, 2>::kBlocksPerSm : Attn<__half, void, D, 1>::kBlocksPerSm))
-    return kv.dim == 64 ? KAIROS_OCC(64) : kv.dim == 128 ? KAIROS_OCC(128) : KAIROS_OCC(256);
-#undef KAIROS_OCC
-}
 
 static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width, Plan* out) {
     const int sms = sm_count();
@@ -640,12 +711,20 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
     const int group = H / kv.heads;
     out->heads_per_block = group > 8 ? 16 : 8;
     out->blocks_per_kv = (group + out->heads_per_block - 1) / out->heads_per_block;
-    const long long per_pair = (((long long)table_width << kv.page_shift) + kTile - 1) / kTile;
-    out->most_tiles = per_pair * B * kv.heads * out->blocks_per_kv;
-    if (out->most_tiles > 0x7fffffffLL) return KAIROS_ERR_SHAPE;
-    const int full = sms * blocks_per_sm(kv, coded, out->heads_per_block);
-    out->workers = (int)max(1LL, min((long long)full, out->most_tiles));
-    out->joins = per_pair > 1 && out->workers > 1;
+    int tile = 0, per_sm = 0;
+#define KAIROS_RING(D)                                                                                (tile = coded ? Ring<D, true>::kTile : Ring<D, false>::kTile,                                       per_sm = coded ? Ring<D, true>::kBlocksPerSm : Ring<D, false>::kBlocksPerSm)
+    if (kv.dim == 64) KAIROS_RING(64);
+    else if (kv.dim == 128) KAIROS_RING(128);
+    else KAIROS_RING(256);
+#undef KAIROS_RING
+    const long long per_pair = (((long long)table_width << kv.page_shift) + tile - 1) / tile;
+    const long long pairs = (long long)B * kv.heads * out->blocks_per_kv;
+    if (per_pair * pairs > 0x7fffffffLL) return KAIROS_ERR_SHAPE;
+    const int full = sms * per_sm;
+    // No pair is cut where there are workers for all of them and none can be longer than a join is worth; otherwise the
+    // device decides by the lengths.
+    out->joins = !(pairs <= full && per_pair <= (long long)kSpare + 1);
+    out->workers = (int)max(1LL, out->joins ? min((long long)full, per_pair * pairs) : pairs);
     out->bytes = out->joins ? (size_t)2 * out->workers * out->heads_per_block * (kv.dim + 2) * 4 : 0;
     return KAIROS_OK;
 }
@@ -653,19 +732,19 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
 template <typename QT, typename Widen, int D, int kHalves>
 static int run_attention(const void* Q, const KvView& kv, const void* table, const void* lens, void* O, void* LSE, void* ws,
                          const AttnShape& p, const Plan& plan, int* status, cudaStream_t st) {
-    using A = Attn<QT, Widen, D, kHalves>;
+    using R = Ring<D, !std::is_void<Widen>::value>;
     static PerDeviceFlag flag;
     auto kernel = paged_attention_kernel<QT, Widen, D, kHalves>;
-    const int rc = ensure_dynamic_smem(flag, kernel, A::kSmem);
+    const int rc = ensure_dynamic_smem(flag, kernel, R::kBytes);
     if (rc != KAIROS_OK) return rc;
-    cudaError_t e = launch_chained(kernel, dim3(plan.workers), dim3(128), A::kSmem, st, static_cast<const QT*>(Q), kv,
+    cudaError_t e = launch_chained(kernel, dim3(plan.workers), dim3(128), R::kBytes, st, static_cast<const QT*>(Q), kv,
                                    static_cast<const int*>(table), static_cast<const int*>(lens), static_cast<QT*>(O),
                                    static_cast<float*>(LSE), static_cast<float*>(ws), p, status);
     if (e != cudaSuccess) return note_cuda_error(e);
-    if (plan.joins) {
+    if (plan.joins && plan.workers > 1) {
         // few pairs: few joins of many parts each, so the channels of one are spread over several blocks
         const int slices = (long long)p.B * kv.heads * p.blocks_per_kv < 64 ? 4 : 1;
-        e = launch_chained(paged_attention_join_kernel<QT, D, A::kHeads>, dim3(plan.workers - 1, slices), dim3(128), 0, st, kv,
+        e = launch_chained(paged_attention_join_kernel<QT, D, 8 * kHalves, R::kTile>, dim3(plan.workers - 1, slices), dim3(128), 0, st, kv,
                            static_cast<const int*>(lens), static_cast<QT*>(O), static_cast<float*>(LSE), static_cast<float*>(ws), p);
         if (e != cudaSuccess) return note_cuda_error(e);
     }
@@ -720,7 +799,7 @@ extern "C" int kairos_paged_attention(const void* Q, const long long* q_strides,
     int* status = device_status_word();
     if (!status) return KAIROS_ERR_CUDA;
     const AttnShape p = {q_strides[0], q_strides[1], table_stride, B, H, H / kv.heads, plan.blocks_per_kv, table_width,
-                         plan.workers, 2, scale * kLog2e};
+                         plan.workers, plan.joins ? 1 : 0, scale * kLog2e};
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (dtype == KAIROS_DTYPE_F16) {
         if (layer->dtype == KAIROS_DTYPE_I8) return pick_attention<__half, WidenI8>(Q, kv, page_table, lens, O, LSE, workspace, p, plan, status, st);
