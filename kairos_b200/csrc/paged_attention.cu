@@ -8,16 +8,19 @@
 // a byte, so HBM sets the pace and everything here serves to keep loads in flight:
 //   * a warp owns a ring of stages of 16 positions (K rows and V rows, 4 KB for 128 channels in fp16 each), filled by
 //     16-byte cp.async; no block-wide barrier until a segment ends;
-//   * the heads that share a kv head are the rows of warp-level tensor instructions (m16n8k16), so a key is read from
-//     shared memory once for all of them.  tcgen05 has no use here: its smallest tile is 64 or 128 rows, 8 to 32 times the
-//     heads there are, and the tensor work is a tenth of what mma.sync gives;
+//   * the heads that share a kv head are the eight columns of warp-level tensor instructions (m16n8k16): scores^T = K q^T
+//     (16 positions a step) and o^T = V^T w^T (16 channels), so a key is read from shared memory once for all of them and
+//     no row of a product is empty.  tcgen05 has no use here: its smallest tile is 64 or 128 rows by 8 columns from
+//     shared memory, where coded values would have to be written back first, and the tensor work is a tenth of what
+//     mma.sync gives;
 //   * the work is cut on the device: all (sequence, kv head) pairs laid end to end in tiles of 64 positions, every block
 //     takes an equal run of tiles, whatever the lengths are.  A pair that lies across blocks leaves one partial result per
 //     block in the workspace and a second kernel joins them, in the order of the blocks (no atomics: same bits every run).
 //
 // Precision.  Scores, maxima, sums and outputs are fp32.  The weights enter the second product as TWO 16-bit numbers
-// (value and remainder), which costs nothing for up to eight heads: the remainders are the eight rows of the tile that
-// would be empty.  Rounding weights to 16 bits alone would add an error as large as the output's own rounding.
+// (value and remainder): rounding them to 16 bits alone would add an error as large as the output's own rounding.
+// The reference m of the exponent need not be the maximum: it moves (and o and l are rescaled) only when a score
+// passes it by 2^kSlack, so most stages need neither a reduction over lanes nor a rescaling.
 #include <type_traits>
 
 #include "paged_kv.cuh"
@@ -27,7 +30,9 @@ namespace kairos {
 int* device_status_word();   // api.cu
 
 constexpr int kWarps = 4;
-constexpr float kLift = 14.f;               // weights are kept times 2^14: fp16's smallest step is then 2^-38 of the largest weight
+// Weights are kept times 2^kLift and pass the reference by 2^kSlack at the most; with a V scale of up to twice the largest
+// so far they stay below 2^15, and fp16's smallest step is 2^-30 of a weight at the reference.
+constexpr float kLift = 6.f, kSlack = 8.f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnShape {
@@ -154,6 +159,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Transposes an 8 x 8 matrix of 16-bit values held as ldmatrix delivers it.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 // Two fp32 as a pair of 16-bit values, and the pair of what the rounding left.
 __device__ __forceinline__ void split(__half, float x, float y, uint32_t* hi, uint32_t* lo) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -207,19 +218,19 @@ __device__ __forceinline__ uint32_t place(int r, int c) {
     else return r * ROWB + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
-// A warp's ring.  A stage holds 16 positions, 32 where rows are short: the work per stage that does not depend on its
-// size (page look-up, maximum over lanes, rescaling) is then spread over more of them.
-template <int D, bool kCoded>
+// A warp's ring.  A stage holds 16 or 32 positions; a warp's output rows have to fit one (see the joining of warps).
+template <int D, bool kCoded, int kHalves>
 struct Ring {
     static constexpr int kRowBytes = kCoded ? D : 2 * D;
     static constexpr int kChunks = kRowBytes / 16;
-    static constexpr int kSub = kCoded || kRowBytes < 256 ? 32 : 16;
+    static constexpr int kSub = kRowBytes >= 256 && !kCoded ? 16 : kHalves == 1 && D == 128 ? 16 : 32;
     static constexpr int kTile = kSub * kWarps;                                // positions per scheduling tile
     static constexpr int kRows = kSub * kRowBytes;
     static constexpr int kStage = 2 * kRows + (kCoded ? 2 * kSub * 4 : 0);
     static constexpr int kStages = kRowBytes >= 128 ? 3 : 4;
     static constexpr int kBytes = kWarps * kStages * kStage;
-    static constexpr int kBlocksPerSm = kBytes > 112 * 1024 ? 1 : kBytes > 74 * 1024 ? 2 : 3;
+    static constexpr int kBlocksPerSm = kBytes > 112 * 1024 ? 1 : kBytes > 74 * 1024 ? 2 : kBytes > 55 * 1024 ? 3 : 4;
+    static_assert(8 * kHalves * D * 4 <= kStage, "a warp's output rows fit one stage of its ring");
 };
 
 // One worker's part of one pair.
@@ -230,14 +241,13 @@ struct Segment {
 // QT: type of q and o; Widen: void for a cache of type QT, else how codes become fp16; kHalves: 1 (up to 8 query heads in
 // a block) or 2 (16).
 template <typename QT, typename Widen, int D, int kHalves>
-__global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value>::kBlocksPerSm))
+__global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHalves>::kBlocksPerSm))
     paged_attention_kernel(const QT* __restrict__ Q, const KvView kv, const int* __restrict__ table, const int* __restrict__ lens,
                            QT* __restrict__ O, float* __restrict__ LSE, float* __restrict__ ws, const AttnShape p, int* status) {
     constexpr bool kCoded = !std::is_void<Widen>::value;
     using MT = typename std::conditional<kCoded, __half, QT>::type;
-    using R = Ring<D, kCoded>;
-    constexpr int kHeads = 8 * kHalves, kSteps = R::kSub / 16, kCols = R::kSub / 8, kTilesN = D / 8, kTile = R::kTile;
-    static_assert(kHeads * D * 4 <= R::kStage, "a warp's output rows fit one stage of its ring");
+    using R = Ring<D, kCoded, kHalves>;
+    constexpr int kHeads = 8 * kHalves, kSteps = R::kSub / 16, kTile = R::kTile;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float jm[kWarps][kHeads], jl[kWarps][kHeads];
     __shared__ uint32_t jslot[kWarps];
@@ -270,8 +280,8 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value>::kB
     int k0, k1, count, head;                    // this warp's positions: k0 .. k0 + kSub - 1, then kTile further, below k1
     const int* pages;
     int ahead[kSteps];                          // pages of the next stage to request
-    uint32_t qa[D / 16][2 * kHalves];
-    float unit[kHalves];                        // score = product * unit (* scale of the key)
+    uint32_t qb[D / 16][2 * kHalves];
+    float unit[kHalves][2];                     // score = product * unit (* scale of the key), heads 2 t and 2 t + 1 (+ 8)
 
     auto look = [&](int i) {
 #pragma unroll
@@ -338,11 +348,11 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value>::kB
             look(i + 1);
             st = st + 1 == R::kStages ? 0 : st + 1;
         }
-        // q as the first operand: rows g (and g + 8) of the block.  For a coded cache the channels of a step are permuted
-        // as the code words lie: a thread's four channels are 4 t .. 4 t + 3.
+        // q as the second operand: head g (and g + 8).  For a coded cache the channels of a step are permuted as the code
+        // words lie: a thread's four channels are 4 t .. 4 t + 3.
 #pragma unroll
         for (int r = 0; r < kHalves; ++r) {
-            unit[r] = p.scale_log2;
+            unit[r][0] = unit[r][1] = p.scale_log2;
             const bool real = g + 8 * r < rows;
             const QT* q = Q + (size_t)sg.b * p.qb + (size_t)(head * p.group + block * kHeads + (real ? g + 8 * r : 0)) * p.qh;
 #pragma unroll
@@ -355,12 +365,12 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value>::kB
                     lo = __ldcg(reinterpret_cast<const unsigned*>(q + 16 * s + 2 * t));
                     hi = __ldcg(reinterpret_cast<const unsigned*>(q + 16 * s + 2 * t + 8));
                 }
-                qa[s][r] = real ? lo : 0u;
-                qa[s][kHalves + r] = real ? hi : 0u;
+                qb[s][2 * r] = real ? lo : 0u;
+                qb[s][2 * r + 1] = real ? hi : 0u;
             }
         }
     };
-    // bf16 rows become fp16 by a power of two of their own: exact to 2^-38 of the row's largest value.
+    // bf16 heads become fp16 by a power of two of their own: exact to 2^-38 of the head's largest value.
     auto settle = [&]() {
         if constexpr (kCoded && std::is_same<QT, __nv_bfloat16>::value) {
 #pragma unroll
@@ -370,19 +380,21 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value>::kB
                 for (int s = 0; s < D / 16; ++s)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const uint32_t w = qa[s][e * kHalves + r];
+                        const uint32_t w = qb[s][2 * r + e];
                         top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u))));
                     }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const int e2 = top > 0.f && top <= 3e38f ? max(-110, min(126, (int)(__float_as_uint(top) >> 23) - 127)) : 13;
                 const float up = __uint_as_float((uint32_t)(127 + 13 - e2) << 23);
-                unit[r] = p.scale_log2 * __uint_as_float((uint32_t)(127 - 13 + e2) << 23);
+                const float back = p.scale_log2 * __uint_as_float((uint32_t)(127 - 13 + e2) << 23);
+                unit[r][0] = __shfl_sync(0xffffffffu, back, 8 * t);
+                unit[r][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
 #pragma unroll
                 for (int s = 0; s < D / 16; ++s)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        uint32_t& w = qa[s][e * kHalves + r];
+                        uint32_t& w = qb[s][2 * r + e];
                         const __half2 h = __floats2half2_rn(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up);
                         w = *reinterpret_cast<const uint32_t*>(&h);
                     }
@@ -393,10 +405,13 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value>::kB
     start(seg);
     for (;;) {
         settle();
-        float o[kTilesN][4] = {};
-        float m[kHalves], l[kHalves], vtop = 7.888609052210118e-31f, vinv = 1.2676506002282294e30f;      // 2^-100, 2^100
+        // o[j][r]: channels 16 j + g and + 8 (coded: g * D / 8 + 2 j and + 1) of heads 2 t, 2 t + 1 (+ 8 r)
+        float o[D / 16][kHalves][4] = {};
+        float m[kHalves][2], base[kHalves][2], l[kHalves][2], vtop = 7.888609052210118e-31f, vinv = 1.2676506002282294e30f;   // 2^-100, 2^100
 #pragma unroll
-        for (int r = 0; r < kHalves; ++r) m[r] = -INFINITY, l[r] = 0.f;
+        for (int r = 0; r < kHalves; ++r)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) m[r][e] = -INFINITY, base[r][e] = -kLift, l[r][e] = 0.f;
 
 #pragma unroll 1
         for (int i = 0; i < count; ++i) {
@@ -411,148 +426,181 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value>::kB
             const bool full = real >= R::kSub && gone == 0;     // the same in all lanes
             slot = slot + 1 == R::kStages ? 0 : slot + 1;
 
-            // scores: columns 2 t, 2 t + 1 of tiles of 8 positions
-            float s[kCols][4] = {};
-            if constexpr (!kCoded) {
+            // scores^T of step h: positions g and g + 8, heads 2 t and 2 t + 1: [0], [1] and [2], [3]
+            float s[kSteps][kHalves][4] = {};
 #pragma unroll
-                for (int c = 0; c < D / 16; ++c)
+            for (int c = 0; c < D / 16; c += kCoded ? 2 : 1)
 #pragma unroll
-                    for (int h = 0; h < kSteps; ++h) {
-                        uint32_t w[4];
-                        ldsm4(ku + place<R::kRowBytes>(16 * h + (lane & 7) + ((lane >> 4) << 3), 2 * c + ((lane >> 3) & 1)), w);
+                for (int h = 0; h < kSteps; ++h) {
+                    uint32_t w[4];              // uncoded: one step of channels; coded: two
+                    ldsm4(ku + place<R::kRowBytes>(16 * h + (lane & 15), (kCoded ? c : 2 * c) + (lane >> 4)), w);
+                    if constexpr (!kCoded) {
 #pragma unroll
-                        for (int n = 0; n < 2; ++n)
-                            mma(MT(), s[2 * h + n], qa[c][0], kHalves == 2 ? qa[c][1] : 0u, qa[c][kHalves],
-                                kHalves == 2 ? qa[c][3] : 0u, w[2 * n], w[2 * n + 1]);
+                        for (int r = 0; r < kHalves; ++r)
+                            mma(MT(), s[h][r], w[0], w[1], w[2], w[3], qb[c][2 * r], qb[c][2 * r + 1]);
+                    } else {
+#pragma unroll
+                        for (int d = 0; d < 2; ++d) {
+                            uint32_t a[4];
+                            Widen::run(w[2 * d], &a[0], &a[2]);
+                            Widen::run(w[2 * d + 1], &a[1], &a[3]);
+#pragma unroll
+                            for (int r = 0; r < kHalves; ++r)
+                                mma(MT(), s[h][r], a[0], a[1], a[2], a[3], qb[c + d][2 * r], qb[c + d][2 * r + 1]);
+                        }
                     }
-            } else {
+                }
+            // positions g, g + 8 of each step: the scale of V, and which of them are no positions at all
+            float vs[kSteps][2];
+            unsigned dead = 0;
+            if (!full) {
 #pragma unroll
-                for (int c = 0; c < D / 16; c += 2)
+                for (int h = 0; h < kSteps; ++h)
 #pragma unroll
-                    for (int h = 0; h < kSteps; ++h) {
-                        uint32_t w[4];          // two steps of 16 channels x two tiles of 8 positions
-                        ldsm4(ku + place<R::kRowBytes>(16 * h + (lane & 7) + (((lane >> 3) & 1) << 3), c + (lane >> 4)), w);
-#pragma unroll
-                        for (int d = 0; d < 2; ++d)
-#pragma unroll
-                            for (int n = 0; n < 2; ++n) {
-                                uint32_t b0, b1;
-                                Widen::run(w[2 * d + n], &b0, &b1);
-                                mma(MT(), s[2 * h + n], qa[c + d][0], kHalves == 2 ? qa[c + d][1] : 0u, qa[c + d][kHalves],
-                                    kHalves == 2 ? qa[c + d][3] : 0u, b0, b1);
-                            }
-                    }
+                    for (int k = 0; k < 2; ++k)
+                        if (16 * h + 8 * k + g >= real || ((gone >> h) & 1u)) dead |= 1u << (2 * h + k);
             }
-            float vs[kCols][2];                 // scale of V over the largest scale so far
-            float grow = 1.f;
+            bool move = false;
             if constexpr (kCoded) {
                 const float* sc = reinterpret_cast<const float*>(stage + 2 * R::kRows);
-                float top = 0.f;
 #pragma unroll
-                for (int n = 0; n < kCols; ++n) {
-                    const float2 k2 = *reinterpret_cast<const float2*>(sc + 8 * n + 2 * t);
-                    const float2 v2 = *reinterpret_cast<const float2*>(sc + R::kSub + 8 * n + 2 * t);
-                    vs[n][0] = v2.x, vs[n][1] = v2.y;
-                    s[n][0] *= k2.x, s[n][1] *= k2.y;
-                    if constexpr (kHalves == 2) s[n][2] *= k2.x, s[n][3] *= k2.y;
-                }
+                for (int h = 0; h < kSteps; ++h)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float ks = sc[16 * h + 8 * k + g];
+                        vs[h][k] = sc[R::kSub + 16 * h + 8 * k + g];
+#pragma unroll
+                        for (int r = 0; r < kHalves; ++r) s[h][r][2 * k] *= ks, s[h][r][2 * k + 1] *= ks;
+                    }
                 if (!full) {                    // scales behind the end may be anything, NaN too
 #pragma unroll
-                    for (int n = 0; n < kCols; ++n)
+                    for (int h = 0; h < kSteps; ++h)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            if (8 * n + 2 * t + e >= real || ((gone >> (n >> 1)) & 1u)) vs[n][e] = 0.f;
+                        for (int k = 0; k < 2; ++k)
+                            if ((dead >> (2 * h + k)) & 1u) vs[h][k] = 0.f;
                 }
 #pragma unroll
-                for (int n = 0; n < kCols; ++n) top = fmaxf(top, fmaxf(fabsf(vs[n][0]), fabsf(vs[n][1])));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                if (top > vtop) {               // the same in all lanes
-                    grow = __fdividef(vtop, top);
-                    vtop = top;
-                    vinv = __frcp_rn(top);
-                }
+                for (int h = 0; h < kSteps; ++h) move |= fabsf(vs[h][0]) > 2.f * vtop || fabsf(vs[h][1]) > 2.f * vtop;
             }
-            uint32_t pa[kCols][2 * kHalves];    // [tile][half]: weights, [tile][kHalves + half]: their remainders
-            float keep[kHalves];
-            bool moved = grow != 1.f;
+            float x[kSteps][kHalves][4];        // exponents
+            auto exponents = [&]() {
 #pragma unroll
-            for (int r = 0; r < kHalves; ++r) {
-                float top = -INFINITY;
+                for (int h = 0; h < kSteps; ++h)
 #pragma unroll
-                for (int n = 0; n < kCols; ++n) s[n][2 * r] *= unit[r], s[n][2 * r + 1] *= unit[r];
+                    for (int r = 0; r < kHalves; ++r)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[h][r][e] = __fmaf_rn(s[h][r][e], unit[r][e & 1], -base[r][e & 1]);
                 if (!full) {
 #pragma unroll
-                    for (int n = 0; n < kCols; ++n)
+                    for (int h = 0; h < kSteps; ++h)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            if (8 * n + 2 * t + e >= real || ((gone >> (n >> 1)) & 1u)) s[n][2 * r + e] = -INFINITY;
+                        for (int r = 0; r < kHalves; ++r)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if ((dead >> (2 * h + (e >> 1))) & 1u) x[h][r][e] = -INFINITY;
                 }
-#pragma unroll
-                for (int n = 0; n < kCols; ++n) top = fmaxf(top, fmaxf(s[n][2 * r], s[n][2 * r + 1]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                top = fmaxf(top, m[r]);
-                const float safe = top == -INFINITY ? 0.f : top;
-                keep[r] = exp2_fast(m[r] - safe);
-                moved |= top != m[r];
-                m[r] = top;
-                const float base = safe - kLift;
-                float sum = 0.f;
-#pragma unroll
-                for (int n = 0; n < kCols; ++n) {
-                    float w0 = exp2_fast(s[n][2 * r] - base), w1 = exp2_fast(s[n][2 * r + 1] - base);
-                    sum += w0 + w1;
-                    if constexpr (kCoded) w0 *= vs[n][0] * vinv, w1 *= vs[n][1] * vinv;
-                    split(MT(), w0, w1, &pa[n][r], &pa[n][kHalves + r]);
-                }
-                l[r] = __fmaf_rn(l[r], keep[r], sum);
-            }
-            if (__any_sync(0xffffffffu, moved)) {
-                const float f0 = keep[0] * grow, f1 = (kHalves == 2 ? keep[kHalves - 1] : keep[0]) * grow;
-#pragma unroll
-                for (int j = 0; j < kTilesN; ++j) o[j][0] *= f0, o[j][1] *= f0, o[j][2] *= f1, o[j][3] *= f1;
-            }
-            // o += weights . V of step h.  kHalves == 1: rows 8..15 are the remainders of rows 0..7; 2: a second product
-            auto weigh = [&](int h, float (&acc)[4], uint32_t b0, uint32_t b1) {
-                const uint32_t(&x)[2 * kHalves] = pa[2 * h];
-                const uint32_t(&y)[2 * kHalves] = pa[2 * h + 1];
-                mma(MT(), acc, x[0], x[1], y[0], y[1], b0, b1);
-                if constexpr (kHalves == 2) mma(MT(), acc, x[2], x[3], y[2], y[3], b0, b1);
             };
+            exponents();
+#pragma unroll
+            for (int r = 0; r < kHalves; ++r)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    move |= m[r][e & 1] == -INFINITY;
+#pragma unroll
+                    for (int h = 0; h < kSteps; ++h) move |= x[h][r][e] > kLift + kSlack;
+                }
+            if (__any_sync(0xffffffffu, move)) {
+                float grow = 1.f;
+                if constexpr (kCoded) {
+                    float top = 0.f;
+#pragma unroll
+                    for (int h = 0; h < kSteps; ++h) top = fmaxf(top, fmaxf(fabsf(vs[h][0]), fabsf(vs[h][1])));
+#pragma unroll
+                    for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+                    if (top > vtop) {
+                        grow = __fdividef(vtop, top);
+                        vtop = top;
+                        vinv = __frcp_rn(top);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < kHalves; ++r)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int h = 0; h < kSteps; ++h) top = fmaxf(top, fmaxf(x[h][r][e], x[h][r][e + 2]));
+#pragma unroll
+                        for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+                        top = fmaxf(m[r][e], top + base[r][e]);
+                        const float safe = top == -INFINITY ? 0.f : top;
+                        const float keep = exp2_fast(m[r][e] - safe);
+                        m[r][e] = top;
+                        base[r][e] = safe - kLift;
+                        l[r][e] *= keep;
+#pragma unroll
+                        for (int j = 0; j < D / 16; ++j) o[j][r][e] *= keep * grow, o[j][r][e + 2] *= keep * grow;
+                    }
+                exponents();
+            }
+            // weights as the second operand of o^T += V^T w^T: positions 2 t, 2 t + 1 (and 8 further) of head g
+            uint32_t wb[kSteps][kHalves][2], rest[kSteps][kHalves][2];
+#pragma unroll
+            for (int h = 0; h < kSteps; ++h)
+#pragma unroll
+                for (int r = 0; r < kHalves; ++r)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        float w0 = exp2_fast(x[h][r][2 * k]), w1 = exp2_fast(x[h][r][2 * k + 1]);
+                        l[r][0] += w0;
+                        l[r][1] += w1;
+                        if constexpr (kCoded) {
+                            const float f = vs[h][k] * vinv;
+                            w0 *= f, w1 *= f;
+                        }
+                        uint32_t hi, lo;
+                        split(MT(), w0, w1, &hi, &lo);
+                        wb[h][r][k] = transpose8(hi);
+                        rest[h][r][k] = transpose8(lo);
+                    }
 #pragma unroll
             for (int h = 0; h < kSteps; ++h) {
+                auto weigh = [&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+                    for (int r = 0; r < kHalves; ++r) {
+                        mma(MT(), o[j][r], a0, a1, a2, a3, wb[h][r][0], wb[h][r][1]);
+                        mma(MT(), o[j][r], a0, a1, a2, a3, rest[h][r][0], rest[h][r][1]);
+                    }
+                };
                 if constexpr (!kCoded) {
 #pragma unroll
-                    for (int c = 0; c < D / 16; ++c) {
+                    for (int j = 0; j < D / 16; ++j) {
                         uint32_t w[4];
-                        ldsm4t(vu + place<R::kRowBytes>(16 * h + (lane & 15), 2 * c + (lane >> 4)), w);
-                        weigh(h, o[2 * c], w[0], w[1]);
-                        weigh(h, o[2 * c + 1], w[2], w[3]);
+                        ldsm4t(vu + place<R::kRowBytes>(16 * h + (lane & 7) + ((lane >> 4) << 3), 2 * j + ((lane >> 3) & 1)), w);
+                        weigh(j, w[0], w[1], w[2], w[3]);
                     }
                 } else {
-                    // column n of tile j is channel n * D / 8 + j: a thread's bytes of a row are D / 8 neighbours
+                    // a thread's bytes of a row are the D / 8 channels from g * D / 8 on
                     constexpr int kWords = D / 32 < 4 ? D / 32 : 4;    // words per access: 2 (8 bytes) or 4 (16 bytes)
 #pragma unroll
                     for (int c = 0; c < D / 8 / (4 * kWords); ++c) {
-                        uint32_t x[4][kWords];
+                        uint32_t v[4][kWords];
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const int key = 16 * h + 2 * t + (k & 1) + ((k >> 1) << 3), byte = g * (D / 8) + c * 16;
                             const uint8_t* from = stage + R::kRows + place<R::kRowBytes>(key, byte >> 4) + (byte & 15);
-                            if constexpr (kWords == 4) *reinterpret_cast<uint4*>(x[k]) = *reinterpret_cast<const uint4*>(from);
-                            else *reinterpret_cast<uint2*>(x[k]) = *reinterpret_cast<const uint2*>(from);
+                            if constexpr (kWords == 4) *reinterpret_cast<uint4*>(v[k]) = *reinterpret_cast<const uint4*>(from);
+                            else *reinterpret_cast<uint2*>(v[k]) = *reinterpret_cast<const uint2*>(from);
                         }
 #pragma unroll
-                        for (int w = 0; w < kWords; ++w) {
-                            uint32_t lo[4], hi[4];      // tiles 4 w .. 4 w + 3: positions 2 t, 2 t + 1 and 8 further
-                            Widen::run(__byte_perm(x[0][w], x[1][w], 0x5140), &lo[0], &lo[1]);
-                            Widen::run(__byte_perm(x[0][w], x[1][w], 0x7362), &lo[2], &lo[3]);
-                            Widen::run(__byte_perm(x[2][w], x[3][w], 0x5140), &hi[0], &hi[1]);
-                            Widen::run(__byte_perm(x[2][w], x[3][w], 0x7362), &hi[2], &hi[3]);
+                        for (int w = 0; w < kWords; ++w)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) weigh(h, o[(c * kWords + w) * 4 + e], lo[e], hi[e]);
-                        }
+                            for (int d = 0; d < 2; ++d) {
+                                uint32_t a0, a1, a2, a3;
+                                Widen::run(__byte_perm(v[0][w], v[1][w], d ? 0x7362 : 0x5140), &a0, &a1);
+                                Widen::run(__byte_perm(v[2][w], v[3][w], d ? 0x7362 : 0x5140), &a2, &a3);
+                                weigh((c * kWords + w) * 2 + d, a0, a1, a2, a3);
+                            }
                     }
                 }
             }
@@ -577,30 +625,32 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value>::kB
         }
 
         // ---- the four warps' parts become one: each leaves its rows in a slot of its ring.  Column c of row r lies at
-        // c ^ 8 (r % 8) ^ 4 (c / 32 % 8): the lanes of a store fall on different banks
-        auto at = [](int r, int c) { return r * D + (c ^ ((r & 7) << 3) ^ (((c >> 5) & 7) << 2)); };
+        // c ^ 8 (r / 2 % 4): the lanes of a store fall on different banks
+        auto at = [](int r, int c) { return r * D + (c ^ (((r >> 1) & 3) << 3)); };
         float* mine = reinterpret_cast<float*>(ring + free_slot * R::kStage);
         if (lane == 0) jslot[warp] = (uint32_t)(warp * R::kStages + free_slot) * R::kStage;
 #pragma unroll
-        for (int r = 0; r < kHalves; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            const int row = g + 8 * r;
-            if (t == 0) jm[warp][row] = m[r], jl[warp][row] = l[r];
-            auto value = [&](int j, int e) { return kHalves == 1 ? o[j][e] + o[j][2 + e] : o[j][2 * r + e]; };
-            if constexpr (kCoded) {
+        for (int r = 0; r < kHalves; ++r)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 2; ++e) {
+                const int row = 8 * r + 2 * t + e;
+                float sum = l[r][e];
 #pragma unroll
-                    for (int j = 0; j < kTilesN; j += 4)
-                        *reinterpret_cast<float4*>(mine + at(row, (2 * t + e) * (D / 8) + j)) =
-                            make_float4(value(j, e) * vtop, value(j + 1, e) * vtop, value(j + 2, e) * vtop, value(j + 3, e) * vtop);
-            } else {
+                for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+                if (g == 0) jm[warp][row] = m[r][e], jl[warp][row] = sum;
+                if constexpr (kCoded) {
 #pragma unroll
-                for (int j = 0; j < kTilesN; ++j)
-                    *reinterpret_cast<float2*>(mine + at(row, 8 * j + 2 * t)) = make_float2(value(j, 0), value(j, 1));
+                    for (int j = 0; j < D / 16; j += 2)
+                        *reinterpret_cast<float4*>(mine + at(row, g * (D / 8) + 2 * j)) =
+                            make_float4(o[j][r][e] * vtop, o[j][r][e + 2] * vtop, o[j + 1][r][e] * vtop, o[j + 1][r][e + 2] * vtop);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j) {
+                        mine[at(row, 16 * j + g)] = o[j][r][e];
+                        mine[at(row, 16 * j + 8 + g)] = o[j][r][e + 2];
+                    }
+                }
             }
-        }
         __syncthreads();
         const int dhead = done.pair / p.blocks_per_kv, dblock = done.pair - dhead * p.blocks_per_kv;
         const int q0 = dhead * p.group + dblock * kHeads, rows = min(kHeads, p.group - dblock * kHeads);
@@ -711,8 +761,12 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
     const int group = H / kv.heads;
     out->heads_per_block = group > 8 ? 16 : 8;
     out->blocks_per_kv = (group + out->heads_per_block - 1) / out->heads_per_block;
+    const bool wide = out->heads_per_block == 16;
     int tile = 0, per_sm = 0;
-#define KAIROS_RING(D)                                                                                (tile = coded ? Ring<D, true>::kTile : Ring<D, false>::kTile,                                       per_sm = coded ? Ring<D, true>::kBlocksPerSm : Ring<D, false>::kBlocksPerSm)
+#define KAIROS_RING(D)                                                                                (wide ? (tile = coded ? Ring<D, true, 2>::kTile : Ring<D, false, 2>::kTile,                 \
+             per_sm = coded ? Ring<D, true, 2>::kBlocksPerSm : Ring<D, false, 2>::kBlocksPerSm) \
+          : (tile = coded ? Ring<D, true, 1>::kTile : Ring<D, false, 1>::kTile,                 \
+             per_sm = coded ? Ring<D, true, 1>::kBlocksPerSm : Ring<D, false, 1>::kBlocksPerSm))
     if (kv.dim == 64) KAIROS_RING(64);
     else if (kv.dim == 128) KAIROS_RING(128);
     else KAIROS_RING(256);
@@ -732,7 +786,7 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
 template <typename QT, typename Widen, int D, int kHalves>
 static int run_attention(const void* Q, const KvView& kv, const void* table, const void* lens, void* O, void* LSE, void* ws,
                          const AttnShape& p, const Plan& plan, int* status, cudaStream_t st) {
-    using R = Ring<D, !std::is_void<Widen>::value>;
+    using R = Ring<D, !std::is_void<Widen>::value, kHalves>;
     static PerDeviceFlag flag;
     auto kernel = paged_attention_kernel<QT, Widen, D, kHalves>;
     const int rc = ensure_dynamic_smem(flag, kernel, R::kBytes);
