@@ -46,29 +46,34 @@ struct AttnShape {
 __device__ __forceinline__ int seq_len(const int* lens, int b, int most) { return max(0, min(__ldcg(lens + b), most)); }
 
 struct Cut {
-    unsigned total, run;                    // tiles of all pairs, tiles per worker
-    int b, pair, tile;                      // where flat tile `x` lies: sequence, pair (kv head, head block) and tile of it
-    int tiles;                              // tiles of that sequence
-    unsigned pair_first;                    // flat index of that pair's first tile
+    unsigned total, run;                    // units of all pairs, units per worker
+    int b, pair, unit;                      // where flat unit `x` lies: sequence, pair (kv head, head block) and unit of it
+    int len;                                // of that sequence
 };
 
-// Tiles that a block may take over what an even cut gives it before cutting pays: a join costs about as long as a block
-// needs for so many tiles.
+// The work of a pair in units: a tile of positions each, and one more for ending it (joining the warps, starting the next
+// pair), which takes about as long; none for an empty sequence.
+template <int kTile>
+__device__ __forceinline__ unsigned units_of(int len) { return len > 0 ? (unsigned)(len + kTile - 1) / kTile + 1 : 0; }
+
+// Units that a block may take over what an even cut gives it before cutting pays: a join costs about as long as a block
+// needs for so many.
 constexpr unsigned kSpare = 6;
 
-// Block-wide (128 threads).  Scans the sequences' tile counts and finds, for this block, the flat tile x:
-//   kMain: where worker blockIdx.x begins; returns false where it has no work.  If every pair is short -- no more than
-//     kSpare tiles over the even run -- and there are no more pairs than workers, a worker takes one whole pair (run = 0);
-//   !kMain: the boundary behind worker blockIdx.x's run; returns false where there is none.
-template <int kTile, bool kMain>
+// Block-wide (128 threads).  Scans the sequences' units and finds the flat unit x where worker blockIdx.x begins; returns
+// false where it has no work.  If every pair is short -- no more than kSpare units over the even run -- and there are no
+// more pairs than workers, a worker takes one whole pair (run = 0).
+template <int kTile>
 __device__ __forceinline__ bool locate(const int* lens, const AttnShape& p, int pairs, int most, Cut* out) {
     __shared__ unsigned warp_sum[kWarps], warp_top[kWarps];
     __shared__ Cut found;
     const int tid = threadIdx.x, per = (p.B + 127) >> 7;
     const int first = tid * per, last = min(p.B, first + per);
     unsigned mine = 0, top = 0;
+    int own_len = 0;                        // the only length of this thread where there are no more sequences than threads
     for (int b = first; b < last; ++b) {
-        const unsigned n = (unsigned)(seq_len(lens, b, most) + kTile - 1) / kTile;
+        own_len = seq_len(lens, b, most);
+        const unsigned n = units_of<kTile>(own_len);
         mine += n;
         top = max(top, n);
     }
@@ -92,22 +97,21 @@ __device__ __forceinline__ bool locate(const int* lens, const AttnShape& p, int 
     const unsigned run = (total + p.workers - 1) / p.workers;
     const bool whole = !p.joins || (top <= run + kSpare && (long long)p.B * pairs <= p.workers);
     if (whole) {
-        if (!kMain) return false;
         const int b = blockIdx.x / pairs;
         if (b >= p.B) return false;
-        const int n = (seq_len(lens, b, most) + kTile - 1) / kTile;
-        *out = Cut{total, 0, b, (int)(blockIdx.x - b * pairs), 0, n, 0};
-        return n > 0;
+        *out = Cut{total, 0, b, (int)(blockIdx.x - b * pairs), 0, seq_len(lens, b, most)};
+        return out->len > 0;
     }
-    const unsigned x = (blockIdx.x + (kMain ? 0 : 1)) * run;
+    const unsigned x = blockIdx.x * run;
     if (x >= total) return false;           // the same for every thread
     unsigned before = upto - mine;
     if (x >= before * pairs && x < upto * pairs) {
         for (int b = first; b < last; ++b) {
-            const unsigned n = (unsigned)(seq_len(lens, b, most) + kTile - 1) / kTile;
+            const int len = per == 1 ? own_len : seq_len(lens, b, most);
+            const unsigned n = units_of<kTile>(len);
             if (x < (before + n) * pairs) {
                 const unsigned rest = x - before * pairs;
-                found = Cut{total, run, b, (int)(rest / n), (int)(rest % n), (int)n, before * pairs + rest / n * n};
+                found = Cut{total, run, b, (int)(rest / n), (int)(rest % n), len};
                 break;
             }
             before += n;
@@ -118,13 +122,22 @@ __device__ __forceinline__ bool locate(const int* lens, const AttnShape& p, int 
     return true;
 }
 
-// Partial results: slot 2 w of worker w is the pair that its run begins in, slot 2 w + 1 the one that it ends in.
+// Partial results in the workspace: slot 2 w of worker w is the pair that its run begins in, slot 2 w + 1 the one that it
+// ends in.  Behind them a record per worker: the pair that begins in its run and lies across the run's end, if there is one.
+struct Crossing {
+    int b, pair;
+    unsigned slot, last;                    // this worker's part, the worker of the last part; last == the worker: none
+};
 template <int R, int D>
 struct Partials {
     static constexpr size_t kFloats = (size_t)R * (D + 2);
     static __device__ __forceinline__ float* o(float* ws, unsigned slot) { return ws + slot * kFloats; }
     static __device__ __forceinline__ float* ml(float* ws, unsigned slot) { return ws + slot * kFloats + R * D; }
+    static __device__ __forceinline__ Crossing* crossing(float* ws, int workers, unsigned worker) {
+        return reinterpret_cast<Crossing*>(ws + 2 * (size_t)workers * kFloats) + worker;
+    }
 };
+static_assert(sizeof(Crossing) == 16, "one 16-byte access");
 
 // ---- instructions -------------------------------------------------------------------------------------------
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
@@ -252,25 +265,43 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
     __shared__ float jm[kWarps][kHeads], jl[kWarps][kHeads];
     __shared__ uint32_t jslot[kWarps];
     chain_wait();
-    chain_release();        // what reads this kernel's results waits for all of it; its set-up may begin
+    chain_release();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int pairs = kv.heads * p.blocks_per_kv, most = p.table_width << kv.page_shift;
-    // sequences without positions have no tile: their rows are written here
-    for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
-        const int n = __ldcg(lens + b);
-        if (n > most) *status = KAIROS_ERR_ARG;
-        if (min(n, most) > 0) continue;
-        for (int i = threadIdx.x; i < p.H * D / 8; i += 128)
-            reinterpret_cast<uint4*>(O + (size_t)b * p.H * D)[i] = make_uint4(0, 0, 0, 0);
-        if (LSE)
-            for (int i = threadIdx.x; i < p.H; i += 128) LSE[(size_t)b * p.H + i] = -INFINITY;
-    }
-    Cut cut;
-    if (!locate<kTile, true>(lens, p, pairs, most, &cut)) return;
-    // flat tiles still to take: a run of the even cut, or (run == 0) one whole pair
-    unsigned left = cut.run ? min(cut.run, cut.total - blockIdx.x * cut.run) : (unsigned)cut.tiles;
-    Segment seg = {cut.b, cut.pair, cut.tile, cut.tiles, min((int)left, cut.tiles - cut.tile), seq_len(lens, cut.b, most)};
+    Cut cut = {};
+    const bool some = locate<kTile>(lens, p, pairs, most, &cut);
+    // Units still to take: a run of the even cut, or (run == 0) one whole pair.
+    unsigned left = !some ? 0u : cut.run ? min(cut.run, cut.total - blockIdx.x * cut.run) : units_of<kTile>(cut.len);
+    Segment seg = {cut.b, cut.pair, cut.unit, 0, 0, cut.len};
     bool first_segment = true;
+    // Takes what this worker's run holds of the pair at seg.tile; false where that is only the unit behind its last tile.
+    auto take = [&]() {
+        seg.tiles = (seg.len + kTile - 1) / kTile;
+        const int units = min((int)left, seg.tiles + 1 - seg.tile);
+        left -= units;
+        seg.take = min(units, seg.tiles - seg.tile);
+        return seg.take > 0;
+    };
+    // The next pair with something to take; false at the end of the run.
+    auto next = [&]() {
+        do {
+            if (left == 0) return false;
+            if (++seg.pair == pairs) {
+                seg.pair = 0;
+                do seg.len = seq_len(lens, ++seg.b, most); while (seg.len == 0);
+            }
+            seg.tile = 0;
+            first_segment = false;
+        } while (!take());
+        return true;
+    };
+    bool more = left > 0 && (take() || next());
+    const unsigned run_end = min((blockIdx.x + 1) * cut.run, cut.total);
+    auto record = [&](const Crossing& c) {
+        *reinterpret_cast<uint4*>(Partials<kHeads, D>::crossing(ws, p.workers, blockIdx.x)) =
+            make_uint4((unsigned)c.b, (unsigned)c.pair, c.slot, c.last);
+    };
+    if (p.joins && threadIdx.x == 0) record({0, 0, 0, blockIdx.x});
 
     uint8_t* ring = smem + warp * (R::kStages * R::kStage);
     const uint32_t ring_u = smem_u32(ring);
@@ -402,8 +433,18 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
         }
     };
 
-    start(seg);
-    for (;;) {
+    if (more) start(seg);
+    // sequences without positions have no tile: their rows are written here, while the first stages are on their way
+    for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+        const int n = __ldcg(lens + b);
+        if (n > most && threadIdx.x == 0) *status = KAIROS_ERR_ARG;
+        if (min(n, most) > 0) continue;
+        for (int i = threadIdx.x; i < p.H * D / 8; i += 128)
+            reinterpret_cast<uint4*>(O + (size_t)b * p.H * D)[i] = make_uint4(0, 0, 0, 0);
+        if (LSE)
+            for (int i = threadIdx.x; i < p.H; i += 128) LSE[(size_t)b * p.H + i] = -INFINITY;
+    }
+    while (more) {
         settle();
         // o[j][r]: channels 16 j + g and + 8 (coded: g * D / 8 + 2 j and + 1) of heads 2 t, 2 t + 1 (+ 8 r)
         float o[D / 16][kHalves][4] = {};
@@ -609,20 +650,10 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
         // ---- the next segment's first stages are requested before this one's parts are joined ----------------
         const Segment done = seg;
         const bool first = first_segment;
-        left -= done.take;
         const uint32_t free_slot = slot == 0 ? R::kStages - 1 : slot - 1;      // the one slot that start() leaves alone
         __syncwarp();                           // every lane has read the last stage
-        if (left) {
-            if (++seg.pair == pairs) {
-                seg.pair = 0;
-                do seg.len = seq_len(lens, ++seg.b, most); while (seg.len == 0);
-                seg.tiles = (seg.len + kTile - 1) / kTile;
-            }
-            seg.tile = 0;
-            seg.take = min((int)left, seg.tiles);
-            first_segment = false;
-            start(seg);
-        }
+        more = next();
+        if (more) start(seg);
 
         // ---- the four warps' parts become one: each leaves its rows in a slot of its ring.  Column c of row r lies at
         // c ^ 8 (r / 2 % 4): the lanes of a store fall on different banks
@@ -656,6 +687,8 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
         const int q0 = dhead * p.group + dblock * kHeads, rows = min(kHeads, p.group - dblock * kHeads);
         const bool whole = done.take == done.tiles;
         const unsigned part = 2 * blockIdx.x + (first ? 0 : 1);
+        if (!whole && done.tile == 0 && threadIdx.x == 0)      // begins here and lies across the run's end
+            record({done.b, done.pair, part, (run_end - done.take + done.tiles - 1) / cut.run});
         for (int i = threadIdx.x; i < rows * (D / 4); i += 128) {
             const int row = i / (D / 4), c = 4 * (i - row * (D / 4));
             float top = -INFINITY;
@@ -684,56 +717,67 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
                 if (c == 0) *reinterpret_cast<float2*>(Partials<kHeads, D>::ml(ws, part) + 2 * row) = make_float2(top, sum);
             }
         }
-        if (!left) break;
-        __syncthreads();                        // the slots belong to the rings again
+        if (more) __syncthreads();              // the slots belong to the rings again
     }
 }
 
-// Block w looks at the boundary between the runs of workers w and w + 1.  Where a pair lies across it and no earlier
-// boundary, its partial results (workers w, w + 1, ... up to the one that holds its last tile) are joined here; the
-// channels are spread over gridDim.y.
-template <typename QT, int D, int kHeads, int kTile>
-__global__ void __launch_bounds__(128) paged_attention_join_kernel(const KvView kv, const int* __restrict__ lens, QT* __restrict__ O,
-                                                                   float* __restrict__ LSE, float* __restrict__ ws,
-                                                                   const AttnShape p) {
+// Block (w, y): the pair, if any, that begins in worker w's run and lies across its end; a slice of 32 items (a head's four
+// channels) of its partial results of workers w, w + 1, ... .  The four warps share the parts, and the order in which parts
+// are added depends on nothing but their number.
+template <typename QT, int D, int kHeads>
+__global__ void __launch_bounds__(128) paged_attention_join_kernel(QT* __restrict__ O, float* __restrict__ LSE,
+                                                                   float* __restrict__ ws, const AttnShape p) {
     using P = Partials<kHeads, D>;
-    // The lengths were there before the kernel whose parts are joined began (it lets this one start only after its own
-    // wait), so the place is found while that kernel still runs.
-    const int pairs = kv.heads * p.blocks_per_kv;
-    Cut cut;
-    const bool some = locate<kTile, false>(lens, p, pairs, p.table_width << kv.page_shift, &cut);
+    constexpr int kPer = 32 / kHeads, kAhead = 8;       // chunks of four channels in a slice; parts whose loads go together
+    __shared__ float4 part_o[kWarps][32];
+    __shared__ float2 part_ml[kWarps][32];
     chain_wait();
     chain_release();
-    if (!some) return;
-    const unsigned x = (blockIdx.x + 1) * cut.run, first = cut.pair_first;
-    if (first >= x || first < x - cut.run) return;      // a pair begins here, or lay across an earlier boundary already
-    const unsigned last = (first + cut.tiles - 1) / cut.run;
-    const int head = cut.pair / p.blocks_per_kv, block = cut.pair - head * p.blocks_per_kv;
+    const uint4 record = __ldcg(reinterpret_cast<const uint4*>(P::crossing(ws, p.workers, blockIdx.x)));
+    const unsigned last = record.w;
+    if (last == blockIdx.x) return;
+    const int b = (int)record.x, pair = (int)record.y, head = pair / p.blocks_per_kv, block = pair - head * p.blocks_per_kv;
     const int rows = min(kHeads, p.group - block * kHeads);
-    const int per = D / 4 / gridDim.y;                  // chunks of four channels of a row in this block
-    for (int i = threadIdx.x; i < rows * per; i += 128) {
-        const int row = i / per, c = i - row * per + blockIdx.y * per;
-        float top = -INFINITY, sum = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (unsigned w = blockIdx.x; w <= last; ++w) {
-            const unsigned slot = 2 * w + (w == blockIdx.x && first > w * cut.run ? 1 : 0);
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(P::ml(ws, slot) + 2 * row));
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(P::o(ws, slot) + row * D + 4 * c));
-            const float next = fmaxf(top, ml.x), safe = next == -INFINITY ? 0.f : next;
-            const float keep = exp2_fast(top - safe), f = exp2_fast(ml.x - safe);
-            top = next;
-            sum = __fmaf_rn(sum, keep, f * ml.y);
-            acc.x = __fmaf_rn(acc.x, keep, f * v.x);
-            acc.y = __fmaf_rn(acc.y, keep, f * v.y);
-            acc.z = __fmaf_rn(acc.z, keep, f * v.z);
-            acc.w = __fmaf_rn(acc.w, keep, f * v.w);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane / kPer, c = 4 * (blockIdx.y * kPer + lane % kPer);
+    float top = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float2 ml, const float4 v) {
+        const float next = fmaxf(top, ml.x), safe = next == -INFINITY ? 0.f : next;
+        const float keep = exp2_fast(top - safe), f = exp2_fast(ml.x - safe);
+        top = next;
+        sum = __fmaf_rn(sum, keep, f * ml.y);
+        acc.x = __fmaf_rn(acc.x, keep, f * v.x);
+        acc.y = __fmaf_rn(acc.y, keep, f * v.y);
+        acc.z = __fmaf_rn(acc.z, keep, f * v.z);
+        acc.w = __fmaf_rn(acc.w, keep, f * v.w);
+    };
+    if (row < rows) {
+        for (unsigned w = blockIdx.x + warp; w <= last; w += kAhead * kWarps) {
+            float2 ml[kAhead];
+            float4 v[kAhead];
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
+                const unsigned u = w + a * kWarps;
+                if (u <= last) {
+                    const unsigned slot = u == blockIdx.x ? record.z : 2 * u;
+                    ml[a] = __ldcg(reinterpret_cast<const float2*>(P::ml(ws, slot) + 2 * row));
+                    v[a] = __ldcg(reinterpret_cast<const float4*>(P::o(ws, slot) + row * D + c));
+                }
+            }
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a)
+                if (w + a * kWarps <= last) add(ml[a], v[a]);
         }
-        const float inv = __fdiv_rn(1.f, sum);
-        const size_t at = (size_t)cut.b * p.H + head * p.group + block * kHeads + row;
-        put4(O + at * D + 4 * c, acc, inv);
-        if (LSE && c == 0) LSE[at] = (top + __log2f(sum) - kLift) * kLn2;
     }
+    part_o[warp][lane] = acc;
+    part_ml[warp][lane] = make_float2(top, sum);
+    __syncthreads();
+    if (warp != 0 || row >= rows) return;
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) add(part_ml[w][lane], part_o[w][lane]);
+    const size_t at = (size_t)b * p.H + head * p.group + block * kHeads + row;
+    put4(O + at * D + c, acc, __fdiv_rn(1.f, sum));
+    if (LSE && c == 0) LSE[at] = (top + __log2f(sum) - kLift) * kLn2;
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------
@@ -771,15 +815,15 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
     else if (kv.dim == 128) KAIROS_RING(128);
     else KAIROS_RING(256);
 #undef KAIROS_RING
-    const long long per_pair = (((long long)table_width << kv.page_shift) + tile - 1) / tile;
+    const long long per_pair = (((long long)table_width << kv.page_shift) + tile - 1) / tile + 1;      // units
     const long long pairs = (long long)B * kv.heads * out->blocks_per_kv;
     if (per_pair * pairs > 0x7fffffffLL) return KAIROS_ERR_SHAPE;
     const int full = sms * per_sm;
     // No pair is cut where there are workers for all of them and none can be longer than a join is worth; otherwise the
     // device decides by the lengths.
-    out->joins = !(pairs <= full && per_pair <= (long long)kSpare + 1);
+    out->joins = !(pairs <= full && per_pair <= (long long)kSpare + 2);
     out->workers = (int)max(1LL, out->joins ? min((long long)full, per_pair * pairs) : pairs);
-    out->bytes = out->joins ? (size_t)2 * out->workers * out->heads_per_block * (kv.dim + 2) * 4 : 0;
+    out->bytes = out->joins ? (size_t)2 * out->workers * out->heads_per_block * (kv.dim + 2) * 4 + (size_t)out->workers * sizeof(Crossing) : 0;
     return KAIROS_OK;
 }
 
@@ -796,10 +840,9 @@ static int run_attention(const void* Q, const KvView& kv, const void* table, con
                                    static_cast<float*>(LSE), static_cast<float*>(ws), p, status);
     if (e != cudaSuccess) return note_cuda_error(e);
     if (plan.joins && plan.workers > 1) {
-        // few pairs: few joins of many parts each, so the channels of one are spread over several blocks
-        const int slices = (long long)p.B * kv.heads * p.blocks_per_kv < 64 ? 4 : 1;
-        e = launch_chained(paged_attention_join_kernel<QT, D, 8 * kHalves, R::kTile>, dim3(plan.workers - 1, slices), dim3(128), 0, st, kv,
-                           static_cast<const int*>(lens), static_cast<QT*>(O), static_cast<float*>(LSE), static_cast<float*>(ws), p);
+        constexpr int kSlices = D / 4 / (32 / (8 * kHalves));
+        e = launch_chained(paged_attention_join_kernel<QT, D, 8 * kHalves>, dim3(plan.workers - 1, kSlices), dim3(128), 0, st,
+                           static_cast<QT*>(O), static_cast<float*>(LSE), static_cast<float*>(ws), p);
         if (e != cudaSuccess) return note_cuda_error(e);
     }
     return launch_status();
