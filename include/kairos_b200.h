@@ -255,9 +255,9 @@ typedef struct {
  * dimension (D <= 512); Y may be X.  positions: int64 with element strides {b, s} (0 broadcasts).  transpose != 0
  * turns the other way with the same magnitude: the transposed operator, i.e. the gradient of X from that of Y.
  * Rows that are 16-byte aligned with D % 16 == 0 and rot % 16 == 0 move in 16-byte accesses, others element-wise. */
-int kairos_rotary(const void* X, const long long* x_strides, void* Y, const long long* y_strides, const void* positions,
-                  const long long* pos_strides, const kairos_rotary_plan* plan, int dtype, int transpose, int B, int S,
-                  int H, int D, kairos_stream_t stream);
+int kairos_rotary(const void* X, long long x_b, long long x_s, long long x_h, void* Y, long long y_b, long long y_s,
+                  long long y_h, const void* positions, long long pos_b, long long pos_s, const kairos_rotary_plan* plan,
+                  int dtype, int transpose, int B, int S, int H, int D, kairos_stream_t stream);
 /* The attention input of T tokens in one pass: of each row of QKV [T, (H + 2 kv_heads) * D] (F16 / BF16, row stride in
  * elements, a multiple of 8) the q heads are turned into Q_out [T, H, D], the k heads are turned and the v heads copied into the
  * cache at slots[t] = page * page_size + offset (int64).  A 16-bit cache has QKV's type; rows of an I8 / E4M3 cache
@@ -282,7 +282,7 @@ int kairos_paged_kv_read(const kairos_kv_layer* kv, const void* slots, void* K_o
  * `workspace` of kairos_paged_attention_workspace_bytes() is scratch of this call alone (contents need no
  * initialisation): calls that may overlap need workspaces of their own. */
 size_t kairos_paged_attention_workspace_bytes(const kairos_kv_layer* kv, int B, int H, int table_width);
-int kairos_paged_attention(const void* Q, const long long* q_strides, const kairos_kv_layer* kv, const void* page_table,
+int kairos_paged_attention(const void* Q, long long q_b, long long q_h, const kairos_kv_layer* kv, const void* page_table,
                            long long table_stride, int table_width, const void* lens, void* O, void* LSE_or_null, int B,
                            int H, float scale, int dtype, void* workspace, size_t workspace_bytes,
                            kairos_stream_t stream);

@@ -12,6 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'libkairos_b200.so')
 
 c_void_p, c_int, c_size_t, c_char_p = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_char_p
+c_longlong = ctypes.c_longlong
 c_u64_p = ctypes.POINTER(ctypes.c_uint64)
 
 # name -> (restype, argtypes); mirrors include/kairos_b200.h one to one
@@ -47,12 +48,13 @@ SIGNATURES = {
     'kairos_add_rms_norm': (c_int, [c_void_p] * 4 + [c_int, c_int, ctypes.c_float, c_void_p]),
     'kairos_silu_mul_quant': (c_int, [c_void_p] * 4 + [c_int, c_int, c_void_p]),
     'kairos_rope_kv': (c_int, [c_void_p] * 4 + [c_int] + [c_void_p] * 3 + [c_int] * 6 + [c_void_p]),
-    'kairos_rotary': (c_int, [c_void_p] * 7 + [c_int] * 6 + [c_void_p]),
-    'kairos_rope_paged_kv': (c_int, [c_void_p, ctypes.c_longlong] + [c_void_p] * 5 + [c_int] * 3 + [c_void_p]),
+    'kairos_rotary': (c_int, ([c_void_p] + [c_longlong] * 3) * 2 + [c_void_p, c_longlong, c_longlong, c_void_p] + [c_int] * 6 +
+                      [c_void_p]),
+    'kairos_rope_paged_kv': (c_int, [c_void_p, c_longlong] + [c_void_p] * 5 + [c_int] * 3 + [c_void_p]),
     'kairos_paged_kv_read': (c_int, [c_void_p] * 4 + [c_int] * 2 + [c_void_p]),
     'kairos_paged_attention_workspace_bytes': (c_size_t, [c_void_p] + [c_int] * 3),
-    'kairos_paged_attention': (c_int, [c_void_p] * 4 + [ctypes.c_longlong, c_int] + [c_void_p] * 3 +
-                               [c_int, c_int, ctypes.c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    'kairos_paged_attention': (c_int, [c_void_p, c_longlong, c_longlong, c_void_p, c_void_p, c_longlong, c_int] +
+                               [c_void_p] * 3 + [c_int, c_int, ctypes.c_float, c_int, c_void_p, c_size_t, c_void_p]),
     'kairos_peer_allreduce_signal_bytes': (c_int, []),
     'kairos_peer_allreduce_f16': (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, ctypes.c_longlong, c_void_p]),
     'kairos_add_rms_norm_peer': (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int,

@@ -869,7 +869,7 @@ extern "C" size_t kairos_paged_attention_workspace_bytes(const kairos_kv_layer* 
     return make_plan(kv, coded, B, H, table_width, &plan) == KAIROS_OK ? plan.bytes : 0;
 }
 
-extern "C" int kairos_paged_attention(const void* Q, const long long* q_strides, const kairos_kv_layer* layer,
+extern "C" int kairos_paged_attention(const void* Q, long long q_b, long long q_h, const kairos_kv_layer* layer,
                                       const void* page_table, long long table_stride, int table_width, const void* lens,
                                       void* O, void* LSE, int B, int H, float scale, int dtype, void* workspace,
                                       size_t workspace_bytes, kairos_stream_t stream) {
@@ -877,7 +877,7 @@ extern "C" int kairos_paged_attention(const void* Q, const long long* q_strides,
     KvView kv;
     int rc = kv_view(layer, &kv);
     if (rc != KAIROS_OK) return rc;
-    if (B < 0 || B > 65535 || H <= 0 || H % kv.heads != 0 || table_width < 0 || table_stride < 0 || !q_strides ||
+    if (B < 0 || B > 65535 || H <= 0 || H % kv.heads != 0 || table_width < 0 || table_stride < 0 ||
         ((long long)table_width << kv.page_shift) > 0x7fffffffLL)
         return KAIROS_ERR_SHAPE;
     const bool coded = layer->dtype == KAIROS_DTYPE_I8 || layer->dtype == KAIROS_DTYPE_E4M3;
@@ -885,7 +885,7 @@ extern "C" int kairos_paged_attention(const void* Q, const long long* q_strides,
         set_last_error("paged_attention: queries are fp16 or bf16, and a 16-bit cache has their type");
         return KAIROS_ERR_ARG;
     }
-    if (q_strides[0] % 8 != 0 || q_strides[1] % 8 != 0) return KAIROS_ERR_ALIGN;
+    if (q_b % 8 != 0 || q_h % 8 != 0) return KAIROS_ERR_ALIGN;
     if (B == 0) return KAIROS_OK;
     if (!Q || !O || !lens || (!page_table && table_width > 0) || ((uintptr_t)Q & 15) || ((uintptr_t)O & 15) ||
         ((uintptr_t)page_table & 3) || ((uintptr_t)lens & 3) || ((uintptr_t)LSE & 3))
@@ -895,7 +895,7 @@ extern "C" int kairos_paged_attention(const void* Q, const long long* q_strides,
     if (workspace_bytes < plan.bytes || (plan.bytes && (!workspace || ((uintptr_t)workspace & 15)))) return KAIROS_ERR_WORKSPACE;
     int* status = device_status_word();
     if (!status) return KAIROS_ERR_CUDA;
-    const AttnShape p = {q_strides[0], q_strides[1], table_stride, B, H, H / kv.heads, plan.blocks_per_kv, table_width,
+    const AttnShape p = {q_b, q_h, table_stride, B, H, H / kv.heads, plan.blocks_per_kv, table_width,
                          plan.workers, plan.joins ? 1 : 0, scale * kLog2e};
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (dtype == KAIROS_DTYPE_F16) {

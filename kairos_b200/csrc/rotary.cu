@@ -111,19 +111,20 @@ static int run_rotary(const void* X, void* Y, const void* positions, const void*
 
 }  // namespace kairos
 
-extern "C" int kairos_rotary(const void* X, const long long* x_strides, void* Y, const long long* y_strides,
-                             const void* positions, const long long* pos_strides, const kairos_rotary_plan* plan,
-                             int dtype, int transpose, int B, int S, int H, int D, kairos_stream_t stream) {
+extern "C" int kairos_rotary(const void* X, long long x_b, long long x_s, long long x_h, void* Y, long long y_b, long long y_s,
+                             long long y_h, const void* positions, long long pos_b, long long pos_s,
+                             const kairos_rotary_plan* plan, int dtype, int transpose, int B, int S, int H, int D,
+                             kairos_stream_t stream) {
     using namespace kairos;
     if (B < 0 || S < 0 || H < 0 || D <= 0 || D > 512) return KAIROS_ERR_SHAPE;
     if ((long long)B * S > 0x7fffffffLL) return KAIROS_ERR_SHAPE;      // one block per token at the least
-    if (!rotary_plan_ok(plan, D) || !x_strides || !y_strides || !pos_strides) return KAIROS_ERR_ARG;
+    if (!rotary_plan_ok(plan, D)) return KAIROS_ERR_ARG;
     if (B == 0 || S == 0 || H == 0) return KAIROS_OK;
     if (!X || !Y || !positions || ((uintptr_t)positions & 7)) return KAIROS_ERR_ALIGN;
     RotaryShape p = {};
-    p.xb = x_strides[0]; p.xs = x_strides[1]; p.xh = x_strides[2];
-    p.yb = y_strides[0]; p.ys = y_strides[1]; p.yh = y_strides[2];
-    p.pb = pos_strides[0]; p.ps = pos_strides[1];
+    p.xb = x_b; p.xs = x_s; p.xh = x_h;
+    p.yb = y_b; p.ys = y_s; p.yh = y_h;
+    p.pb = pos_b; p.ps = pos_s;
     p.tokens = (long long)B * S;
     p.S = S; p.H = H; p.D = D; p.rot = plan->rot; p.layout = plan->layout;
     p.magnitude = plan->magnitude;

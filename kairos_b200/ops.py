@@ -8,8 +8,6 @@ torch's current stream (the reference's GEMV/GEMM launch on the legacy default s
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from ._lib import check, lib
@@ -282,49 +280,66 @@ def silu_mul_quant(gate_up, want_f16=False, blocked=False):
 
 
 # ---- decoding over a paged key-value cache ----------------------------------------------------------
+# A call costs microseconds of host time, as much as the smallest kernels take, so the checks below ask each tensor for
+# as little as they can and tell what is wrong only once something is.
 _FLOATS = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
-_HALVES = (torch.float16, torch.bfloat16)
-_Three, _Two = ctypes.c_longlong * 3, ctypes.c_longlong * 2
+_HALVES = {torch.float16: 0, torch.bfloat16: 1}
+_empty, _int32, _int64, _float32 = torch.empty, torch.int32, torch.int64, torch.float32
 
 
-def _index(t, dtype, device, name):
-    if t.dtype != dtype or t.device != device or not t.is_contiguous():
-        raise ValueError(f'{name}: expected a contiguous tensor of {dtype} on {device}, got {t.dtype} on {t.device}')
-    return t.data_ptr()
+def _call(index, fn, *args):
+    """fn(*args, stream) on torch's current stream of device `index`."""
+    if index == _current_device():
+        return fn(*args, _raw_stream(index))
+    with torch.cuda.device(index):
+        return fn(*args, _raw_stream(index))
 
 
-def _same_device(device, other, name):
-    if not device.type == 'cuda' or other != device:
-        raise ValueError(f'{name} is on {other}, the activations are on {device}: expected one CUDA device')
+def _one_device(index, owner, name):
+    """The activations' device (-1: none) has to be the one of the cache or the plan."""
+    if index < 0 or index != owner:
+        raise ValueError(f'the activations are on CUDA device {index}, {name} is on {owner} (-1: not a CUDA device)')
 
 
-def _head_strides(t):
-    """Element strides of (batch, sequence, head) of [.., H, D]; a dimension of one element has none."""
-    s = [0 if n == 1 else st for n, st in zip(t.shape[:-1], t.stride()[:-1])]
-    return _Three(0, *s) if t.dim() == 3 else _Three(*s)
+def _bad(t, name, want, index):
+    return ValueError(f'{name}: expected {want} on CUDA device {index}, got {t.dtype} {tuple(t.shape)}, strides {t.stride()}, '
+                      f'on {t.device}')
 
 
 def rotary(x, positions, rotary, transpose=False, out=None):
     """Heads [T, H, D] or [B, S, H, D] (fp16, bf16 or fp32; dense last dimension, any other strides) turned by their
     int64 positions, [T] or broadcastable to [B, S], with the plan of a :class:`Rotary`.  ``transpose`` turns back with the same
     magnitude: the gradient of x from that of the result.  ``out`` may be x."""
-    if x.dtype not in _FLOATS or x.dim() not in (3, 4) or x.shape[-1] != rotary.head_dim or x.stride(-1) != 1:
-        raise ValueError(f'x: expected fp16, bf16 or fp32 [.., heads, {rotary.head_dim}] with a dense last dimension, '
-                         f'got {x.dtype} {tuple(x.shape)}')
-    _same_device(x.device, rotary.steps.device, 'rotary')
-    if positions.dtype != torch.int64 or positions.device != x.device:
-        raise ValueError(f'positions: expected int64 on {x.device}, got {positions.dtype} on {positions.device}')
+    shape, strides, code, index = x.shape, x.stride(), _FLOATS.get(x.dtype), x.get_device()
+    dims = len(shape)
+    if code is None or not 3 <= dims <= 4 or shape[-1] != rotary.head_dim or strides[-1] != 1:
+        raise _bad(x, 'x', f'fp16, bf16 or fp32 [.., heads, {rotary.head_dim}] with a dense last dimension', index)
+    if index < 0 or index != rotary.index:
+        _one_device(index, rotary.index, 'rotary')
+    if positions.dtype != _int64 or positions.get_device() != index:
+        raise _bad(positions, 'positions', 'int64', index)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1:
-        raise ValueError('out: expected the shape, type and device of x and a dense last dimension')
-    at = positions.expand(x.shape[:-2])
-    b, s = (1, x.shape[0]) if x.dim() == 3 else x.shape[:2]
-    ps = _Two(0, at.stride(0)) if x.dim() == 3 else _Two(*at.stride())
-    with _on(x.device):
-        check(lib.kairos_rotary(x.data_ptr(), _head_strides(x), out.data_ptr(), _head_strides(out), at.data_ptr(), ps,
-                                rotary.plan_ptr, _FLOATS[x.dtype], 1 if transpose else 0, b, s, x.shape[-2], x.shape[-1],
-                                stream_ptr()), 'rotary')
+        out = _empty(shape, dtype=x.dtype, device=x.device)
+    elif out.shape != shape or out.dtype != x.dtype or out.get_device() != index or out.stride(-1) != 1:
+        raise _bad(out, 'out', f'{x.dtype} {tuple(shape)} with a dense last dimension', index)
+    to, at = out.stride(), positions
+    if dims == 3:
+        b, (s, h, d) = 1, shape
+        if at.shape != (s,):
+            at = at.expand(s)
+        xs, ys, ps = (0, strides[0], strides[1]), (0, to[0], to[1]), (0, at.stride(0))
+    else:
+        b, s, h, d = shape
+        if at.shape != (b, s):
+            at = at.expand(b, s)
+        xs, ys, ps = strides[:3], to[:3], at.stride()
+    if b == 1 or s == 1 or h == 1:             # the stride of a dimension of one element may be anything: none
+        one = (b == 1, s == 1, h == 1)
+        xs, ys = ([0 if o else v for o, v in zip(one, t)] for t in (xs, ys))
+    rc = _call(index, lib.kairos_rotary, x.data_ptr(), *xs, out.data_ptr(), *ys, at.data_ptr(), *ps, rotary.plan_ptr, code,
+               1 if transpose else 0, b, s, h, d)
+    if rc < 0:
+        check(rc, 'rotary')
     return out
 
 
@@ -333,28 +348,28 @@ def rope_paged_kv(qkv, positions, slots, rotary, cache, layer=0, q_out=None):
     turned q heads [T, H, D], and stores the turned k heads and the v heads at ``slots`` [T] of the cache's `layer`, in
     the cache's type (int8 / e4m3 rows are quantized from fp32).  positions and slots are int64 [T]; a negative slot is
     padding and stores nothing; slots must be distinct."""
-    d, hkv = cache.head_dim, cache.kv_heads
-    if qkv.dtype not in _HALVES or qkv.dim() != 2 or qkv.shape[1] % d or (qkv.shape[1] and qkv.stride(1) != 1):
-        raise ValueError(f'qkv: expected fp16 or bf16 [tokens, heads * {d}] with dense rows, got {qkv.dtype} {tuple(qkv.shape)}')
-    t, h = qkv.shape[0], qkv.shape[1] // d - 2 * hkv
+    d, shape, code, index = cache.head_dim, qkv.shape, _HALVES.get(qkv.dtype), qkv.get_device()
+    if code is None or len(shape) != 2 or shape[1] % d or qkv.stride(1) != 1:
+        raise _bad(qkv, 'qkv', f'fp16 or bf16 [tokens, heads * {d}] with dense rows', index)
+    t, h = shape[0], shape[1] // d - 2 * cache.kv_heads
     if h <= 0 or rotary.head_dim != d:
-        raise ValueError(f'qkv has {qkv.shape[1] // d} heads of {d}: the cache holds {hkv} kv heads, the rotary plan turns '
-                         f'heads of {rotary.head_dim}')
-    dev = qkv.device
-    _same_device(dev, cache.device, 'cache')
-    _same_device(dev, rotary.steps.device, 'rotary')
-    if positions.numel() != t or slots.numel() != t:
-        raise ValueError(f'positions and slots: expected {t} each, got {positions.numel()} and {slots.numel()}')
+        raise ValueError(f'qkv has {shape[1] // d} heads of {d}: the cache holds {cache.kv_heads} kv heads, the rotary plan '
+                         f'turns heads of {rotary.head_dim}')
+    if index < 0 or index != cache.index or index != rotary.index:
+        _one_device(index, cache.index, 'cache')
+        _one_device(index, rotary.index, 'rotary')
+    if positions.dtype != _int64 or positions.get_device() != index or positions.shape != (t,) or not positions.is_contiguous():
+        raise _bad(positions, 'positions', f'contiguous int64 [{t}]', index)
+    if slots.dtype != _int64 or slots.get_device() != index or slots.shape != (t,) or not slots.is_contiguous():
+        raise _bad(slots, 'slots', f'contiguous int64 [{t}]', index)
     if q_out is None:
-        q_out = torch.empty((t, h, d), dtype=qkv.dtype, device=dev)
-    elif q_out.shape != (t, h, d) or q_out.dtype != qkv.dtype or q_out.device != dev or not q_out.is_contiguous():
-        raise ValueError(f'q_out: expected a contiguous {qkv.dtype} [{t}, {h}, {d}] on {dev}')
-    with _on(dev):
-        check(lib.kairos_rope_paged_kv(qkv.data_ptr(), qkv.stride(0) if t > 1 else qkv.shape[1],
-                                       _index(positions, torch.int64, dev, 'positions'),
-                                       _index(slots, torch.int64, dev, 'slots'), rotary.plan_ptr,
-                                       cache.layer_ptrs[layer], q_out.data_ptr(), t, h, _FLOATS[qkv.dtype], stream_ptr()),
-              'rope_paged_kv')
+        q_out = _empty((t, h, d), dtype=qkv.dtype, device=qkv.device)
+    elif q_out.shape != (t, h, d) or q_out.dtype != qkv.dtype or q_out.get_device() != index or not q_out.is_contiguous():
+        raise _bad(q_out, 'q_out', f'contiguous {qkv.dtype} [{t}, {h}, {d}]', index)
+    rc = _call(index, lib.kairos_rope_paged_kv, qkv.data_ptr(), qkv.stride(0) if t > 1 else shape[1], positions.data_ptr(),
+               slots.data_ptr(), rotary.plan_ptr, cache.layer_ptrs[layer], q_out.data_ptr(), t, h, code)
+    if rc < 0:
+        check(rc, 'rope_paged_kv')
     return q_out
 
 
@@ -362,20 +377,26 @@ def paged_kv_read(cache, slots, layer=0, dtype=torch.float16, out=None):
     """(k, v), each [T, kv_heads, D] of `dtype` (fp16, bf16 or fp32): what the cache's `layer` holds at ``slots`` (int64
     [T]), quantized rows as the values they stand for; zeros where the slot is negative.  ``out``: the two tensors to
     fill."""
-    if dtype not in _FLOATS:
+    code, index = _FLOATS.get(dtype), slots.get_device()
+    if code is None:
         raise ValueError(f'dtype: expected fp16, bf16 or fp32, got {dtype}')
-    dev = cache.device
-    _same_device(slots.device, dev, 'cache')
-    shape = (slots.numel(), cache.kv_heads, cache.head_dim)
+    if index < 0 or index != cache.index:
+        _one_device(index, cache.index, 'cache')
+    if slots.dtype != _int64 or slots.dim() != 1 or not slots.is_contiguous():
+        raise _bad(slots, 'slots', 'contiguous int64 [tokens]', index)
+    t = slots.shape[0]
+    shape = (t, cache.kv_heads, cache.head_dim)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
-    for o in out:
-        if o.shape != shape or o.dtype != dtype or o.device != dev or not o.is_contiguous():
-            raise ValueError(f'out: expected two contiguous {dtype} {shape} on {dev}')
-    with _on(dev):
-        check(lib.kairos_paged_kv_read(cache.layer_ptrs[layer], _index(slots, torch.int64, dev, 'slots'), out[0].data_ptr(),
-                                       out[1].data_ptr(), shape[0], _FLOATS[dtype], stream_ptr()), 'paged_kv_read')
-    return out
+        k, v = _empty(shape, dtype=dtype, device=slots.device), _empty(shape, dtype=dtype, device=slots.device)
+    else:
+        k, v = out
+        for o in (k, v):
+            if o.shape != shape or o.dtype != dtype or o.get_device() != index or not o.is_contiguous():
+                raise _bad(o, 'out', f'two contiguous {dtype} {shape}', index)
+    rc = _call(index, lib.kairos_paged_kv_read, cache.layer_ptrs[layer], slots.data_ptr(), k.data_ptr(), v.data_ptr(), t, code)
+    if rc < 0:
+        check(rc, 'paged_kv_read')
+    return k, v
 
 
 def paged_attention(q, cache, page_table, lens, layer=0, scale=None, out=None, return_lse=False):
@@ -384,30 +405,38 @@ def paged_attention(q, cache, page_table, lens, layer=0, scale=None, out=None, r
     behind the end are not read), lens int32 [B]; scale defaults to 1 / sqrt(D).  Returns o [B, H, D], with
     ``return_lse`` also the fp32 [B, H] logarithm of the softmax's denominator.  An empty sequence gives zeros and
     -inf."""
-    dev, d = q.device, cache.head_dim
-    if q.dtype not in _HALVES or q.dim() != 3 or q.shape[2] != d or q.stride(2) != 1:
-        raise ValueError(f'q: expected fp16 or bf16 [batch, heads, {d}] with a dense last dimension, got {q.dtype} {tuple(q.shape)}')
-    _same_device(dev, cache.device, 'cache')
-    b, h, _ = q.shape
-    if page_table.dim() != 2 or page_table.shape[0] != b or page_table.dtype != torch.int32 or \
-            page_table.device != dev or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise ValueError(f'page_table: expected int32 [{b}, pages] with dense rows on {dev}, got {page_table.dtype} '
-                         f'{tuple(page_table.shape)} on {page_table.device}')
-    if lens.numel() != b:
-        raise ValueError(f'lens: expected {b}, got {lens.numel()}')
+    shape, strides, code, index = q.shape, q.stride(), _HALVES.get(q.dtype), q.get_device()
+    if code is None or len(shape) != 3 or shape[2] != cache.head_dim or strides[2] != 1:
+        raise _bad(q, 'q', f'fp16 or bf16 [batch, heads, {cache.head_dim}] with a dense last dimension', index)
+    if index < 0 or index != cache.index:
+        _one_device(index, cache.index, 'cache')
+    b, h, d = shape
+    pages, steps = page_table.shape, page_table.stride()
+    if len(pages) != 2 or pages[0] != b or page_table.dtype != _int32 or page_table.get_device() != index or \
+            (steps[1] != 1 and pages[1] > 1):
+        raise _bad(page_table, 'page_table', f'int32 [{b}, pages] with dense rows', index)
+    if lens.dtype != _int32 or lens.get_device() != index or lens.shape != (b,) or not lens.is_contiguous():
+        raise _bad(lens, 'lens', f'contiguous int32 [{b}]', index)
+    device = q.device
     if out is None:
-        out = torch.empty((b, h, d), dtype=q.dtype, device=dev)
-    elif out.shape != (b, h, d) or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
-        raise ValueError(f'out: expected a contiguous {q.dtype} [{b}, {h}, {d}] on {dev}')
-    lse = torch.empty((b, h), dtype=torch.float32, device=dev) if return_lse else None
-    width, kv = page_table.shape[1], cache.layer_ptrs[layer]
-    with _on(dev):
-        need = lib.kairos_paged_attention_workspace_bytes(kv, b, h, width)
-        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None    # this call's own: see the header
-        check(lib.kairos_paged_attention(q.data_ptr(), _Two(q.stride(0) if b > 1 else 0, q.stride(1) if h > 1 else 0), kv,
-                                         page_table.data_ptr(), page_table.stride(0) if b > 1 else width, width,
-                                         _index(lens, torch.int32, dev, 'lens'), out.data_ptr(),
-                                         None if lse is None else lse.data_ptr(), b, h,
-                                         d ** -0.5 if scale is None else float(scale), _FLOATS[q.dtype],
-                                         None if ws is None else ws.data_ptr(), need, stream_ptr()), 'paged_attention')
+        out = _empty(shape, dtype=q.dtype, device=device)
+    elif out.shape != shape or out.dtype != q.dtype or out.get_device() != index or not out.is_contiguous():
+        raise _bad(out, 'out', f'contiguous {q.dtype} {tuple(shape)}', index)
+    lse = _empty((b, h), dtype=_float32, device=device) if return_lse else None
+    width, kv = pages[1], cache.layer_ptrs[layer]
+    key = (b, h, width)
+    need = cache.workspace_bytes.get(key)
+    if need is None:
+        if len(cache.workspace_bytes) > 4096:
+            cache.workspace_bytes.clear()
+        with torch.cuda.device(index):
+            need = cache.workspace_bytes[key] = lib.kairos_paged_attention_workspace_bytes(kv, b, h, width)
+    # scratch of this call alone: an allocation that is cached per stream, and private to a graph under capture
+    ws = _empty(need, dtype=torch.uint8, device=device) if need else None
+    rc = _call(index, lib.kairos_paged_attention, q.data_ptr(), strides[0] if b > 1 else 0, strides[1] if h > 1 else 0, kv,
+               page_table.data_ptr(), steps[0] if b > 1 else width, width, lens.data_ptr(), out.data_ptr(),
+               lse.data_ptr() if return_lse else None, b, h, d ** -0.5 if scale is None else scale, code,
+               ws.data_ptr() if need else None, need)
+    if rc < 0:
+        check(rc, 'paged_attention')
     return (out, lse) if return_lse else out

@@ -73,6 +73,9 @@ class PagedKVCache:
                                  self.num_pages, self.kv_heads, self.page_size, self.head_dim, KV_DTYPES[k.dtype])
                          for i in range(self.layers)]
         self.layer_ptrs = [ctypes.addressof(s) for s in self._structs]
+        # as the operators ask for it on every call
+        self.index = self.device.index if self.device.index is not None else -1
+        self.workspace_bytes = {}               # (batch, heads, table width) -> bytes of an attention call's scratch
         self._next, self._returned = 0, []      # pages never handed out start at _next
         self._pages = {}
 

@@ -41,6 +41,7 @@ class Rotary:
         turns = [int(round(f / (2 * math.pi) * 2.0 ** 64)) % (1 << 64) for f in self.frequencies.tolist()]
         signed = [t - (1 << 64) if t >= 1 << 63 else t for t in turns]
         self.steps = torch.tensor(signed, dtype=torch.int64, device=device)
+        self.index = self.steps.get_device() if self.steps.is_cuda else -1
         self.plan = RotaryPlan(self.steps.data_ptr(), self.magnitude, rot, LAYOUTS[layout])
         self.plan_ptr = ctypes.addressof(self.plan)
 

@@ -145,9 +145,8 @@ BAD_LAYERS = [(dict(pages=0), SHAPE), (dict(kv_heads=-1), SHAPE), (dict(page_siz
 
 
 def attention(kv, q=P, strides=(256, 64), table=P, table_stride=4, width=4, lens=P, o=P, lse=None, b=2, h=4, dtype=0, ws=P, wsb=1 << 30):
-    st = (ctypes.c_longlong * 2)(*strides)
-    return lib.kairos_paged_attention(q, ctypes.cast(st, ctypes.c_void_p), ctypes.addressof(kv), table, table_stride, width,
-                                      lens, o, lse, b, h, 1.0, dtype, ws, wsb, None)
+    return lib.kairos_paged_attention(q, *strides, ctypes.addressof(kv), table, table_stride, width, lens, o, lse, b, h, 1.0,
+                                      dtype, ws, wsb, None)
 
 
 def write(kv, qkv=P, stride=512, pos=P, slots=P, plan=(P, 1.0, 64, 0), q=P, t=3, h=4, dtype=0):
@@ -156,9 +155,8 @@ def write(kv, qkv=P, stride=512, pos=P, slots=P, plan=(P, 1.0, 64, 0), q=P, t=3,
 
 
 def turn(x=P, y=P, pos=P, plan=(P, 1.0, 64, 0), dtype=0, b=1, s=3, h=4, d=64):
-    pl, st3, st2 = _lib.RotaryPlan(*plan), (ctypes.c_longlong * 3)(0, 256, 64), (ctypes.c_longlong * 2)(0, 1)
-    a = ctypes.addressof
-    return lib.kairos_rotary(x, a(st3), y, a(st3), pos, a(st2), a(pl), dtype, 0, b, s, h, d, None)
+    pl = _lib.RotaryPlan(*plan)
+    return lib.kairos_rotary(x, 0, 256, 64, y, 0, 256, 64, pos, 0, 1, ctypes.addressof(pl), dtype, 0, b, s, h, d, None)
 
 
 @pytest.mark.parametrize('kw,code', BAD_LAYERS)
