@@ -63,129 +63,158 @@ struct CodesE4M3 {
 struct WriteShape {
     long long row_stride;
     int T, H, rot, layout, tokens_per_block;
+    unsigned by_heads, by_pairs;                // div_magic of H + 2 kv heads and rot / 2
     float magnitude;
 };
 
-// Codes = void: the cache holds the activation's own type.  One block takes `tokens_per_block` tokens: their angles go
-// to shared memory once, then every thread moves cells of 16 elements; the D / 16 threads of a row are neighbours in
-// one warp, so the row's maximum is a few shuffles.
+// Codes = void: the cache holds the activation's own type.  One block takes `tokens_per_block` tokens; the D / 16 cells of
+// a row go to neighbouring threads of one warp, so the row's maximum is a few shuffles.  A thread requests its first cells
+// before the block computes the tokens' angles, once for all heads, into shared memory.
 template <typename T, typename Codes, int D>
-__global__ void __launch_bounds__(256) rope_paged_kv_kernel(const T* __restrict__ QKV, const long long* __restrict__ positions,
+__global__ void __launch_bounds__(256, 3) rope_paged_kv_kernel(const T* __restrict__ QKV, const long long* __restrict__ positions,
                                                             const long long* __restrict__ slots,
                                                             const unsigned long long* __restrict__ steps, const KvView kv,
                                                             T* __restrict__ Q, const WriteShape p, int* status) {
-    constexpr int kLanes = D / 16;
+    constexpr int kLanes = D / 16, kStep = 256 / kLanes, kU = kCells<T>;
     __shared__ __align__(16) float cs[kTablePairs], sn[kTablePairs];
     chain_release();
     chain_wait();
     const int t0 = blockIdx.x * p.tokens_per_block;
     const int here = min(p.tokens_per_block, p.T - t0);
-    const int pairs = p.rot >> 1;
-    for (int i = threadIdx.x; i < here * pairs; i += 256) {
-        const int t = i / pairs, pair = i - t * pairs;
-        float c, s;
-        turn_of(__ldcg(positions + t0 + t), __ldg(steps + pair), p.magnitude, &c, &s);
-        cs[i] = c;
-        sn[i] = s;
-    }
-    __syncthreads();
-    const int heads = p.H + 2 * kv.heads;
-    const int total = here * heads * kLanes;
+    const int pairs = p.rot >> 1, heads = p.H + 2 * kv.heads, rows = here * heads;
     const long long capacity = (long long)kv.pages << kv.page_shift;
-    for (int base = 0; base < total; base += 256) {        // whole warps stay together for the shuffles
-        const int i = base + threadIdx.x;
-        const bool live = i < total;
-        const int row = (live ? i : 0) / kLanes, j = i % kLanes;
-        const int t = row / heads, head = row - t * heads;
-        const T* x = QKV + (size_t)(t0 + t) * p.row_stride + (size_t)head * D;
-        const Cell cell = cell_of(j, p.rot, p.layout);
-        float a[8], b[8];
-        load8(x + cell.first, a);
-        load8(x + cell.second, b);
-        if (cell.pair >= 0 && head < p.H + kv.heads) turn_cell(a, b, cs + t * pairs, sn + t * pairs, cell.pair, p.layout);
-        float amax = 0.f;
-        if constexpr (!std::is_void<Codes>::value) amax = row_amax(a, b, kLanes);
-        if (!live) continue;
-        if (head < p.H) {
-            T* q = Q + ((size_t)(t0 + t) * p.H + head) * D;
-            store8(q + cell.first, a);
-            store8(q + cell.second, b);
-            continue;
+    const int at = threadIdx.x / kLanes, j = threadIdx.x % kLanes;
+    const Cell cell = cell_of(j, p.rot, p.layout);
+    for (int base = 0; base < rows; base += kU * kStep) {
+        RawCell<T> raw[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int r = min(base + u * kStep + at, rows - 1), t = div_small(r, p.by_heads);      // whole warps stay together
+            raw[u].load(QKV + (size_t)(t0 + t) * p.row_stride + (size_t)(r - t * heads) * D, cell);
         }
-        const long long slot = __ldcg(slots + t0 + t);
-        if (slot < 0) continue;                            // padding
-        if (slot >= capacity) {
-            *status = KAIROS_ERR_ARG;
-            continue;
-        }
-        const bool is_v = head >= p.H + kv.heads;
-        const size_t r = pool_row(kv, slot, head - p.H - (is_v ? kv.heads : 0));
-        if constexpr (std::is_void<Codes>::value) {
-            T* y = static_cast<T*>(is_v ? kv.v : kv.k) + r * D;
-            store8(y + cell.first, a);
-            store8(y + cell.second, b);
-        } else {
-            float scale = __fdiv_rn(amax, Codes::kTop);
-            uint2 qa = make_uint2(0, 0), qb = qa;
-            if (scale > 0.f) {                             // false for a row of zeros and for NaN: codes 0
-                const float inv = __frcp_rn(scale);
-                qa = Codes::encode(a, scale, inv);
-                qb = Codes::encode(b, scale, inv);
+        if (base == 0) {
+            for (int i = threadIdx.x; i < here * pairs; i += 256) {
+                const int t = div_small(i, p.by_pairs), pair = i - t * pairs;
+                float c, s;
+                turn_of(__ldcg(positions + t0 + t), __ldg(steps + pair), p.magnitude, &c, &s);
+                cs[i] = c;
+                sn[i] = s;
             }
-            uint8_t* y = static_cast<uint8_t*>(is_v ? kv.v : kv.k) + r * D;
-            *reinterpret_cast<uint2*>(y + cell.first) = qa;
-            *reinterpret_cast<uint2*>(y + cell.second) = qb;
-            if (j == 0) (is_v ? kv.vs : kv.ks)[r] = scale;
+            __syncthreads();
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int r = base + u * kStep + at;
+            const bool live = r < rows;
+            const int t = div_small(min(r, rows - 1), p.by_heads), head = min(r, rows - 1) - t * heads;
+            float a[8], b[8];
+            RawCell<T>::widen(raw[u].w[0], a);
+            RawCell<T>::widen(raw[u].w[1], b);
+            if (cell.pair >= 0 && head < p.H + kv.heads) turn_cell(a, b, cs + t * pairs, sn + t * pairs, cell.pair, p.layout);
+            float amax = 0.f;
+            if constexpr (!std::is_void<Codes>::value) amax = row_amax(a, b, kLanes);
+            if (!live) continue;
+            if (head < p.H) {
+                T* q = Q + ((size_t)(t0 + t) * p.H + head) * D;
+                store8(q + cell.first, a);
+                store8(q + cell.second, b);
+                continue;
+            }
+            const long long slot = __ldcg(slots + t0 + t);
+            if (slot < 0) continue;                        // padding
+            if (slot >= capacity) {
+                *status = KAIROS_ERR_ARG;
+                continue;
+            }
+            const bool is_v = head >= p.H + kv.heads;
+            const size_t to = pool_row(kv, slot, head - p.H - (is_v ? kv.heads : 0));
+            if constexpr (std::is_void<Codes>::value) {
+                T* y = static_cast<T*>(is_v ? kv.v : kv.k) + to * D;
+                store8(y + cell.first, a);
+                store8(y + cell.second, b);
+            } else {
+                const float scale = __fdiv_rn(amax, Codes::kTop);
+                uint2 qa = make_uint2(0, 0), qb = qa;
+                if (scale > 0.f) {                         // false for a row of zeros and for NaN: codes 0
+                    const float inv = __frcp_rn(scale);
+                    qa = Codes::encode(a, scale, inv);
+                    qb = Codes::encode(b, scale, inv);
+                }
+                uint8_t* y = static_cast<uint8_t*>(is_v ? kv.v : kv.k) + to * D;
+                *reinterpret_cast<uint2*>(y + cell.first) = qa;
+                *reinterpret_cast<uint2*>(y + cell.second) = qb;
+                if (j == 0) (is_v ? kv.vs : kv.ks)[to] = scale;
+            }
         }
     }
 }
 
-// One thread brings the same eight channels of a K row and of its V row.
+// One thread brings the same eight channels of a K row and of its V row, of two rows half the grid apart, so that four
+// independent rows are under way.
 template <typename C, typename Codes, typename T>
 __global__ void __launch_bounds__(256) paged_kv_read_kernel(const KvView kv, const long long* __restrict__ slots,
-                                                            T* __restrict__ K, T* __restrict__ V, long long total,
-                                                            int* status) {
+                                                            T* __restrict__ K, T* __restrict__ V, int total, int half,
+                                                            unsigned by_heads, int* status) {
+    constexpr bool kCoded = !std::is_void<Codes>::value;
     chain_release();
     chain_wait();
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= total) return;
-    const int chunks = kv.dim >> 3;
-    const int c = (int)(i % chunks);
-    const long long row = i / chunks;
-    const int head = (int)(row % kv.heads);
-    const long long slot = __ldcg(slots + row / kv.heads);
-    float k[8] = {}, v[8] = {};
-    if (slot >= 0 && slot < ((long long)kv.pages << kv.page_shift)) {
-        const size_t r = pool_row(kv, slot, head);
-        if constexpr (std::is_void<Codes>::value) {
-            load8(static_cast<const C*>(kv.k) + r * kv.dim + 8 * c, k);
-            load8(static_cast<const C*>(kv.v) + r * kv.dim + 8 * c, v);
-        } else {
-            const uint2 kc = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(kv.k) + r * kv.dim) + c);
-            const uint2 vc = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(kv.v) + r * kv.dim) + c);
-            const float ks = __ldcg(kv.ks + r), vs = __ldcg(kv.vs + r);
-            Codes::decode(kc, k);
-            Codes::decode(vc, v);
+    const int chunk_shift = kv.dim == 64 ? 3 : kv.dim == 128 ? 4 : 5;
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= half) return;
+    const int c = 8 * (i & ((1 << chunk_shift) - 1));
+    const long long capacity = (long long)kv.pages << kv.page_shift;
+    uint4 kw[2], vw[2];
+    float ks[2] = {}, vs[2] = {};
+    bool there[2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                k[e] *= ks;
-                v[e] *= vs;
+    for (int u = 0; u < 2; ++u) {
+        const int row = (i + u * half) >> chunk_shift;
+        const bool mine = i + u * half < total;
+        const int token = by_heads ? (int)__umulhi((unsigned)row, by_heads) : row;
+        const long long slot = mine ? __ldcg(slots + token) : -1;
+        there[u] = slot >= 0 && slot < capacity;
+        if (slot >= capacity) *status = KAIROS_ERR_ARG;
+        kw[u] = vw[u] = make_uint4(0, 0, 0, 0);
+        if (there[u]) {
+            const size_t r = pool_row(kv, slot, row - token * kv.heads);
+            if constexpr (kCoded) {
+                const uint2 x = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(kv.k) + r * kv.dim + c));
+                const uint2 y = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(kv.v) + r * kv.dim + c));
+                kw[u].x = x.x, kw[u].y = x.y, vw[u].x = y.x, vw[u].y = y.y;
+                ks[u] = __ldcg(kv.ks + r), vs[u] = __ldcg(kv.vs + r);
+            } else {
+                kw[u] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const C*>(kv.k) + r * kv.dim + c));
+                vw[u] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const C*>(kv.v) + r * kv.dim + c));
             }
         }
-    } else if (slot >= 0) {
-        *status = KAIROS_ERR_ARG;
     }
-    store8(K + row * kv.dim + 8 * c, k);
-    store8(V + row * kv.dim + 8 * c, v);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        if (i + u * half >= total) break;
+        const size_t to = (size_t)(i + u * half) * 8;
+        auto put8 = [&](const uint4& w, float scale, T* out) {
+            float f[8];
+            if constexpr (kCoded) {
+                Codes::decode(make_uint2(w.x, w.y), f);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] *= scale;
+            } else {
+                const uint4 one[1] = {w};
+                RawCell<C>::widen(one, f);
+            }
+            store8(out + to, f);
+        };
+        put8(kw[u], ks[u], K);
+        put8(vw[u], vs[u], V);
+    }
 }
 
 template <typename T, typename Codes, int D>
 static int run_write(const void* QKV, const void* positions, const void* slots, const void* steps, const KvView& kv, void* Q,
                      WriteShape p, int* status, cudaStream_t st) {
-    const int cells = (p.H + 2 * kv.heads) * (D / 16);
-    int tb = cells >= 256 ? 1 : (256 + cells - 1) / cells;
-    if (p.rot) tb = min(tb, kTablePairs / (p.rot / 2));
-    p.tokens_per_block = max(1, tb);
+    p.tokens_per_block = rows_tokens(p.T, p.H + 2 * kv.heads, p.rot);
+    p.by_heads = div_magic(p.H + 2 * kv.heads);
+    p.by_pairs = div_magic(max(1, p.rot / 2));
     const cudaError_t e = launch_chained(
         rope_paged_kv_kernel<T, Codes, D>, dim3((unsigned)((p.T + p.tokens_per_block - 1) / p.tokens_per_block)), dim3(256), 0,
         st, static_cast<const T*>(QKV), static_cast<const long long*>(positions), static_cast<const long long*>(slots),
@@ -204,13 +233,18 @@ static int pick_write(const void* QKV, const void* positions, const void* slots,
 
 template <typename C, typename Codes, typename T>
 static int run_read(const KvView& kv, const void* slots, void* K, void* V, long long T_, int* status, cudaStream_t st) {
-    const long long total = T_ * kv.heads * (kv.dim / 8);
-    const long long blocks = (total + 255) / 256;
-    if (blocks > 0x7fffffffLL) return KAIROS_ERR_SHAPE;
-    const cudaError_t e = launch_chained(paged_kv_read_kernel<C, Codes, T>, dim3((unsigned)blocks), dim3(256), 0, st, kv,
-                                         static_cast<const long long*>(slots), static_cast<T*>(K), static_cast<T*>(V), total,
-                                         status);
-    if (e != cudaSuccess) return note_cuda_error(e);
+    // whole tokens a launch, so that 32-bit indexes and the division by a multiplication are exact (rows * heads < 2^32)
+    const long long per_token = (long long)kv.heads * (kv.dim / 8);
+    const long long most = max(1LL, min((1LL << 30) / per_token, (long long)0xffffffffLL / kv.heads / kv.heads));
+    for (long long t0 = 0; t0 < T_; t0 += most) {
+        const int total = (int)(min(most, T_ - t0) * per_token);
+        const int half = ((total / 2 + 255) & ~255) + (total < 512 ? total : 0);
+        const cudaError_t e = launch_chained(paged_kv_read_kernel<C, Codes, T>, dim3((min(half, total) + 255) / 256), dim3(256), 0, st,
+                                             kv, static_cast<const long long*>(slots) + t0,
+                                             static_cast<T*>(K) + t0 * kv.heads * kv.dim, static_cast<T*>(V) + t0 * kv.heads * kv.dim,
+                                             total, min(half, total), div_magic(kv.heads), status);
+        if (e != cudaSuccess) return note_cuda_error(e);
+    }
     return launch_status();
 }
 
@@ -237,7 +271,7 @@ extern "C" int kairos_rope_paged_kv(const void* QKV, long long row_stride, const
     const int rc = kv_view(layer, &kv);
     if (rc != KAIROS_OK) return rc;
     if (T < 0 || H <= 0 || row_stride % 8 != 0 || row_stride < (long long)(H + 2LL * kv.heads) * kv.dim) return KAIROS_ERR_SHAPE;
-    if ((H + 2LL * kv.heads) * kv.dim > (1 << 24)) return KAIROS_ERR_SHAPE;
+    if (H + 2LL * kv.heads >= 65536) return KAIROS_ERR_SHAPE;
     if (!rotary_plan_ok(plan, kv.dim) || plan->rot % 16 != 0) {
         set_last_error("rope_paged_kv: the rotated part is a multiple of 16 channels, at most the head");
         return KAIROS_ERR_ARG;

@@ -14,9 +14,9 @@ inline int kv_view(const kairos_kv_layer* kv, KvView* out) {
     if (!kv) return KAIROS_ERR_ARG;
     int shift = 0;
     while (shift < 8 && (1 << shift) != kv->page_size) ++shift;
-    if (kv->pages <= 0 || kv->kv_heads <= 0 || shift < 4 || (1 << shift) != kv->page_size ||
+    if (kv->pages <= 0 || kv->kv_heads <= 0 || kv->kv_heads > 65535 || shift < 4 || (1 << shift) != kv->page_size ||
         (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256)) {
-        set_last_error("paged cache: pages and kv_heads > 0, page_size 16, 32, 64, 128 or 256, head_dim 64, 128 or 256");
+        set_last_error("paged cache: pages and kv_heads > 0 (kv_heads < 65536), page_size 16, 32, 64, 128 or 256, head_dim 64, 128 or 256");
         return KAIROS_ERR_SHAPE;
     }
     if (!kv->k || !kv->v || ((uintptr_t)kv->k & 15) || ((uintptr_t)kv->v & 15)) return KAIROS_ERR_ALIGN;

@@ -6,45 +6,64 @@ namespace kairos {
 
 struct RotaryShape {
     long long xb, xs, xh, yb, ys, yh, pb, ps;   // element strides of X, Y and the positions
-    long long tokens;                            // B * S
+    long long tokens;                            // B * S, below 2^31
     int S, H, D, rot, layout, tokens_per_block;
+    unsigned by_heads, by_pairs, by_lanes;       // div_magic of H, rot / 2, D / 16
     float magnitude, sign;
 };
 
-// One block turns `tokens_per_block` tokens: their angles go to shared memory once, then every thread moves cells.
+// One block turns `tokens_per_block` tokens.  A row's D / 16 cells go to neighbouring threads; a thread requests its first
+// cells before the block computes the tokens' angles, once for all heads, into shared memory.
 template <typename T>
 __global__ void __launch_bounds__(256) rotary_kernel(const T* X, T* Y, const long long* __restrict__ positions,
                                                      const unsigned long long* __restrict__ steps, const RotaryShape p) {
+    constexpr int kU = kCells<T>;
     __shared__ __align__(16) float cs[kTablePairs], sn[kTablePairs];
     chain_release();
     chain_wait();
     const long long t0 = (long long)blockIdx.x * p.tokens_per_block;
     const int here = (int)min((long long)p.tokens_per_block, p.tokens - t0);
-    const int pairs = p.rot >> 1;
-    for (int i = threadIdx.x; i < here * pairs; i += 256) {
-        const int t = i / pairs, pair = i - t * pairs;
-        const long long b = (t0 + t) / p.S, s = (t0 + t) - b * p.S;
-        float c, sv;
-        turn_of(__ldcg(positions + b * p.pb + s * p.ps), __ldg(steps + pair), p.magnitude, &c, &sv);
-        cs[i] = c;
-        sn[i] = sv * p.sign;
-    }
-    __syncthreads();
-    const int per_row = p.D >> 4;
-    const int per_token = p.H * per_row;
-    for (int i = threadIdx.x; i < here * per_token; i += 256) {
-        const int t = i / per_token, k = i - t * per_token;
-        const int h = k / per_row, j = k - h * per_row;
-        const long long b = (t0 + t) / p.S, s = (t0 + t) - b * p.S;
-        const T* x = X + b * p.xb + s * p.xs + h * p.xh;
-        T* y = Y + b * p.yb + s * p.ys + h * p.yh;
-        const Cell cell = cell_of(j, p.rot, p.layout);
-        float a[8], c[8];
-        load8(x + cell.first, a);
-        load8(x + cell.second, c);
-        if (cell.pair >= 0) turn_cell(a, c, cs + t * pairs, sn + t * pairs, cell.pair, p.layout);
-        store8(y + cell.first, a);
-        store8(y + cell.second, c);
+    const int pairs = p.rot >> 1, lanes = p.D >> 4, rows = here * p.H;
+    const int at = div_small((int)threadIdx.x, p.by_lanes), j = (int)threadIdx.x - at * lanes;
+    const int step = div_small(256, p.by_lanes);        // rows in one go; threads behind the last whole row idle
+    const bool idle = at >= step;
+    const Cell cell = cell_of(j, p.rot, p.layout);
+    auto place = [&](int r, long long sb, long long ss, long long sh) {
+        const int t = div_small(r, p.by_heads);
+        const long long token = t0 + t, b = p.S == p.tokens ? 0 : (unsigned)token / (unsigned)p.S;
+        return b * sb + (token - b * p.S) * ss + (r - t * p.H) * sh;
+    };
+    for (int base = 0; base < rows; base += kU * step) {
+        RawCell<T> raw[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int r = base + u * step + at;
+            if (r < rows && !idle) raw[u].load(X + place(r, p.xb, p.xs, p.xh), cell);
+        }
+        if (base == 0) {
+            for (int i = threadIdx.x; i < here * pairs; i += 256) {
+                const int t = div_small(i, p.by_pairs), pair = i - t * pairs;
+                const long long token = t0 + t, b = p.S == p.tokens ? 0 : (unsigned)token / (unsigned)p.S;
+                float c, s;
+                turn_of(__ldcg(positions + b * p.pb + (token - b * p.S) * p.ps), __ldg(steps + pair), p.magnitude, &c, &s);
+                cs[i] = c;
+                sn[i] = s * p.sign;
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int r = base + u * step + at;
+            if (r >= rows || idle) continue;
+            float a[8], b[8];
+            RawCell<T>::widen(raw[u].w[0], a);
+            RawCell<T>::widen(raw[u].w[1], b);
+            const int t = div_small(r, p.by_heads);
+            if (cell.pair >= 0) turn_cell(a, b, cs + t * pairs, sn + t * pairs, cell.pair, p.layout);
+            T* y = Y + place(r, p.yb, p.ys, p.yh);
+            store8(y + cell.first, a);
+            store8(y + cell.second, b);
+        }
     }
 }
 
@@ -84,7 +103,7 @@ __global__ void __launch_bounds__(256) rotary_scalar_kernel(const T* X, T* Y, co
 template <typename T>
 static int run_rotary(const void* X, void* Y, const void* positions, const void* steps, RotaryShape p, cudaStream_t st) {
     const int per16 = 16 / (int)sizeof(T);
-    const bool wide = (p.D % 16) == 0 && (p.rot % 16) == 0 && ((uintptr_t)X & 15) == 0 && ((uintptr_t)Y & 15) == 0 &&
+    const bool wide = p.H < 65536 && (p.D % 16) == 0 && (p.rot % 16) == 0 && ((uintptr_t)X & 15) == 0 && ((uintptr_t)Y & 15) == 0 &&
                       p.xb % per16 == 0 && p.xs % per16 == 0 && p.xh % per16 == 0 && p.yb % per16 == 0 &&
                       p.ys % per16 == 0 && p.yh % per16 == 0;
     const T* x = static_cast<const T*>(X);
@@ -93,11 +112,10 @@ static int run_rotary(const void* X, void* Y, const void* positions, const void*
     const unsigned long long* st64 = static_cast<const unsigned long long*>(steps);
     cudaError_t e;
     if (wide) {
-        // a block has at least 256 cells where the heads of one token are few, and its angles fit its table
-        const int cells = p.H * (p.D / 16);
-        int tb = cells >= 256 ? 1 : (256 + cells - 1) / cells;
-        if (p.rot) tb = min(tb, kTablePairs / (p.rot / 2));
-        p.tokens_per_block = max(1, tb);
+        p.tokens_per_block = rows_tokens(p.tokens, p.H, p.rot);
+        p.by_heads = div_magic(p.H);
+        p.by_pairs = div_magic(max(1, p.rot / 2));
+        p.by_lanes = div_magic(p.D / 16);
         const long long blocks = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
         e = launch_chained(rotary_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, x, y, pos, st64, p);
     } else {

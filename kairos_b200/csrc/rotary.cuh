@@ -3,6 +3,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace kairos {
@@ -115,7 +117,55 @@ __device__ __forceinline__ void turn_cell(float (&a)[8], float (&b)[8], const fl
     }
 }
 
+// The 16 elements of a cell as they come from memory: a thread requests several cells before it turns the first.
+template <typename T>
+struct RawCell {
+    static constexpr int kWords = 8 * (int)sizeof(T) / 16;     // 16-byte words of a chunk
+    uint4 w[2][kWords];
+    __device__ __forceinline__ void load(const T* row, const Cell& c) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            w[0][i] = __ldcg(reinterpret_cast<const uint4*>(row + c.first) + i);
+            w[1][i] = __ldcg(reinterpret_cast<const uint4*>(row + c.second) + i);
+        }
+    }
+    static __device__ __forceinline__ void widen(const uint4 (&x)[kWords], float (&f)[8]) {
+        const uint32_t* v = reinterpret_cast<const uint32_t*>(x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                f[2 * i] = __uint_as_float(v[2 * i]);
+                f[2 * i + 1] = __uint_as_float(v[2 * i + 1]);
+            } else if constexpr (std::is_same<T, __half>::value) {
+                const float2 t = __half22float2(*reinterpret_cast<const __half2*>(v + i));
+                f[2 * i] = t.x;
+                f[2 * i + 1] = t.y;
+            } else {
+                f[2 * i] = __uint_as_float(v[i] << 16);
+                f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+            }
+        }
+    }
+};
+// Cells that a thread has under way: 128 bytes of loads.
+template <typename T>
+constexpr int kCells = sizeof(T) == 4 ? 2 : 4;
+
 constexpr int kTablePairs = 2048;   // pairs whose cos and sin a block keeps: 16 KB of shared memory
+
+// i / d for i, d below 2^16 by one multiplication; `magic` = ceil(2^32 / d).
+inline unsigned div_magic(int d) { return d == 1 ? 0u : (unsigned)((0x100000000ull + d - 1) / d); }
+__device__ __forceinline__ int div_small(int i, unsigned magic) { return magic ? (int)__umulhi((unsigned)i, magic) : i; }
+
+// Tokens of a block: about 256 rows (heads of tokens), which fills its threads' cells whatever the number of heads, where
+// there are enough tokens for every SM to have two such blocks; else one token, so that a decode step spreads over the
+// SMs.  The angles of a block's tokens fit its table.
+inline int rows_tokens(long long tokens, int rows, int rot) {
+    int tb = rows >= 256 ? 1 : 256 / rows;
+    if (tokens * rows < 2 * 148 * 256) tb = 1;
+    if (rot) tb = min(tb, kTablePairs / (rot / 2));
+    return max(1, min(tb, 64));
+}
 
 inline bool rotary_plan_ok(const kairos_rotary_plan* p, int D) {
     return p && p->rot >= 0 && p->rot <= D && (p->rot & 1) == 0 && (p->layout == 0 || p->layout == 1) &&

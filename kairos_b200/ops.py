@@ -284,7 +284,7 @@ def silu_mul_quant(gate_up, want_f16=False, blocked=False):
 # as little as they can and tell what is wrong only once something is.
 _FLOATS = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _HALVES = {torch.float16: 0, torch.bfloat16: 1}
-_empty, _int32, _int64, _float32 = torch.empty, torch.int32, torch.int64, torch.float32
+_int32, _int64 = torch.int32, torch.int64
 
 
 def _call(index, fn, *args):
@@ -319,7 +319,7 @@ def rotary(x, positions, rotary, transpose=False, out=None):
     if positions.dtype != _int64 or positions.get_device() != index:
         raise _bad(positions, 'positions', 'int64', index)
     if out is None:
-        out = _empty(shape, dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x)
     elif out.shape != shape or out.dtype != x.dtype or out.get_device() != index or out.stride(-1) != 1:
         raise _bad(out, 'out', f'{x.dtype} {tuple(shape)} with a dense last dimension', index)
     to, at = out.stride(), positions
@@ -363,7 +363,7 @@ def rope_paged_kv(qkv, positions, slots, rotary, cache, layer=0, q_out=None):
     if slots.dtype != _int64 or slots.get_device() != index or slots.shape != (t,) or not slots.is_contiguous():
         raise _bad(slots, 'slots', f'contiguous int64 [{t}]', index)
     if q_out is None:
-        q_out = _empty((t, h, d), dtype=qkv.dtype, device=qkv.device)
+        q_out = qkv.new_empty((t, h, d))
     elif q_out.shape != (t, h, d) or q_out.dtype != qkv.dtype or q_out.get_device() != index or not q_out.is_contiguous():
         raise _bad(q_out, 'q_out', f'contiguous {qkv.dtype} [{t}, {h}, {d}]', index)
     rc = _call(index, lib.kairos_rope_paged_kv, qkv.data_ptr(), qkv.stride(0) if t > 1 else shape[1], positions.data_ptr(),
@@ -387,7 +387,8 @@ def paged_kv_read(cache, slots, layer=0, dtype=torch.float16, out=None):
     t = slots.shape[0]
     shape = (t, cache.kv_heads, cache.head_dim)
     if out is None:
-        k, v = _empty(shape, dtype=dtype, device=slots.device), _empty(shape, dtype=dtype, device=slots.device)
+        k = slots.new_empty(shape, dtype=dtype)
+        v = torch.empty_like(k)
     else:
         k, v = out
         for o in (k, v):
@@ -417,12 +418,11 @@ def paged_attention(q, cache, page_table, lens, layer=0, scale=None, out=None, r
         raise _bad(page_table, 'page_table', f'int32 [{b}, pages] with dense rows', index)
     if lens.dtype != _int32 or lens.get_device() != index or lens.shape != (b,) or not lens.is_contiguous():
         raise _bad(lens, 'lens', f'contiguous int32 [{b}]', index)
-    device = q.device
     if out is None:
-        out = _empty(shape, dtype=q.dtype, device=device)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     elif out.shape != shape or out.dtype != q.dtype or out.get_device() != index or not out.is_contiguous():
         raise _bad(out, 'out', f'contiguous {q.dtype} {tuple(shape)}', index)
-    lse = _empty((b, h), dtype=_float32, device=device) if return_lse else None
+    lse = q.new_empty((b, h), dtype=torch.float32) if return_lse else None
     width, kv = pages[1], cache.layer_ptrs[layer]
     key = (b, h, width)
     need = cache.workspace_bytes.get(key)
@@ -432,7 +432,7 @@ def paged_attention(q, cache, page_table, lens, layer=0, scale=None, out=None, r
         with torch.cuda.device(index):
             need = cache.workspace_bytes[key] = lib.kairos_paged_attention_workspace_bytes(kv, b, h, width)
     # scratch of this call alone: an allocation that is cached per stream, and private to a graph under capture
-    ws = _empty(need, dtype=torch.uint8, device=device) if need else None
+    ws = page_table.new_empty(need >> 2) if need else None
     rc = _call(index, lib.kairos_paged_attention, q.data_ptr(), strides[0] if b > 1 else 0, strides[1] if h > 1 else 0, kv,
                page_table.data_ptr(), steps[0] if b > 1 else width, width, lens.data_ptr(), out.data_ptr(),
                lse.data_ptr() if return_lse else None, b, h, d ** -0.5 if scale is None else scale, code,
