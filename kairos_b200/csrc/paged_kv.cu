@@ -7,26 +7,35 @@
 
 namespace kairos {
 
-// Largest magnitude of a row held by `lanes` consecutive threads (a power of two, aligned), 16 values each;
-// NaN if the row has an infinity or a NaN.
+// Largest magnitude of a row held by `lanes` consecutive threads (a power of two, aligned), 16 values each; NaN if the row
+// has an infinity or a NaN.  Magnitudes are compared as bit patterns, in whose order infinities and NaN are the largest.
 __device__ __forceinline__ float row_amax(const float (&a)[8], const float (&b)[8], int lanes) {
-    float m = 0.f;
+    unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, fmaxf(fabsf(a[i]), fabsf(b[i])));
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) bad |= !(fabsf(a[i]) <= FLT_MAX) | !(fabsf(b[i]) <= FLT_MAX);
-    if (bad) m = __int_as_float(0x7f800000);
-    for (int o = lanes >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    return m <= FLT_MAX ? m : __int_as_float(0x7fffffff);
+    for (int i = 0; i < 8; ++i) m = max(m, max(__float_as_uint(a[i]) & 0x7fffffffu, __float_as_uint(b[i]) & 0x7fffffffu));
+    for (int o = lanes >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return __uint_as_float(m < 0x7f800000u ? m : 0x7fffffffu);
 }
 
+// Codes of eight values: the nearest of x / scale, as IEEE division rounds it.  x * inv is within 3 * 2^-24 of the quotient,
+// relative to it, so both round alike unless the product lies next to a border between two codes; a chunk with such a
+// value (or with a scale whose inverse is not a normal number) is divided.
 struct CodesI8 {
     static constexpr float kTop = 127.f;
     static __device__ __forceinline__ uint2 encode(const float (&x)[8], float scale, float inv) {
+        const float magic = 12582912.f;             // 1.5 * 2^23: adding it rounds to a whole number in the low byte
         uint32_t q[8];
+        bool exact = scale < FLT_MIN;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = (uint32_t)max(-127, min(127, rint_div(x[i], scale, inv)));
+        for (int i = 0; i < 8; ++i) {
+            const float r = __fmul_rn(x[i], inv), s = __fadd_rn(r, magic);
+            exact |= !(fabsf(__fadd_rn(r, -__fadd_rn(s, -magic))) <= 0.4999f);
+            q[i] = __float_as_uint(s);
+        }
+        if (exact) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] = (uint32_t)max(-127, min(127, __float2int_rn(__fdiv_rn(x[i], scale))));
+        }
         uint2 out;
         out.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
         out.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
@@ -40,12 +49,24 @@ struct CodesI8 {
 };
 struct CodesE4M3 {
     static constexpr float kTop = 448.f;
-    static __device__ __forceinline__ uint2 encode(const float (&x)[8], float scale, float) {
+    static __device__ __forceinline__ uint2 encode(const float (&x)[8], float scale, float inv) {
+        float y[8];
+        bool exact = scale < FLT_MIN;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            y[i] = __fmul_rn(x[i], inv);
+            const uint32_t bits = __float_as_uint(y[i]);
+            // from 2^-6 on codes keep three bits behind the first: the other twenty are next to one half at a border
+            exact |= (bits & 0x000fffffu) - 0x0007fff8u <= 0x10u;
+            exact |= fabsf(y[i]) < 0.015625f && y[i] != 0.f;
+        }
+        if (exact) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = __fdiv_rn(x[i], scale);
+        }
         uint32_t p[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            p[i] = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x[2 * i], scale), __fdiv_rn(x[2 * i + 1], scale)),
-                                            __NV_SATFINITE, __NV_E4M3);
+        for (int i = 0; i < 4; ++i) p[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i], y[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
         return make_uint2(p[0] | (p[1] << 16), p[2] | (p[3] << 16));
     }
     static __device__ __forceinline__ void decode(const uint2& v, float (&f)[8]) {
@@ -71,7 +92,7 @@ struct WriteShape {
 // a row go to neighbouring threads of one warp, so the row's maximum is a few shuffles.  A thread requests its first cells
 // before the block computes the tokens' angles, once for all heads, into shared memory.
 template <typename T, typename Codes, int D>
-__global__ void __launch_bounds__(256, 3) rope_paged_kv_kernel(const T* __restrict__ QKV, const long long* __restrict__ positions,
+__global__ void __launch_bounds__(256, 4) rope_paged_kv_kernel(const T* __restrict__ QKV, const long long* __restrict__ positions,
                                                             const long long* __restrict__ slots,
                                                             const unsigned long long* __restrict__ steps, const KvView kv,
                                                             T* __restrict__ Q, const WriteShape p, int* status) {
@@ -112,7 +133,9 @@ __global__ void __launch_bounds__(256, 3) rope_paged_kv_kernel(const T* __restri
             RawCell<T>::widen(raw[u].w[1], b);
             if (cell.pair >= 0 && head < p.H + kv.heads) turn_cell(a, b, cs + t * pairs, sn + t * pairs, cell.pair, p.layout);
             float amax = 0.f;
-            if constexpr (!std::is_void<Codes>::value) amax = row_amax(a, b, kLanes);
+            if constexpr (!std::is_void<Codes>::value) {
+                if (__any_sync(0xffffffffu, head >= p.H)) amax = row_amax(a, b, kLanes);
+            }
             if (!live) continue;
             if (head < p.H) {
                 T* q = Q + ((size_t)(t0 + t) * p.H + head) * D;

@@ -15,7 +15,7 @@ struct RotaryShape {
 // One block turns `tokens_per_block` tokens.  A row's D / 16 cells go to neighbouring threads; a thread requests its first
 // cells before the block computes the tokens' angles, once for all heads, into shared memory.
 template <typename T>
-__global__ void __launch_bounds__(256) rotary_kernel(const T* X, T* Y, const long long* __restrict__ positions,
+__global__ void __launch_bounds__(256, 4) rotary_kernel(const T* X, T* Y, const long long* __restrict__ positions,
                                                      const unsigned long long* __restrict__ steps, const RotaryShape p) {
     constexpr int kU = kCells<T>;
     __shared__ __align__(16) float cs[kTablePairs], sn[kTablePairs];
