@@ -4,8 +4,10 @@ The reference measures end to end with a HuggingFace Llama/Qwen checkpoint and `
 (utils/perf_eval.py:236-275, kairos/main_ablation.py:108-140).  Checkpoints are not available here,
 so this module builds the same decoder geometry with random weights (N(0, 0.02)), swaps every linear of
 the decoder layers through ``quantize_model`` exactly as the reference does (lm_head stays fp16), and
-runs prefill + greedy decode with a static KV cache.  Everything that is not a linear (RMSNorm, RoPE,
-attention, SiLU) is stock torch, as it is stock HuggingFace code in the reference.  The decode step is
+runs prefill + greedy decode with a static KV cache, or with a paged one (``Decoder.allocate_paged``: prompts of
+different lengths, fp16 / int8 / e4m3 rows, the library's own decode attention).  Without the paged cache everything
+that is not a linear (RMSNorm, RoPE, attention, SiLU) can be stock torch, as it is stock HuggingFace code in the
+reference.  The decode step is
 captured into a CUDA graph, so the per-token host cost is one graph launch.
 """
 from __future__ import annotations
@@ -22,8 +24,10 @@ import torch.nn.functional as F
 
 from . import ops
 from .dynamic_linear import COMP_TYPE_NAME, DynamicLinear
+from .paged_kv import PagedKVCache
 from .perf_profiler import Profiler
 from .quant_model import quantize_model
+from .rotary import Rotary
 
 
 @dataclass
@@ -204,6 +208,7 @@ class Decoder(torch.nn.Module):
             quantize_model(wrap, quant_strategy=quant_strategy, device=self.device)
             self.model.layers.append(layer)
         self.kv = None
+        self.paged = None            # PagedKVCache of allocate_paged()
         self.graph = None
         self._prefill_graphs = {}
         # Row-parallel outputs of up to `peer_allreduce_tokens` tokens are summed by the library's own kernel
@@ -223,15 +228,19 @@ class Decoder(torch.nn.Module):
         return shapes
 
     # ---- state ------------------------------------------------------------------------------
+    def _reserve(self, tokens):
+        from .runtime import default_context
+        ctx = DynamicLinear.context or default_context(self.device)
+        shapes = self.linear_shapes()
+        ctx.reserve(tokens, max(s[0] for s in shapes), max(s[1] for s in shapes))
+
     def allocate(self, batch, max_len, max_tokens=None):
         """Static state for `batch` sequences of up to `max_len` positions.  `max_tokens` (default
         batch * max_len) sizes the library's activation / split-K workspaces once, so that no later call
         reallocates a buffer a captured CUDA graph still points to."""
         cfg = self.cfg
-        from .runtime import default_context
-        ctx = DynamicLinear.context or default_context(self.device)
-        shapes = self.linear_shapes()
-        ctx.reserve(max_tokens or batch * max_len, max(s[0] for s in shapes), max(s[1] for s in shapes))
+        self._reserve(max_tokens or batch * max_len)
+        self.paged = None
         shape = (len(self.model.layers), 2, batch, cfg.n_kv_heads, max_len, cfg.head_dim)
         self.kv = torch.zeros(shape, dtype=torch.float16, device=self.device)
         self.max_len = max_len
@@ -243,6 +252,40 @@ class Decoder(torch.nn.Module):
         self.next_tok = torch.zeros((batch, 1), dtype=torch.long, device=self.device)
         self.graph = None
         self._prefill_graphs = {}
+
+    def allocate_paged(self, batch, max_len, kv_dtype=torch.float16, page_size=64, num_pages=None, max_tokens=None,
+                       rope_scaling=None):
+        """Static state for `batch` sequences of up to `max_len` positions over a paged cache whose rows are fp16, int8 or
+        e4m3 (`kv_dtype`).  `num_pages` (default: enough for every sequence at max_len) may be smaller: pages are handed
+        out as sequences grow.  `rope_scaling`: see :class:`Rotary`."""
+        cfg = self.cfg
+        self._reserve(max_tokens or batch * max_len)
+        width = -(-max_len // page_size)
+        self.kv = None
+        self.paged = PagedKVCache(len(self.model.layers), num_pages or batch * width, cfg.n_kv_heads, cfg.head_dim, page_size,
+                                  kv_dtype, self.device)
+        self.rotary = Rotary(cfg.head_dim, theta=cfg.rope_theta, scaling=rope_scaling, device=self.device)
+        self.max_len, self.batch = max_len, batch
+        self.lengths = [0] * batch                                # host's copy of `lens`
+        # decode-step buffers (static addresses for the CUDA graph)
+        self.tok = torch.zeros((batch, 1), dtype=torch.long, device=self.device)
+        self.next_tok = torch.zeros((batch, 1), dtype=torch.long, device=self.device)
+        self.lens = torch.zeros((batch,), dtype=torch.int32, device=self.device)
+        self.table = torch.full((batch, width), -1, dtype=torch.int32, device=self.device)
+        self.graph = None
+        self._prefill_graphs = {}
+
+    def _grow(self, counts):
+        """Pages for counts[i] more positions of sequence i; the table on the device follows where one got a new page."""
+        new = False
+        for i, n in enumerate(counts):
+            if self.lengths[i] + n > self.max_len:
+                raise ValueError(f'sequence {i}: {self.lengths[i]} + {n} positions exceed the {self.max_len} of allocate_paged')
+        for i, n in enumerate(counts):
+            held = -(-self.lengths[i] // self.paged.page_size)
+            new |= len(self.paged.reserve(i, self.lengths[i] + n)) > held
+        if new:
+            self.table.copy_(self.paged.page_table(range(self.batch), width=self.table.shape[1]))
 
     def release_graphs(self):
         """Drop the captured CUDA graphs.  With tensor parallelism they hold the captured collectives, and a
@@ -305,22 +348,14 @@ class Decoder(torch.nn.Module):
             return lin.forward_q8(xq, sx)
         return lin(self._norm(mod, x, delta))
 
-    def _layer(self, li, layer, x, delta, pos0, decode):
-        """One decoder layer on the residual stream x (updated in place).  `delta` is the output of the
-        previous layer's MLP, not yet added; returns this layer's MLP output in the same way, so that each
-        residual addition is carried by the norm that follows it."""
+    def _static_layer(self, li, qkv, pos0, decode):
+        """Rotary positions, cache write and attention of one layer over the contiguous cache."""
         cfg = self.cfg
-        b, s, _ = x.shape
+        b, s, _ = qkv.shape
         nh, nkv, d = cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
-        a = layer.self_attn
-        if self.fuse:
-            qkv = self._norm_then_linear(layer.input_layernorm, x, delta, a.qkv_proj)   # [B, S, (H + 2 Hkv) D]
-        else:
-            h = self._norm(layer.input_layernorm, x, delta)
-            qkv = torch.cat((a.q_proj(h), a.k_proj(h), a.v_proj(h)), dim=-1)
         kc, vc = self.kv[li, 0], self.kv[li, 1]
         if self.glue == 'cuda':
-            q = torch.empty((b, nh, s, d), dtype=torch.float16, device=x.device)
+            q = torch.empty((b, nh, s, d), dtype=torch.float16, device=qkv.device)
             ops.rope_kv(qkv, self.cos, self.sin, q, kc, vc, b, s, nh, nkv, d,
                         pos_dev=self.pos if decode else None, pos0=pos0)
         else:
@@ -344,7 +379,45 @@ class Decoder(torch.nn.Module):
         else:
             o = F.scaled_dot_product_attention(q, kc[:, :, pos0:pos0 + s], vc[:, :, pos0:pos0 + s], is_causal=True,
                                                enable_gqa=True)
-        o = o.transpose(1, 2).reshape(b, s, nh * d)
+        return o.transpose(1, 2).reshape(b, s, nh * d)
+
+    def _paged_layer(self, li, qkv, decode):
+        """The same over the paged cache: qkv [tokens, (H + 2 Hkv) D] of all sequences, one after the other.  A prefill
+        attends over what the cache holds (the values its rows stand for), so it may continue an earlier one."""
+        q = ops.rope_paged_kv(qkv, self.positions, self.slots, self.rotary, self.paged, layer=li)
+        if decode:
+            return ops.paged_attention(q, self.paged, self.table, self.lens, layer=li)
+        k, v = ops.paged_kv_read(self.paged, self.seen_slots, layer=li, dtype=q.dtype)
+        if len(set((n, total) for n, total, _ in self.chunks)) == 1:          # one shape for the whole batch: one call
+            n, total, mask = self.chunks[0]
+            qi, ki, vi = (t.view(len(self.chunks), -1, *t.shape[1:]).transpose(1, 2) for t in (q, k, v))
+            oi = F.scaled_dot_product_attention(qi, ki, vi, attn_mask=mask, is_causal=mask is None, enable_gqa=True)
+            return oi.transpose(1, 2).reshape(q.shape)
+        out, first, seen = torch.empty_like(q), 0, 0
+        for n, total, mask in self.chunks:
+            qi, ki, vi = (t.transpose(0, 1)[None] for t in (q[first:first + n], k[seen:seen + total], v[seen:seen + total]))
+            oi = F.scaled_dot_product_attention(qi, ki, vi, attn_mask=mask, is_causal=mask is None, enable_gqa=True)
+            out[first:first + n] = oi[0].transpose(0, 1)
+            first, seen = first + n, seen + total
+        return out
+
+    def _layer(self, li, layer, x, delta, pos0, decode):
+        """One decoder layer on the residual stream x (updated in place).  `delta` is the output of the
+        previous layer's MLP, not yet added; returns this layer's MLP output in the same way, so that each
+        residual addition is carried by the norm that follows it."""
+        cfg = self.cfg
+        b, s, _ = x.shape
+        nh, nkv, d = cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
+        a = layer.self_attn
+        if self.fuse:
+            qkv = self._norm_then_linear(layer.input_layernorm, x, delta, a.qkv_proj)   # [B, S, (H + 2 Hkv) D]
+        else:
+            h = self._norm(layer.input_layernorm, x, delta)
+            qkv = torch.cat((a.q_proj(h), a.k_proj(h), a.v_proj(h)), dim=-1)
+        if self.paged is not None:
+            o = self._paged_layer(li, qkv.view(b * s, -1), decode).view(b, s, nh * d)
+        else:
+            o = self._static_layer(li, qkv, pos0, decode)
         attn_out = self._row_parallel(a.o_proj, o)
         m = layer.mlp
         if not self.fuse:
@@ -396,14 +469,49 @@ class Decoder(torch.nn.Module):
         self.pos.fill_(s)
         return logits
 
+    def _prefill_paged(self, prompts, keep):
+        """Logits of the last token of every prompt ([B, S] or a list of B token vectors, none of them empty).  keep: the
+        sequences go on from what the cache holds of them; else they start anew."""
+        prompts = list(prompts)
+        counts = [len(p) for p in prompts]
+        if len(prompts) != self.batch or min(counts) < 1:
+            raise ValueError(f'expected {self.batch} prompts of at least one token, got lengths {counts}')
+        keys = range(self.batch)
+        if not keep:
+            for i in keys:
+                if self.lengths[i]:
+                    self.paged.release(i)
+            self.lengths = [0] * self.batch
+        self._grow(counts)
+        starts, totals = self.lengths, [a + n for a, n in zip(self.lengths, counts)]
+        self.slots, self.positions = self.paged.slots(keys, counts, starts)
+        self.seen_slots = self.slots if not any(starts) else self.paged.slots(keys, totals)[0]
+        masks = [None if a == 0 else torch.arange(a + n, device=self.device) <= torch.arange(a, a + n, device=self.device)[:, None]
+                 for a, n in zip(starts, counts)]
+        self.chunks = list(zip(counts, totals, masks))
+        x, delta = self._stack(self.embed[torch.cat(prompts)][None], False)
+        delta = self._as_tensor(delta)
+        last = torch.tensor(counts, device=self.device).cumsum(0) - 1
+        h = self._norm(self.norm, x[:, last].contiguous(), None if delta is None else delta[:, last].contiguous())
+        self.lengths = totals
+        self.lens.copy_(torch.tensor(totals, dtype=torch.int32))
+        return h.reshape(self.batch, -1) @ self.lm_head.t()
+
     @torch.no_grad()
-    def prefill(self, tokens, return_logits=False, use_graph=False):
+    def prefill(self, tokens, return_logits=False, use_graph=False, keep=False):
         """tokens [B, S] -> next token ids [B, 1]; fills the KV cache for positions 0..S-1.
+
+        With a paged cache the prompts may differ in length (a list of token vectors) and, with `keep`, continue what the
+        sequences already hold (a prompt in chunks, another turn of a conversation); such a prefill runs eagerly.
 
         use_graph: replay a CUDA graph captured for this (B, S) (the ~500 launches of a prefill are then off
         the host's critical path); the prompt is copied into the graph's static token buffer.  The graph is
         captured after two eager passes, so every converted weight it needs is in the conversion cache."""
-        if not use_graph:
+        if self.paged is not None:
+            logits = self._prefill_paged(tokens, keep)
+        elif keep:
+            raise ValueError('prefill(keep=True) continues sequences of a paged cache (allocate_paged)')
+        elif not use_graph:
             logits = self._prefill_body(tokens)
         else:
             key = tuple(tokens.shape)
@@ -429,6 +537,38 @@ class Decoder(torch.nn.Module):
             return logits
         return first_argmax(logits)
 
+    def _paged_decode_body(self):
+        # the new token's position is the sequence's length so far; its slot follows from the page table
+        self.positions = self.lens.long()
+        page = self.table.gather(1, (self.positions // self.paged.page_size)[:, None])[:, 0].long()
+        self.slots = page * self.paged.page_size + self.positions % self.paged.page_size
+        self.lens.add_(1)
+        x, delta = self._stack(self.embed[self.tok], True)
+        self.logits = self._norm(self.norm, x, delta).reshape(x.shape[0], -1) @ self.lm_head.t()
+        self.next_tok.copy_(first_argmax(self.logits))
+
+    def _paged_decode_step(self, use_graph):
+        self._grow([1] * self.batch)
+        if use_graph and self.graph is None:
+            before = self.lens.clone()
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                for _ in range(2):
+                    self._paged_decode_body()
+                    self.lens.copy_(before)
+            torch.cuda.synchronize()
+            self.graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(self.graph, stream=side):
+                self._paged_decode_body()
+            self.lens.copy_(before)
+            torch.cuda.synchronize()
+        if use_graph:
+            self.graph.replay()
+        else:
+            self._paged_decode_body()
+        self.lengths = [n + 1 for n in self.lengths]
+
     def _decode_body(self):
         self.mask.index_fill_(3, self.pos, 0.0)
         x, delta = self._stack(self.embed[self.tok], True)
@@ -438,7 +578,10 @@ class Decoder(torch.nn.Module):
 
     @torch.no_grad()
     def decode_step(self, use_graph=True):
-        """One token for every sequence: reads self.tok, writes self.next_tok, advances self.pos."""
+        """One token for every sequence: reads self.tok, writes self.next_tok, advances self.pos (paged: self.lens)."""
+        if self.paged is not None:
+            self._paged_decode_step(use_graph)
+            return
         if not use_graph:
             self._decode_body()
             return
@@ -473,14 +616,18 @@ class Decoder(torch.nn.Module):
 
 
 @torch.no_grad()
-def measure_ttft_tpot(model, batch, prompt_len=1024, new_tokens=512, warmup=2, ttft_times=5, seed=0):
+def measure_ttft_tpot(model, batch, prompt_len=1024, new_tokens=512, warmup=2, ttft_times=5, seed=0, kv_dtype=None):
     """TTFT = mean wall time of prefill + first token over `ttft_times` runs; TPOT = (time of a full
     generation - TTFT) / (new_tokens - 1); throughput = batch * new_tokens / (TTFT + (new_tokens-1) * TPOT)
-    (utils/perf_eval.py:236-275 and kairos/main_ablation.py:111-125 of the reference)."""
+    (utils/perf_eval.py:236-275 and kairos/main_ablation.py:111-125 of the reference).  kv_dtype: over a paged cache of
+    that type instead of the contiguous one."""
     dev = model.device
     gen = torch.Generator(device=dev).manual_seed(seed)
     tokens = torch.randint(0, model.cfg.vocab, (batch, prompt_len), generator=gen, device=dev)
-    model.allocate(batch, prompt_len + new_tokens + 8)
+    if kv_dtype is None:
+        model.allocate(batch, prompt_len + new_tokens + 8)
+    else:
+        model.allocate_paged(batch, prompt_len + new_tokens + 8, kv_dtype)
     for _ in range(warmup):
         model.generate(tokens, 4)
     torch.cuda.synchronize()
