@@ -38,7 +38,8 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 struct AttnShape {
     long long qb, qh, table_stride;
     int B, H, group, blocks_per_kv;         // head blocks (of 8 or 16 query heads) per kv head
-    int table_width, workers, joins;        // joins == 0: no pair is ever cut
+    int table_width, workers;
+    int cluster;                            // blocks of a cluster that share one pair; 0: the even cut over all workers
     float scale_log2;
 };
 
@@ -95,7 +96,7 @@ __device__ __forceinline__ bool locate(const int* lens, const AttnShape& p, int 
     }
     total *= pairs;
     const unsigned run = (total + p.workers - 1) / p.workers;
-    const bool whole = !p.joins || (top <= run + kSpare && (long long)p.B * pairs <= p.workers);
+    const bool whole = top <= run + kSpare && (long long)p.B * pairs <= p.workers;
     if (whole) {
         const int b = blockIdx.x / pairs;
         if (b >= p.B) return false;
@@ -171,6 +172,24 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// A thread-block cluster: barrier halves, and the shared memory of block `rank` at the address that `a` has in this one.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t cluster_map(uint32_t a, int rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t a) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    return v;
 }
 // Transposes an 8 x 8 matrix of 16-bit values held as ldmatrix delivers it.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -264,15 +283,29 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float jm[kWarps][kHeads], jl[kWarps][kHeads];
     __shared__ uint32_t jslot[kWarps];
+    __shared__ float2 jpart[kHeads];
     chain_wait();
     chain_release();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int pairs = kv.heads * p.blocks_per_kv, most = p.table_width << kv.page_shift;
     Cut cut = {};
-    const bool some = locate<kTile>(lens, p, pairs, most, &cut);
-    // Units still to take: a run of the even cut, or (run == 0) one whole pair.
-    unsigned left = !some ? 0u : cut.run ? min(cut.run, cut.total - blockIdx.x * cut.run) : units_of<kTile>(cut.len);
-    Segment seg = {cut.b, cut.pair, cut.unit, 0, 0, cut.len};
+    unsigned left = 0;                          // units still to take: a run of the even cut, or (run == 0) one whole pair
+    Segment seg = {};
+    bool more = false;
+    if (p.cluster) {                            // a pair per cluster, its tiles shared evenly by the cluster's blocks
+        const int place = blockIdx.x / p.cluster, rank = blockIdx.x - place * p.cluster;
+        seg.b = place / pairs;
+        seg.pair = place - seg.b * pairs;
+        seg.len = seq_len(lens, seg.b, most);
+        seg.tiles = (seg.len + kTile - 1) / kTile;
+        const int share = (seg.tiles + p.cluster - 1) / p.cluster;
+        seg.tile = rank * share;
+        seg.take = max(0, min(share, seg.tiles - seg.tile));
+        more = seg.len > 0;                     // the same for the whole cluster; a block without tiles joins with nothing
+    } else if (locate<kTile>(lens, p, pairs, most, &cut)) {
+        left = cut.run ? min(cut.run, cut.total - blockIdx.x * cut.run) : units_of<kTile>(cut.len);
+        seg = {cut.b, cut.pair, cut.unit, 0, 0, cut.len};
+    }
     bool first_segment = true;
     // Takes what this worker's run holds of the pair at seg.tile; false where that is only the unit behind its last tile.
     auto take = [&]() {
@@ -295,13 +328,13 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
         } while (!take());
         return true;
     };
-    bool more = left > 0 && (take() || next());
+    if (left > 0) more = take() || next();
     const unsigned run_end = min((blockIdx.x + 1) * cut.run, cut.total);
     auto record = [&](const Crossing& c) {
         *reinterpret_cast<uint4*>(Partials<kHeads, D>::crossing(ws, p.workers, blockIdx.x)) =
             make_uint4((unsigned)c.b, (unsigned)c.pair, c.slot, c.last);
     };
-    if (p.joins && threadIdx.x == 0) record({0, 0, 0, blockIdx.x});
+    if (!p.cluster && threadIdx.x == 0) record({0, 0, 0, blockIdx.x});
 
     uint8_t* ring = smem + warp * (R::kStages * R::kStage);
     const uint32_t ring_u = smem_u32(ring);
@@ -650,9 +683,10 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
         // ---- the next segment's first stages are requested before this one's parts are joined ----------------
         const Segment done = seg;
         const bool first = first_segment;
-        const uint32_t free_slot = slot == 0 ? R::kStages - 1 : slot - 1;      // the one slot that start() leaves alone
         __syncwarp();                           // every lane has read the last stage
         more = next();
+        // the one slot that start() leaves alone; any will do where nothing follows
+        const uint32_t free_slot = more && slot != 0 ? slot - 1 : R::kStages - 1;
         if (more) start(seg);
 
         // ---- the four warps' parts become one: each leaves its rows in a slot of its ring.  Column c of row r lies at
@@ -687,7 +721,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
         const int q0 = dhead * p.group + dblock * kHeads, rows = min(kHeads, p.group - dblock * kHeads);
         const bool whole = done.take == done.tiles;
         const unsigned part = 2 * blockIdx.x + (first ? 0 : 1);
-        if (!whole && done.tile == 0 && threadIdx.x == 0)      // begins here and lies across the run's end
+        if (!p.cluster && !whole && done.tile == 0 && threadIdx.x == 0)      // begins here and lies across the run's end
             record({done.b, done.pair, part, (run_end - done.take + done.tiles - 1) / cut.run});
         for (int i = threadIdx.x; i < rows * (D / 4); i += 128) {
             const int row = i / (D / 4), c = 4 * (i - row * (D / 4));
@@ -707,7 +741,10 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
                 acc.z = __fmaf_rn(f, v.z, acc.z);
                 acc.w = __fmaf_rn(f, v.w, acc.w);
             }
-            if (whole) {
+            if (p.cluster > 1) {                // warp 0's first slot: nothing follows in its ring
+                *reinterpret_cast<float4*>(smem + (row * D + c) * 4) = acc;
+                if (c == 0) jpart[row] = make_float2(top, sum);
+            } else if (whole) {
                 const float inv = __fdiv_rn(1.f, sum);
                 const size_t to = (size_t)done.b * p.H + q0 + row;
                 put4(O + to * D + c, acc, inv);
@@ -716,6 +753,37 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
                 *reinterpret_cast<float4*>(Partials<kHeads, D>::o(ws, part) + row * D + c) = acc;
                 if (c == 0) *reinterpret_cast<float2*>(Partials<kHeads, D>::ml(ws, part) + 2 * row) = make_float2(top, sum);
             }
+        }
+        if (p.cluster > 1) {
+            // ---- the cluster's parts become one, read from its blocks' shared memory; each block forms its share of the
+            // output, and none leaves before all have read
+            __syncwarp();
+            cluster_arrive();
+            cluster_wait();
+            for (int i = threadIdx.x + 128 * (blockIdx.x % p.cluster); i < rows * (D / 4); i += 128 * p.cluster) {
+                const int row = i / (D / 4), c = 4 * (i - row * (D / 4));
+                float top = -INFINITY, sum = 0.f;
+                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                const uint32_t from_o = smem_u32(smem) + (row * D + c) * 4, from_ml = smem_u32(&jpart[row]);
+                for (int k = 0; k < p.cluster; ++k) top = fmaxf(top, ld_cluster2(cluster_map(from_ml, k)).x);
+                const float safe = top == -INFINITY ? 0.f : top;
+                for (int k = 0; k < p.cluster; ++k) {
+                    const float2 ml = ld_cluster2(cluster_map(from_ml, k));
+                    const float4 v = ld_cluster4(cluster_map(from_o, k));
+                    const float f = exp2_fast(ml.x - safe);
+                    sum = __fmaf_rn(f, ml.y, sum);
+                    acc.x = __fmaf_rn(f, v.x, acc.x);
+                    acc.y = __fmaf_rn(f, v.y, acc.y);
+                    acc.z = __fmaf_rn(f, v.z, acc.z);
+                    acc.w = __fmaf_rn(f, v.w, acc.w);
+                }
+                const size_t to = (size_t)done.b * p.H + q0 + row;
+                put4(O + to * D + c, acc, __fdiv_rn(1.f, sum));
+                if (LSE && c == 0) LSE[to] = (top + __log2f(sum) - kLift) * kLn2;
+            }
+            __syncwarp();
+            cluster_arrive();
+            cluster_wait();
         }
         if (more) __syncthreads();              // the slots belong to the rings again
     }
@@ -794,8 +862,7 @@ static int sm_count() {
 }
 
 struct Plan {
-    int heads_per_block, blocks_per_kv, workers;
-    bool joins;
+    int heads_per_block, blocks_per_kv, workers, cluster;
     size_t bytes;
 };
 
@@ -815,15 +882,22 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
     else if (kv.dim == 128) KAIROS_RING(128);
     else KAIROS_RING(256);
 #undef KAIROS_RING
-    const long long per_pair = (((long long)table_width << kv.page_shift) + tile - 1) / tile + 1;      // units
+    const long long tiles = (((long long)table_width << kv.page_shift) + tile - 1) / tile;
     const long long pairs = (long long)B * kv.heads * out->blocks_per_kv;
-    if (per_pair * pairs > 0x7fffffffLL) return KAIROS_ERR_SHAPE;
+    if ((tiles + 1) * pairs > 0x7fffffffLL) return KAIROS_ERR_SHAPE;
     const int full = sms * per_sm;
-    // No pair is cut where there are workers for all of them and none can be longer than a join is worth; otherwise the
-    // device decides by the lengths.
-    out->joins = !(pairs <= full && per_pair <= (long long)kSpare + 2);
-    out->workers = (int)max(1LL, out->joins ? min((long long)full, per_pair * pairs) : pairs);
-    out->bytes = out->joins ? (size_t)2 * out->workers * out->heads_per_block * (kv.dim + 2) * 4 + (size_t)out->workers * sizeof(Crossing) : 0;
+    // Where the table bounds every pair to a few tiles a block, clusters of one to eight blocks take one pair each and
+    // meet in shared memory: one launch, no scan of the lengths, no workspace.  Otherwise the device cuts the work by the
+    // lengths, which costs some 8 us more but keeps every block busy whatever they are.  Two tiles a block at the least: 256
+    // positions take 5.1 us in one block, 512 take 7.0 in one and 5.9 in a cluster of four.  Sixteen at the most (twelve
+    // where pairs are few): in fp16, 32 sequences of 1024 positions take 24.0 us in blocks of their own and 27.9 cut (18.1
+    // and 22.7 with lengths from 32 to 1024), 16 of 2048 in clusters of two 25.0 and 29.9 (19.5 and 20.4), 16 of 4096
+    // 44.0 and 49.4 (33.0 and 31.4), one of 8192 in clusters of eight 15.9 and 14.0.
+    int cluster = 1;
+    while (cluster < 8 && pairs * cluster * 2 <= full && tiles > 4 && tiles >= 4 * cluster) cluster *= 2;
+    out->cluster = pairs * cluster <= full && (tiles + cluster - 1) / cluster <= (pairs < 32 ? 12 : 16) ? cluster : 0;
+    out->workers = (int)(out->cluster ? pairs * out->cluster : max(1LL, min((long long)full, (tiles + 1) * pairs)));
+    out->bytes = out->cluster ? 0 : (size_t)2 * out->workers * out->heads_per_block * (kv.dim + 2) * 4 + (size_t)out->workers * sizeof(Crossing);
     return KAIROS_OK;
 }
 
@@ -835,11 +909,29 @@ static int run_attention(const void* Q, const KvView& kv, const void* table, con
     auto kernel = paged_attention_kernel<QT, Widen, D, kHalves>;
     const int rc = ensure_dynamic_smem(flag, kernel, R::kBytes);
     if (rc != KAIROS_OK) return rc;
-    cudaError_t e = launch_chained(kernel, dim3(plan.workers), dim3(128), R::kBytes, st, static_cast<const QT*>(Q), kv,
-                                   static_cast<const int*>(table), static_cast<const int*>(lens), static_cast<QT*>(O),
-                                   static_cast<float*>(LSE), static_cast<float*>(ws), p, status);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(plan.workers);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = R::kBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    if (plan.cluster > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = plan.cluster;
+        attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    if (chained_launch_enabled()) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++cfg.numAttrs;
+    }
+    cfg.attrs = attr;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const QT*>(Q), kv, static_cast<const int*>(table),
+                                       static_cast<const int*>(lens), static_cast<QT*>(O), static_cast<float*>(LSE),
+                                       static_cast<float*>(ws), p, status);
     if (e != cudaSuccess) return note_cuda_error(e);
-    if (plan.joins && plan.workers > 1) {
+    if (!plan.cluster && plan.workers > 1) {
         constexpr int kSlices = D / 4 / (32 / (8 * kHalves));
         e = launch_chained(paged_attention_join_kernel<QT, D, 8 * kHalves>, dim3(plan.workers - 1, kSlices), dim3(128), 0, st,
                            static_cast<QT*>(O), static_cast<float*>(LSE), static_cast<float*>(ws), p);
@@ -896,7 +988,7 @@ extern "C" int kairos_paged_attention(const void* Q, long long q_b, long long q_
     int* status = device_status_word();
     if (!status) return KAIROS_ERR_CUDA;
     const AttnShape p = {q_b, q_h, table_stride, B, H, H / kv.heads, plan.blocks_per_kv, table_width,
-                         plan.workers, plan.joins ? 1 : 0, scale * kLog2e};
+                         plan.workers, plan.cluster, scale * kLog2e};
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (dtype == KAIROS_DTYPE_F16) {
         if (layer->dtype == KAIROS_DTYPE_I8) return pick_attention<__half, WidenI8>(Q, kv, page_table, lens, O, LSE, workspace, p, plan, status, st);
