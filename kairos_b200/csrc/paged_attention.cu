@@ -33,6 +33,8 @@ constexpr int kWarps = 4;
 // Weights are kept times 2^kLift and pass the reference by 2^kSlack at the most; with a V scale of up to twice the largest
 // so far they stay below 2^15, and fp16's smallest step is 2^-30 of a weight at the reference.
 constexpr float kLift = 6.f, kSlack = 8.f;
+// Reference (less kLift) of a head before its first score: any score passes it.
+constexpr float kUnset = -1e30f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnShape {
@@ -343,6 +345,11 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
     unsigned bad = 0;                           // per 16 positions of a slot: page outside the pool
     int k0, k1, count, head;                    // this warp's positions: k0 .. k0 + kSub - 1, then kTile further, below k1
     const int* pages;
+    // this lane's first 16 bytes of the segment's head in page 0, of its scales (lanes 0..3: K, 4..7: V); a page further
+    const uint8_t *seg_k, *seg_v;
+    const float* seg_scale = nullptr;
+    const unsigned page_rows = (unsigned)kv.heads << kv.page_shift;
+    const size_t page_bytes = (size_t)page_rows * R::kRowBytes;
     int ahead[kSteps];                          // pages of the next stage to request
     uint32_t qb[D / 16][2 * kHalves];
     float unit[kHalves][2];                     // score = product * unit (* scale of the key), heads 2 t and 2 t + 1 (+ 8)
@@ -368,9 +375,10 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
                     bad |= bit;
                     *status = KAIROS_ERR_ARG;
                 }
-                const size_t row = (((size_t)(unsigned)(ok ? ahead[h] : 0) * kv.heads + head) << kv.page_shift) + (key & page_mask);
-                const uint8_t* ks = static_cast<const uint8_t*>(kv.k) + row * R::kRowBytes + lane * 16;
-                const uint8_t* vs = static_cast<const uint8_t*>(kv.v) + row * R::kRowBytes + lane * 16;
+                const unsigned page = ok ? (unsigned)ahead[h] : 0u, in_page = (unsigned)(key & page_mask);
+                const size_t off = (size_t)page * page_bytes + in_page * R::kRowBytes;
+                const uint8_t* ks = seg_k + off;
+                const uint8_t* vs = seg_v + off;
                 if (ok && real >= 16) {
 #pragma unroll
                     for (int n = 0; n < R::kChunks / 2; ++n) {
@@ -389,7 +397,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
                 if constexpr (kCoded) {         // lanes 0..3: scales of K, 4..7: of V
                     if (lane < 8)
                         cp16(dst + 2 * R::kRows + (lane >> 2) * (R::kSub * 4) + h * 64 + (lane & 3) * 16,
-                             (lane < 4 ? kv.ks : kv.vs) + row + (lane & 3) * 4, ok && real > 0);
+                             seg_scale + ((size_t)page * page_rows + in_page), ok && real > 0);
                 }
             }
         }
@@ -404,6 +412,10 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
         k1 = min((sg.tile + sg.take) * kTile, sg.len);
         count = k0 < k1 ? (k1 - k0 + kTile - 1) / kTile : 0;
         pages = table + (size_t)sg.b * p.table_stride;
+        const unsigned head_row = (unsigned)head << kv.page_shift;
+        seg_k = static_cast<const uint8_t*>(kv.k) + (size_t)head_row * R::kRowBytes + lane * 16;
+        seg_v = static_cast<const uint8_t*>(kv.v) + (size_t)head_row * R::kRowBytes + lane * 16;
+        if constexpr (kCoded) seg_scale = (lane < 4 ? kv.ks : kv.vs) + head_row + (lane & 3) * 4;
         look(0);
         int st = slot;
 #pragma unroll
@@ -485,7 +497,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
 #pragma unroll
         for (int r = 0; r < kHalves; ++r)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) m[r][e] = -INFINITY, base[r][e] = -kLift, l[r][e] = 0.f;
+            for (int e = 0; e < 2; ++e) m[r][e] = -INFINITY, base[r][e] = kUnset, l[r][e] = 0.f;
 
 #pragma unroll 1
         for (int i = 0; i < count; ++i) {
@@ -578,11 +590,9 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
 #pragma unroll
             for (int r = 0; r < kHalves; ++r)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    move |= m[r][e & 1] == -INFINITY;
+                for (int e = 0; e < 4; ++e)
 #pragma unroll
                     for (int h = 0; h < kSteps; ++h) move |= x[h][r][e] > kLift + kSlack;
-                }
             if (__any_sync(0xffffffffu, move)) {
                 float grow = 1.f;
                 if constexpr (kCoded) {
@@ -603,14 +613,17 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
                     for (int e = 0; e < 2; ++e) {
                         float top = -INFINITY;
 #pragma unroll
-                        for (int h = 0; h < kSteps; ++h) top = fmaxf(top, fmaxf(x[h][r][e], x[h][r][e + 2]));
+                        for (int h = 0; h < kSteps; ++h)
+#pragma unroll
+                            for (int k = 0; k < 4; k += 2)
+                                if (!((dead >> (2 * h + (k >> 1))) & 1u)) top = fmaxf(top, s[h][r][e + k] * unit[r][e]);
 #pragma unroll
                         for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-                        top = fmaxf(m[r][e], top + base[r][e]);
+                        top = fmaxf(m[r][e], top);
                         const float safe = top == -INFINITY ? 0.f : top;
                         const float keep = exp2_fast(m[r][e] - safe);
                         m[r][e] = top;
-                        base[r][e] = safe - kLift;
+                        base[r][e] = top == -INFINITY ? kUnset : top - kLift;
                         l[r][e] *= keep;
 #pragma unroll
                         for (int j = 0; j < D / 16; ++j) o[j][r][e] *= keep * grow, o[j][r][e + 2] *= keep * grow;
