@@ -17,22 +17,23 @@ __device__ __forceinline__ float row_amax(const float (&a)[8], const float (&b)[
     return __uint_as_float(m < 0x7f800000u ? m : 0x7fffffffu);
 }
 
-// Codes of eight values: the nearest of x / scale, as IEEE division rounds it.  x * inv is within 3 * 2^-24 of the quotient,
-// relative to it, so both round alike unless the product lies next to a border between two codes; a chunk with such a
-// value (or with a scale whose inverse is not a normal number) is divided.
+// Codes of eight values: the nearest of x / scale, as IEEE division rounds it.  With inv the rounded 1 / scale, x times
+// inv (1 - 2^-22) and x times inv (1 + 2^-22) enclose the quotient, whatever their own roundings (3 * 2^-24 in all), so where
+// both become the same code it is the quotient's.  A chunk with a value next to a border between two codes, or with a
+// scale whose inverse is not a normal number, is divided.
+constexpr float kBelow = 1.f - 2.384185791015625e-07f, kAbove = 1.f + 2.384185791015625e-07f;
 struct CodesI8 {
     static constexpr float kTop = 127.f;
     static __device__ __forceinline__ uint2 encode(const float (&x)[8], float scale, float inv) {
         const float magic = 12582912.f;             // 1.5 * 2^23: adding it rounds to a whole number in the low byte
-        uint32_t q[8];
-        bool exact = scale < FLT_MIN;
+        const float below = inv * kBelow, above = inv * kAbove;
+        uint32_t q[8], differ = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float r = __fmul_rn(x[i], inv), s = __fadd_rn(r, magic);
-            exact |= !(fabsf(__fadd_rn(r, -__fadd_rn(s, -magic))) <= 0.4999f);
-            q[i] = __float_as_uint(s);
+            q[i] = __float_as_uint(__fmaf_rn(x[i], below, magic));
+            differ |= q[i] ^ __float_as_uint(__fmaf_rn(x[i], above, magic));
         }
-        if (exact) {
+        if (differ || scale < FLT_MIN) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) q[i] = (uint32_t)max(-127, min(127, __float2int_rn(__fdiv_rn(x[i], scale))));
         }
@@ -50,23 +51,18 @@ struct CodesI8 {
 struct CodesE4M3 {
     static constexpr float kTop = 448.f;
     static __device__ __forceinline__ uint2 encode(const float (&x)[8], float scale, float inv) {
-        float y[8];
-        bool exact = scale < FLT_MIN;
+        const float below = inv * kBelow, above = inv * kAbove;
+        uint32_t p[4], differ = 0;
+        auto code2 = [](float a, float b) { return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3); };
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            y[i] = __fmul_rn(x[i], inv);
-            const uint32_t bits = __float_as_uint(y[i]);
-            // from 2^-6 on codes keep three bits behind the first: the other twenty are next to one half at a border
-            exact |= (bits & 0x000fffffu) - 0x0007fff8u <= 0x10u;
-            exact |= fabsf(y[i]) < 0.015625f && y[i] != 0.f;
+        for (int i = 0; i < 4; ++i) {
+            p[i] = code2(x[2 * i] * below, x[2 * i + 1] * below);
+            differ |= p[i] ^ code2(x[2 * i] * above, x[2 * i + 1] * above);
         }
-        if (exact) {
+        if (differ || scale < FLT_MIN) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = __fdiv_rn(x[i], scale);
+            for (int i = 0; i < 4; ++i) p[i] = code2(__fdiv_rn(x[2 * i], scale), __fdiv_rn(x[2 * i + 1], scale));
         }
-        uint32_t p[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i], y[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
         return make_uint2(p[0] | (p[1] << 16), p[2] | (p[3] << 16));
     }
     static __device__ __forceinline__ void decode(const uint2& v, float (&f)[8]) {
@@ -84,7 +80,7 @@ struct CodesE4M3 {
 struct WriteShape {
     long long row_stride;
     int T, H, rot, layout, tokens_per_block;
-    unsigned by_heads, by_pairs;                // div_magic of H + 2 kv heads and rot / 2
+    unsigned by_q, by_kv, by_pairs;             // div_magic of H, 2 kv heads and rot / 2
     float magnitude;
 };
 
@@ -102,7 +98,14 @@ __global__ void __launch_bounds__(256, 4) rope_paged_kv_kernel(const T* __restri
     chain_wait();
     const int t0 = blockIdx.x * p.tokens_per_block;
     const int here = min(p.tokens_per_block, p.T - t0);
-    const int pairs = p.rot >> 1, heads = p.H + 2 * kv.heads, rows = here * heads;
+    // rows of the block: the q heads of its tokens, then their k and v heads, so that most warps have one kind
+    const int pairs = p.rot >> 1, q_rows = here * p.H, rows = q_rows + 2 * here * kv.heads;
+    auto split = [&](int r, int* t, int* head) {
+        const bool q = r < q_rows;
+        const int k = q ? r : r - q_rows, per = q ? p.H : 2 * kv.heads;
+        *t = div_small(k, q ? p.by_q : p.by_kv);
+        *head = k - *t * per + (q ? 0 : p.H);
+    };
     const long long capacity = (long long)kv.pages << kv.page_shift;
     const int at = threadIdx.x / kLanes, j = threadIdx.x % kLanes;
     const Cell cell = cell_of(j, p.rot, p.layout);
@@ -110,8 +113,9 @@ __global__ void __launch_bounds__(256, 4) rope_paged_kv_kernel(const T* __restri
         RawCell<T> raw[kU];
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-            const int r = min(base + u * kStep + at, rows - 1), t = div_small(r, p.by_heads);      // whole warps stay together
-            raw[u].load(QKV + (size_t)(t0 + t) * p.row_stride + (size_t)(r - t * heads) * D, cell);
+            int t, head;
+            split(min(base + u * kStep + at, rows - 1), &t, &head);        // whole warps stay together
+            raw[u].load(QKV + (size_t)(t0 + t) * p.row_stride + head * D, cell);
         }
         if (base == 0) {
             for (int i = threadIdx.x; i < here * pairs; i += 256) {
@@ -127,7 +131,8 @@ __global__ void __launch_bounds__(256, 4) rope_paged_kv_kernel(const T* __restri
         for (int u = 0; u < kU; ++u) {
             const int r = base + u * kStep + at;
             const bool live = r < rows;
-            const int t = div_small(min(r, rows - 1), p.by_heads), head = min(r, rows - 1) - t * heads;
+            int t, head;
+            split(min(r, rows - 1), &t, &head);
             float a[8], b[8];
             RawCell<T>::widen(raw[u].w[0], a);
             RawCell<T>::widen(raw[u].w[1], b);
@@ -236,7 +241,8 @@ template <typename T, typename Codes, int D>
 static int run_write(const void* QKV, const void* positions, const void* slots, const void* steps, const KvView& kv, void* Q,
                      WriteShape p, int* status, cudaStream_t st) {
     p.tokens_per_block = rows_tokens(p.T, p.H + 2 * kv.heads, p.rot);
-    p.by_heads = div_magic(p.H + 2 * kv.heads);
+    p.by_q = div_magic(p.H);
+    p.by_kv = div_magic(2 * kv.heads);
     p.by_pairs = div_magic(max(1, p.rot / 2));
     const cudaError_t e = launch_chained(
         rope_paged_kv_kernel<T, Codes, D>, dim3((unsigned)((p.T + p.tokens_per_block - 1) / p.tokens_per_block)), dim3(256), 0,
