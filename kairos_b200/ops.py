@@ -324,20 +324,19 @@ def rotary(x, positions, rotary, transpose=False, out=None):
         raise _bad(out, 'out', f'{x.dtype} {tuple(shape)} with a dense last dimension', index)
     to, at = out.stride(), positions
     if dims == 3:
-        b, (s, h, d) = 1, shape
+        b, xb, yb, pb, (s, h, d) = 1, 0, 0, 0, shape
         if at.shape != (s,):
             at = at.expand(s)
-        xs, ys, ps = (0, strides[0], strides[1]), (0, to[0], to[1]), (0, at.stride(0))
     else:
         b, s, h, d = shape
         if at.shape != (b, s):
             at = at.expand(b, s)
-        xs, ys, ps = strides[:3], to[:3], at.stride()
-    if b == 1 or s == 1 or h == 1:             # the stride of a dimension of one element may be anything: none
-        one = (b == 1, s == 1, h == 1)
-        xs, ys = ([0 if o else v for o, v in zip(one, t)] for t in (xs, ys))
-    rc = _call(index, lib.kairos_rotary, x.data_ptr(), *xs, out.data_ptr(), *ys, at.data_ptr(), *ps, rotary.plan_ptr, code,
-               1 if transpose else 0, b, s, h, d)
+        xb, yb, pb = (strides[0], to[0], at.stride(0)) if b > 1 else (0, 0, 0)
+    # the stride of a dimension of one element may be anything: none
+    xs, ys, ps = (strides[-3], to[-3], at.stride(-1)) if s > 1 else (0, 0, 0)
+    xh, yh = (strides[-2], to[-2]) if h > 1 else (0, 0)
+    rc = _call(index, lib.kairos_rotary, x.data_ptr(), xb, xs, xh, out.data_ptr(), yb, ys, yh, at.data_ptr(), pb, ps,
+               rotary.plan_ptr, code, 1 if transpose else 0, b, s, h, d)
     if rc < 0:
         check(rc, 'rotary')
     return out

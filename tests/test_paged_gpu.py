@@ -387,6 +387,29 @@ def test_attention_long_and_many(dtype, kv, lens, h, hkv, d):
 
 
 @pytest.mark.parametrize('dtype,kv', TYPES)
+@pytest.mark.parametrize('d', [64, 128, 256])
+@pytest.mark.parametrize('lens', [[1], [64], [65, 0, 3], [600], [129, 1025], [1023, 0, 511, 513, 1, 900], [4000, 17], [257] * 40,
+                                  [2500, 1, 0, 64, 640] * 5])
+@pytest.mark.parametrize('h,hkv', [(5, 1), (24, 2)])
+def test_attention_whatever_shares_the_work(dtype, kv, d, lens, h, hkv):
+    """The table's width decides whether blocks, clusters of 2, 4 or 8 blocks, or a cut by the lengths on the device share a
+    sequence: the same lengths with tables of growing width, every result against 64 bits."""
+    from kairos_b200 import ops
+    c, q, table, n = attention_case(dtype, kv, lens, h, hkv, d, 16, seed=len(lens) + d)
+    ref = None
+    for width in (table.shape[1], 70, 140, 300, 900, 3000):
+        if width < table.shape[1]:
+            continue
+        wide = torch.full((len(lens), width), -1, dtype=torch.int32, device=DEV)
+        wide[:, :table.shape[1]] = table
+        got, lse = ops.paged_attention(q, c, wide, n, return_lse=True)
+        if ref is None or not torch.equal(got, ref[0]) or not torch.equal(lse, ref[1]):
+            check_attention(c, q, table, lens, got, lse)
+            ref = got, lse
+    assert status() == 0
+
+
+@pytest.mark.parametrize('dtype,kv', TYPES)
 def test_attention_peaked_scores_and_scale(dtype, kv):
     """Scores tens apart, so that running maxima keep changing; a scale of its own, zero and negative ones."""
     from kairos_b200 import ops
