@@ -294,15 +294,23 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
     unsigned left = 0;                          // units still to take: a run of the even cut, or (run == 0) one whole pair
     Segment seg = {};
     bool more = false;
-    if (p.cluster) {                            // a pair per cluster, its tiles shared evenly by the cluster's blocks
+    const int stride = p.cluster ? p.cluster * kTile : kTile;      // from one of this block's tiles to the next
+    int first_pages[R::kStages - 1][kSteps];
+    if (p.cluster) {                            // a pair per cluster, its tiles dealt to the cluster's blocks in turn
         const int place = blockIdx.x / p.cluster, rank = blockIdx.x - place * p.cluster;
         seg.b = place / pairs;
         seg.pair = place - seg.b * pairs;
+        seg.tile = rank;
+        // the first tiles' places do not depend on the length, so their pages are looked up together with it
+#pragma unroll
+        for (int i = 0; i < R::kStages - 1; ++i)
+#pragma unroll
+            for (int h = 0; h < kSteps; ++h) {
+                const int key = rank * kTile + warp * R::kSub + i * stride + 16 * h;
+                first_pages[i][h] = key < most ? __ldcg(table + (size_t)seg.b * p.table_stride + (key >> kv.page_shift)) : 0;
+            }
         seg.len = seq_len(lens, seg.b, most);
-        seg.tiles = (seg.len + kTile - 1) / kTile;
-        const int share = (seg.tiles + p.cluster - 1) / p.cluster;
-        seg.tile = rank * share;
-        seg.take = max(0, min(share, seg.tiles - seg.tile));
+        seg.tiles = seg.take = (seg.len + kTile - 1) / kTile;
         more = seg.len > 0;                     // the same for the whole cluster; a block without tiles joins with nothing
     } else if (locate<kTile>(lens, p, pairs, most, &cut)) {
         left = cut.run ? min(cut.run, cut.total - blockIdx.x * cut.run) : units_of<kTile>(cut.len);
@@ -343,7 +351,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
     const int page_mask = (1 << kv.page_shift) - 1;
     int slot = 0;                               // ring slot of the next stage to read
     unsigned bad = 0;                           // per 16 positions of a slot: page outside the pool
-    int k0, k1, count, head;                    // this warp's positions: k0 .. k0 + kSub - 1, then kTile further, below k1
+    int k0, k1, count, head;                    // this warp's positions: k0 .. k0 + kSub - 1, then `stride` further, below k1
     const int* pages;
     // this lane's first 16 bytes of the segment's head in page 0, of its scales (lanes 0..3: K, 4..7: V); a page further
     const uint8_t *seg_k, *seg_v;
@@ -354,28 +362,28 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
     uint32_t qb[D / 16][2 * kHalves];
     float unit[kHalves][2];                     // score = product * unit (* scale of the key), heads 2 t and 2 t + 1 (+ 8)
 
-    auto look = [&](int i) {
+    auto look = [&](int i, int (&to)[kSteps]) {
 #pragma unroll
         for (int h = 0; h < kSteps; ++h) {
-            const int key = k0 + i * kTile + 16 * h;
-            if (h == 0 || kv.page_shift < 5) ahead[h] = key < k1 ? __ldcg(pages + (key >> kv.page_shift)) : 0;
-            else ahead[h] = ahead[0];
+            const int key = k0 + i * stride + 16 * h;
+            if (h == 0 || kv.page_shift < 5) to[h] = key < k1 ? __ldcg(pages + (key >> kv.page_shift)) : 0;
+            else to[h] = to[0];
         }
     };
-    auto request = [&](int i, int st) {         // stage i of the segment into slot st, from the pages in `ahead`
+    auto request = [&](int i, int st, const int (&from)[kSteps]) {     // stage i of the segment, in pages `from`, into slot st
         if (i < count) {
             const uint32_t dst = ring_u + st * R::kStage;
 #pragma unroll
             for (int h = 0; h < kSteps; ++h) {
-                const int key = k0 + i * kTile + 16 * h, real = k1 - key;
-                const bool ok = (unsigned)ahead[h] < (unsigned)kv.pages;
+                const int key = k0 + i * stride + 16 * h, real = k1 - key;
+                const bool ok = (unsigned)from[h] < (unsigned)kv.pages;
                 const unsigned bit = 1u << (st * kSteps + h);
                 bad &= ~bit;
                 if (!ok && real > 0) {
                     bad |= bit;
                     *status = KAIROS_ERR_ARG;
                 }
-                const unsigned page = ok ? (unsigned)ahead[h] : 0u, in_page = (unsigned)(key & page_mask);
+                const unsigned page = ok ? (unsigned)from[h] : 0u, in_page = (unsigned)(key & page_mask);
                 const size_t off = (size_t)page * page_bytes + in_page * R::kRowBytes;
                 const uint8_t* ks = seg_k + off;
                 const uint8_t* vs = seg_v + off;
@@ -409,19 +417,22 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
         const int block = sg.pair - head * p.blocks_per_kv;
         const int rows = min(kHeads, p.group - block * kHeads);
         k0 = sg.tile * kTile + warp * R::kSub;
-        k1 = min((sg.tile + sg.take) * kTile, sg.len);
-        count = k0 < k1 ? (k1 - k0 + kTile - 1) / kTile : 0;
+        k1 = p.cluster ? sg.len : min((sg.tile + sg.take) * kTile, sg.len);
+        count = k0 < k1 ? (k1 - k0 + stride - 1) / stride : 0;
         pages = table + (size_t)sg.b * p.table_stride;
         const unsigned head_row = (unsigned)head << kv.page_shift;
         seg_k = static_cast<const uint8_t*>(kv.k) + (size_t)head_row * R::kRowBytes + lane * 16;
         seg_v = static_cast<const uint8_t*>(kv.v) + (size_t)head_row * R::kRowBytes + lane * 16;
         if constexpr (kCoded) seg_scale = (lane < 4 ? kv.ks : kv.vs) + head_row + (lane & 3) * 4;
-        look(0);
+        if (!p.cluster) {                       // all look-ups together, then the requests
+#pragma unroll
+            for (int i = 0; i < R::kStages - 1; ++i) look(i, first_pages[i]);
+        }
+        look(R::kStages - 1, ahead);
         int st = slot;
 #pragma unroll
         for (int i = 0; i < R::kStages - 1; ++i) {
-            request(i, st);
-            look(i + 1);
+            request(i, st, first_pages[i]);
             st = st + 1 == R::kStages ? 0 : st + 1;
         }
         // q as the second operand: head g (and g + 8).  For a coded cache the channels of a step are permuted as the code
@@ -503,11 +514,11 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
         for (int i = 0; i < count; ++i) {
             cp_wait<R::kStages - 2>();
             __syncwarp();                       // every lane's copies have landed; the stage before has been read
-            request(i + R::kStages - 1, slot == 0 ? R::kStages - 1 : slot - 1);
-            look(i + R::kStages);
+            request(i + R::kStages - 1, slot == 0 ? R::kStages - 1 : slot - 1, ahead);
+            look(i + R::kStages, ahead);
             const uint32_t ku = ring_u + slot * R::kStage, vu = ku + R::kRows;
             const uint8_t* stage = ring + slot * R::kStage;
-            const int real = k1 - (k0 + i * kTile);
+            const int real = k1 - (k0 + i * stride);
             const unsigned gone = (bad >> (slot * kSteps)) & ((1u << kSteps) - 1);
             const bool full = real >= R::kSub && gone == 0;     // the same in all lanes
             slot = slot + 1 == R::kStages ? 0 : slot + 1;
@@ -887,7 +898,8 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
     out->blocks_per_kv = (group + out->heads_per_block - 1) / out->heads_per_block;
     const bool wide = out->heads_per_block == 16;
     int tile = 0, per_sm = 0;
-#define KAIROS_RING(D)                                                                                (wide ? (tile = coded ? Ring<D, true, 2>::kTile : Ring<D, false, 2>::kTile,                 \
+#define KAIROS_RING(D)                                                                          \
+    (wide ? (tile = coded ? Ring<D, true, 2>::kTile : Ring<D, false, 2>::kTile,                 \
              per_sm = coded ? Ring<D, true, 2>::kBlocksPerSm : Ring<D, false, 2>::kBlocksPerSm) \
           : (tile = coded ? Ring<D, true, 1>::kTile : Ring<D, false, 1>::kTile,                 \
              per_sm = coded ? Ring<D, true, 1>::kBlocksPerSm : Ring<D, false, 1>::kBlocksPerSm))

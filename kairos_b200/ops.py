@@ -402,7 +402,7 @@ def paged_kv_read(cache, slots, layer=0, dtype=torch.float16, out=None):
 def paged_attention(q, cache, page_table, lens, layer=0, scale=None, out=None, return_lse=False):
     """Attention of one new token per sequence: q [B, H, D] (fp16 / bf16, strided batch and heads) over the first
     ``lens[b]`` positions of sequence b, whose pages are row b of ``page_table``.  page_table is int32 [B, W] (entries
-    behind the end are not read), lens int32 [B]; scale defaults to 1 / sqrt(D).  Returns o [B, H, D], with
+    behind the end may hold anything), lens int32 [B]; scale defaults to 1 / sqrt(D).  Returns o [B, H, D], with
     ``return_lse`` also the fp32 [B, H] logarithm of the softmax's denominator.  An empty sequence gives zeros and
     -inf."""
     shape, strides, code, index = q.shape, q.stride(), _HALVES.get(q.dtype), q.get_device()
