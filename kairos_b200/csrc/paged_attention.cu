@@ -424,14 +424,12 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
         seg_k = static_cast<const uint8_t*>(kv.k) + (size_t)head_row * R::kRowBytes + lane * 16;
         seg_v = static_cast<const uint8_t*>(kv.v) + (size_t)head_row * R::kRowBytes + lane * 16;
         if constexpr (kCoded) seg_scale = (lane < 4 ? kv.ks : kv.vs) + head_row + (lane & 3) * 4;
-        if (!p.cluster) {                       // all look-ups together, then the requests
-#pragma unroll
-            for (int i = 0; i < R::kStages - 1; ++i) look(i, first_pages[i]);
-        }
-        look(R::kStages - 1, ahead);
         int st = slot;
+        if (!p.cluster) look(0, first_pages[0]);
 #pragma unroll
         for (int i = 0; i < R::kStages - 1; ++i) {
+            if (i + 1 == R::kStages - 1) look(i + 1, ahead);
+            else if (!p.cluster) look(i + 1, first_pages[i + 1]);
             request(i, st, first_pages[i]);
             st = st + 1 == R::kStages ? 0 : st + 1;
         }
@@ -913,13 +911,14 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
     const int full = sms * per_sm;
     // Where the table bounds every pair to a few tiles a block, clusters of one to eight blocks take one pair each and
     // meet in shared memory: one launch, no scan of the lengths, no workspace.  Otherwise the device cuts the work by the
-    // lengths, which costs some 8 us more but keeps every block busy whatever they are.  Two tiles a block at the least: 256
-    // positions take 5.1 us in one block, 512 take 7.0 in one and 5.9 in a cluster of four.  Sixteen at the most (twelve
+    // lengths, which costs some 8 us more but keeps every block busy whatever they are.  Up to four tiles go to one block, more
+    // are shared by two tiles a block: 256 positions take 5.1 us in one block and in four, 512 take 7.0 in one, 6.6 in two
+    // and 5.9 in four.  Sixteen at the most (twelve
     // where pairs are few): in fp16, 32 sequences of 1024 positions take 24.0 us in blocks of their own and 27.9 cut (18.1
     // and 22.7 with lengths from 32 to 1024), 16 of 2048 in clusters of two 25.0 and 29.9 (19.5 and 20.4), 16 of 4096
     // 44.0 and 49.4 (33.0 and 31.4), one of 8192 in clusters of eight 15.9 and 14.0.
     int cluster = 1;
-    while (cluster < 8 && pairs * cluster * 2 <= full && tiles > 4 && tiles >= 4 * cluster) cluster *= 2;
+    while (cluster < 8 && pairs * cluster * 2 <= full && tiles > 4 && tiles > 2 * cluster) cluster *= 2;
     out->cluster = pairs * cluster <= full && (tiles + cluster - 1) / cluster <= (pairs < 32 ? 12 : 16) ? cluster : 0;
     out->workers = (int)(out->cluster ? pairs * out->cluster : max(1LL, min((long long)full, (tiles + 1) * pairs)));
     out->bytes = out->cluster ? 0 : (size_t)2 * out->workers * out->heads_per_block * (kv.dim + 2) * 4 + (size_t)out->workers * sizeof(Crossing);
