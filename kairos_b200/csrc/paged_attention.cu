@@ -54,10 +54,11 @@ struct Cut {
     int len;                                // of that sequence
 };
 
-// The work of a pair in units: a tile of positions each, and one more for ending it (joining the warps, starting the next
-// pair), which takes about as long; none for an empty sequence.
+// The work of a pair in units: a tile of positions each, and kEnding more for ending it (joining the warps, starting the
+// next pair); none for an empty sequence.
+constexpr int kEnding = 2;                  // 1: 256 sequences of 1 to 500 positions 64.0 us for 56.4, 64 of 1 to 4000 93.9 for 88.0; 3: no gain
 template <int kTile>
-__device__ __forceinline__ unsigned units_of(int len) { return len > 0 ? (unsigned)(len + kTile - 1) / kTile + 1 : 0; }
+__device__ __forceinline__ unsigned units_of(int len) { return len > 0 ? (unsigned)(len + kTile - 1) / kTile + kEnding : 0; }
 
 // Units that a block may take over what an even cut gives it before cutting pays: a join costs about as long as a block
 // needs for so many.
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
     // Takes what this worker's run holds of the pair at seg.tile; false where that is only the unit behind its last tile.
     auto take = [&]() {
         seg.tiles = (seg.len + kTile - 1) / kTile;
-        const int units = min((int)left, seg.tiles + 1 - seg.tile);
+        const int units = min((int)left, seg.tiles + kEnding - seg.tile);
         left -= units;
         seg.take = min(units, seg.tiles - seg.tile);
         return seg.take > 0;
@@ -907,7 +908,7 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
 #undef KAIROS_RING
     const long long tiles = (((long long)table_width << kv.page_shift) + tile - 1) / tile;
     const long long pairs = (long long)B * kv.heads * out->blocks_per_kv;
-    if ((tiles + 1) * pairs > 0x7fffffffLL) return KAIROS_ERR_SHAPE;
+    if ((tiles + kEnding) * pairs > 0x7fffffffLL) return KAIROS_ERR_SHAPE;
     const int full = sms * per_sm;
     // Where the table bounds every pair to a few tiles a block, clusters of one to eight blocks take one pair each and
     // meet in shared memory: one launch, no scan of the lengths, no workspace.  Otherwise the device cuts the work by the
@@ -920,7 +921,12 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
     int cluster = 1;
     while (cluster < 8 && pairs * cluster * 2 <= full && tiles > 4 && tiles > 2 * cluster) cluster *= 2;
     out->cluster = pairs * cluster <= full && (tiles + cluster - 1) / cluster <= (pairs < 32 ? 12 : 16) ? cluster : 0;
-    out->workers = (int)(out->cluster ? pairs * out->cluster : max(1LL, min((long long)full, (tiles + 1) * pairs)));
+    // With many more pairs than blocks fit, blocks of their own in several rounds are balanced by their number and end a
+    // pair without holding the next one up: 128 sequences of 1000 positions in int8 51.7 us and 66.4 cut, 128 of 2048 93.6
+    // and 109.1 (fp16 85.0 and 87.3, 161.3 and 167.1).  From some forty tiles on the last round's tail costs more (64
+    // sequences of 1 to 4000, fp16: 91.6 and 87.6), and just over one round (320 pairs for 296 blocks) does too.
+    if (cluster == 1 && 2 * pairs >= 3 * (long long)full && tiles <= 40) out->cluster = 1;
+    out->workers = (int)(out->cluster ? pairs * out->cluster : max(1LL, min((long long)full, (tiles + kEnding) * pairs)));
     out->bytes = out->cluster ? 0 : (size_t)2 * out->workers * out->heads_per_block * (kv.dim + 2) * 4 + (size_t)out->workers * sizeof(Crossing);
     return KAIROS_OK;
 }
