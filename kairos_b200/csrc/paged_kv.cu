@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(256) paged_kv_read_kernel(const KvView kv, con
 template <typename T, typename Codes, int D>
 static int run_write(const void* QKV, const void* positions, const void* slots, const void* steps, const KvView& kv, void* Q,
                      WriteShape p, int* status, cudaStream_t st) {
-    p.tokens_per_block = rows_tokens(p.T, p.H + 2 * kv.heads, p.rot, kCells<T> * (256 / (D / 16)));
+    p.tokens_per_block = rows_tokens(p.T, p.H + 2 * kv.heads, p.rot, kCells<T> * (256 / (D / 16)), 128);
     p.by_q = div_magic(p.H);
     p.by_kv = div_magic(2 * kv.heads);
     p.by_pairs = div_magic(max(1, p.rot / 2));

@@ -112,7 +112,7 @@ static int run_rotary(const void* X, void* Y, const void* positions, const void*
     const unsigned long long* st64 = static_cast<const unsigned long long*>(steps);
     cudaError_t e;
     if (wide) {
-        p.tokens_per_block = rows_tokens(p.tokens, p.H, p.rot, kCells<T> * (256 / (p.D / 16)));
+        p.tokens_per_block = rows_tokens(p.tokens, p.H, p.rot, kCells<T> * (256 / (p.D / 16)), sizeof(T) == 4 ? 64 : 128);
         p.by_heads = div_magic(p.H);
         p.by_pairs = div_magic(max(1, p.rot / 2));
         p.by_lanes = div_magic(p.D / 16);

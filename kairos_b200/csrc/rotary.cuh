@@ -171,18 +171,18 @@ constexpr int kTablePairs = 2048;   // pairs whose cos and sin a block keeps: 16
 inline unsigned div_magic(int d) { return d == 1 ? 0u : (unsigned)((0x100000000ull + d - 1) / d); }
 __device__ __forceinline__ int div_small(int i, unsigned magic) { return magic ? (int)__umulhi((unsigned)i, magic) : i; }
 
-// Tokens of a block: 128 rows (heads of tokens) or a few more, so that they fill whole batches of `batch` rows (what its
-// threads have under way together) best, where there are enough tokens for every SM to have two such blocks; else one
-// token, so that a decode step spreads over the SMs.  64 and 256 rows measured up to 25% and 14% slower.  The angles of a
-// block's tokens fit its table.
-inline int rows_tokens(long long tokens, int rows, int rot, int batch) {
-    if (tokens * rows < 2 * 148 * 128) return 1;
+// Tokens of a block: about `target` rows (heads of tokens) or up to twice as many, so that they fill whole batches of
+// `batch` rows (what its threads have under way together) best, where there are enough tokens for every SM to have two such
+// blocks; else one token, so that a decode step spreads over the SMs.  128 rows of 16-bit values, 64 of fp32 ones: half and
+// twice as many measured up to 25% and 14% slower.  The angles of a block's tokens fit its table.
+inline int rows_tokens(long long tokens, int rows, int rot, int batch, int target) {
+    if (tokens * rows < 2 * 148 * target) return 1;
     const int most = min(64, rot ? kTablePairs / (rot / 2) : 64);
     int best = 1;
     long long best_done = 0, best_room = 1;                 // rows of a block over the rows of its batches
-    for (int tb = 1; tb <= most && (tb == 1 || tb * rows <= 256); ++tb) {
+    for (int tb = 1; tb <= most && (tb == 1 || tb * rows <= 2 * target); ++tb) {
         const long long done = (long long)tb * rows, room = (done + batch - 1) / batch * batch;
-        if (done < 112 && tb < most && (tb + 1) * rows <= 256) continue;
+        if (8 * done < 7 * target && tb < most && (tb + 1) * rows <= 2 * target) continue;
         if (done * best_room > best_done * room) best = tb, best_done = done, best_room = room;
     }
     return best;
