@@ -275,7 +275,7 @@ int kairos_paged_kv_read(const kairos_kv_layer* kv, const void* slots, void* K_o
 /* Attention of one new token per sequence: O[b,h,:] = sum_j softmax_j(scale * Q[b,h,:] . K[j,:]) V[j,:] over the
  * sequence's lens[b] positions, position j at offset j % page_size of page page_table[b, j / page_size].
  * Q [B, H, D] F16 / BF16 with element strides {b, h} (multiples of 8); O dense [B, H, D] of the same type; a 16-bit cache has Q's
- * type.  H % kv_heads == 0 (head h reads kv head h / (H / kv_heads)).  LSE [B, H] fp32 (natural logarithm of the
+ * type.  table_width * page_size <= 2^30 and H % kv_heads == 0 (head h reads kv head h / (H / kv_heads)).  LSE [B, H] fp32 (natural logarithm of the
  * softmax's denominator) when not null.  lens[b] <= 0: O = 0, LSE = -inf.  Entries of the table behind the end may
  * hold anything.  A page outside the pool is left out of the sum, lens[b] is cut to table_width * page_size, and both
  * raise the status word (KAIROS_ERR_ARG).  Scores, softmax sums and outputs are accumulated in fp32.

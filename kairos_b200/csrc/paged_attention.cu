@@ -161,6 +161,12 @@ __device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
+__device__ __forceinline__ void lds(uint32_t (&v)[4], uint32_t a) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void lds(uint32_t (&v)[2], uint32_t a) {
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a) : "memory");
+}
 __device__ __forceinline__ void mma(__half, float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -263,9 +269,12 @@ struct Ring {
     static constexpr int kRows = kSub * kRowBytes;
     static constexpr int kStage = 2 * kRows + (kCoded ? 2 * kSub * 4 : 0);
     static constexpr int kStages = kRowBytes >= 128 ? 3 : 4;
-    static constexpr int kBytes = kWarps * kStages * kStage;
+    static constexpr int kRing = kStages * kStage;
+    static constexpr int kBytes = kWarps * kRing + kRowBytes;                  // the rings begin at a multiple of a row
     static constexpr int kBlocksPerSm = kBytes > 112 * 1024 ? 1 : kBytes > 74 * 1024 ? 2 : kBytes > 55 * 1024 ? 3 : 4;
     static_assert(8 * kHalves * D * 4 <= kStage, "a warp's output rows fit one stage of its ring");
+    static_assert(kStage % kRowBytes == 0, "stages begin at a multiple of a row: chunk addresses are xored into them");
+    static constexpr int kSwizzle = kRowBytes >= 128 ? 7 : 0;                  // bits of a row that move its chunks (64 bytes: see place)
 };
 
 // One worker's part of one pair.
@@ -283,7 +292,8 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
     using MT = typename std::conditional<kCoded, __half, QT>::type;
     using R = Ring<D, kCoded, kHalves>;
     constexpr int kHeads = 8 * kHalves, kSteps = R::kSub / 16, kTile = R::kTile;
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ __align__(128) uint8_t dynamic[];
+    uint8_t* const smem = dynamic + ((0u - smem_u32(dynamic)) & (R::kRowBytes - 1));
     __shared__ float jm[kWarps][kHeads], jl[kWarps][kHeads];
     __shared__ uint32_t jslot[kWarps];
     __shared__ float2 jpart[kHeads];
@@ -347,12 +357,18 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
     };
     if (!p.cluster && threadIdx.x == 0) record({0, 0, 0, blockIdx.x});
 
-    uint8_t* ring = smem + warp * (R::kStages * R::kStage);
+    uint8_t* ring = smem + warp * R::kRing;
     const uint32_t ring_u = smem_u32(ring);
     const int page_mask = (1 << kv.page_shift) - 1;
-    int slot = 0;                               // ring slot of the next stage to read
+    int cur = 0, prev = R::kRing - R::kStage;   // byte offsets in the ring: the next stage to read, and the one before it
     unsigned bad = 0;                           // per 16 positions of a slot: page outside the pool
-    int k0, k1, count, head;                    // this warp's positions: k0 .. k0 + kSub - 1, then `stride` further, below k1
+    int k0, k1, head;                           // this warp's positions: k0 .. k0 + kSub - 1, then `stride` further, below k1
+    // Where this lane reads and writes in a stage; a chunk or row further is an xor of chunk bits or a constant.
+    const uint32_t k_lane = place<R::kRowBytes>(lane & 15, lane >> 4);
+    const uint32_t v_lane = R::kRows + (kCoded ? place<R::kRowBytes>(2 * t, g * (D / 8) >> 4) + (g * (D / 8) & 15)
+                                               : place<R::kRowBytes>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1));
+    const uint32_t cp_lane = place<R::kRowBytes>(lane / R::kChunks, lane % R::kChunks);
+    constexpr int kCpRows = 32 / R::kChunks;    // rows that a warp copies at once
     const int* pages;
     // this lane's first 16 bytes of the segment's head in page 0, of its scales (lanes 0..3: K, 4..7: V); a page further
     const uint8_t *seg_k, *seg_v;
@@ -363,25 +379,23 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
     uint32_t qb[D / 16][2 * kHalves];
     float unit[kHalves][2];                     // score = product * unit (* scale of the key), heads 2 t and 2 t + 1 (+ 8)
 
-    auto look = [&](int i, int (&to)[kSteps]) {
+    auto look = [&](int key0, int (&to)[kSteps]) {
 #pragma unroll
         for (int h = 0; h < kSteps; ++h) {
-            const int key = k0 + i * stride + 16 * h;
+            const int key = key0 + 16 * h;
             if (h == 0 || kv.page_shift < 5) to[h] = key < k1 ? __ldcg(pages + (key >> kv.page_shift)) : 0;
             else to[h] = to[0];
         }
     };
-    auto request = [&](int i, int st, const int (&from)[kSteps]) {     // stage i of the segment, in pages `from`, into slot st
-        if (i < count) {
-            const uint32_t dst = ring_u + st * R::kStage;
+    auto request = [&](int key0, int slot, const int (&from)[kSteps]) {    // positions from key0 on, in pages `from`, into a slot
+        if (key0 < k1) {
+            const uint32_t dst = ring_u + slot;
 #pragma unroll
             for (int h = 0; h < kSteps; ++h) {
-                const int key = k0 + i * stride + 16 * h, real = k1 - key;
+                const int key = key0 + 16 * h, real = k1 - key;
                 const bool ok = (unsigned)from[h] < (unsigned)kv.pages;
-                const unsigned bit = 1u << (st * kSteps + h);
-                bad &= ~bit;
                 if (!ok && real > 0) {
-                    bad |= bit;
+                    bad |= 1u << (slot / R::kStage * kSteps + h);
                     *status = KAIROS_ERR_ARG;
                 }
                 const unsigned page = ok ? (unsigned)from[h] : 0u, in_page = (unsigned)(key & page_mask);
@@ -391,16 +405,17 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
                 if (ok && real >= 16) {
 #pragma unroll
                     for (int n = 0; n < R::kChunks / 2; ++n) {
-                        const int c = lane + 32 * n;
-                        cp16(dst + place<R::kRowBytes>(16 * h + c / R::kChunks, c % R::kChunks), ks + 512 * n);
-                        cp16(dst + R::kRows + place<R::kRowBytes>(16 * h + c / R::kChunks, c % R::kChunks), vs + 512 * n);
+                        const uint32_t to = ((dst + cp_lane) ^ ((n * kCpRows & R::kSwizzle) << 4)) + (16 * h + n * kCpRows) * R::kRowBytes;
+                        cp16(to, ks + 512 * n);
+                        cp16(to + R::kRows, vs + 512 * n);
                     }
                 } else {                        // rows behind the end, or of no page, are zeros: 0 * weight stays 0
 #pragma unroll
                     for (int n = 0; n < R::kChunks / 2; ++n) {
-                        const int c = lane + 32 * n, r = c / R::kChunks;
-                        cp16(dst + place<R::kRowBytes>(16 * h + r, c % R::kChunks), ks + 512 * n, ok && r < real);
-                        cp16(dst + R::kRows + place<R::kRowBytes>(16 * h + r, c % R::kChunks), vs + 512 * n, ok && r < real);
+                        const uint32_t to = ((dst + cp_lane) ^ ((n * kCpRows & R::kSwizzle) << 4)) + (16 * h + n * kCpRows) * R::kRowBytes;
+                        const bool there = ok && n * kCpRows + lane / R::kChunks < real;
+                        cp16(to, ks + 512 * n, there);
+                        cp16(to + R::kRows, vs + 512 * n, there);
                     }
                 }
                 if constexpr (kCoded) {         // lanes 0..3: scales of K, 4..7: of V
@@ -419,20 +434,19 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
         const int rows = min(kHeads, p.group - block * kHeads);
         k0 = sg.tile * kTile + warp * R::kSub;
         k1 = p.cluster ? sg.len : min((sg.tile + sg.take) * kTile, sg.len);
-        count = k0 < k1 ? (k1 - k0 + stride - 1) / stride : 0;
         pages = table + (size_t)sg.b * p.table_stride;
         const unsigned head_row = (unsigned)head << kv.page_shift;
         seg_k = static_cast<const uint8_t*>(kv.k) + (size_t)head_row * R::kRowBytes + lane * 16;
         seg_v = static_cast<const uint8_t*>(kv.v) + (size_t)head_row * R::kRowBytes + lane * 16;
         if constexpr (kCoded) seg_scale = (lane < 4 ? kv.ks : kv.vs) + head_row + (lane & 3) * 4;
-        int st = slot;
-        if (!p.cluster) look(0, first_pages[0]);
+        int slot = cur;
+        if (!p.cluster) look(k0, first_pages[0]);
 #pragma unroll
         for (int i = 0; i < R::kStages - 1; ++i) {
-            if (i + 1 == R::kStages - 1) look(i + 1, ahead);
-            else if (!p.cluster) look(i + 1, first_pages[i + 1]);
-            request(i, st, first_pages[i]);
-            st = st + 1 == R::kStages ? 0 : st + 1;
+            if (i + 1 == R::kStages - 1) look(k0 + (i + 1) * stride, ahead);
+            else if (!p.cluster) look(k0 + (i + 1) * stride, first_pages[i + 1]);
+            request(k0 + i * stride, slot, first_pages[i]);
+            slot = slot == R::kRing - R::kStage ? 0 : slot + R::kStage;
         }
         // q as the second operand: head g (and g + 8).  For a coded cache the channels of a step are permuted as the code
         // words lie: a thread's four channels are 4 t .. 4 t + 3.
@@ -510,17 +524,23 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
             for (int e = 0; e < 2; ++e) m[r][e] = -INFINITY, base[r][e] = kUnset, l[r][e] = 0.f;
 
 #pragma unroll 1
-        for (int i = 0; i < count; ++i) {
+        for (int pos = k0; pos < k1; pos += stride) {
             cp_wait<R::kStages - 2>();
             __syncwarp();                       // every lane's copies have landed; the stage before has been read
-            request(i + R::kStages - 1, slot == 0 ? R::kStages - 1 : slot - 1, ahead);
-            look(i + R::kStages, ahead);
-            const uint32_t ku = ring_u + slot * R::kStage, vu = ku + R::kRows;
-            const uint8_t* stage = ring + slot * R::kStage;
-            const int real = k1 - (k0 + i * stride);
-            const unsigned gone = (bad >> (slot * kSteps)) & ((1u << kSteps) - 1);
-            const bool full = real >= R::kSub && gone == 0;     // the same in all lanes
-            slot = slot + 1 == R::kStages ? 0 : slot + 1;
+            request(pos + (R::kStages - 1) * stride, prev, ahead);
+            look(pos + R::kStages * stride, ahead);
+            const uint32_t ku = ring_u + cur + k_lane, vu = ring_u + cur + v_lane;
+            const uint8_t* stage = ring + cur;
+            const int real = k1 - pos;
+            const bool full = real >= R::kSub && bad == 0;      // the same in all lanes
+            unsigned gone = 0;
+            if (!full) {
+                const int shift = cur / R::kStage * kSteps;
+                gone = (bad >> shift) & ((1u << kSteps) - 1);
+                bad &= ~(gone << shift);
+            }
+            prev = cur;
+            cur = cur == R::kRing - R::kStage ? 0 : cur + R::kStage;
 
             // scores^T of step h: positions g and g + 8, heads 2 t and 2 t + 1: [0], [1] and [2], [3]
             float s[kSteps][kHalves][4] = {};
@@ -529,7 +549,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
 #pragma unroll
                 for (int h = 0; h < kSteps; ++h) {
                     uint32_t w[4];              // uncoded: one step of channels; coded: two
-                    ldsm4(ku + place<R::kRowBytes>(16 * h + (lane & 15), (kCoded ? c : 2 * c) + (lane >> 4)), w);
+                    ldsm4((ku ^ ((kCoded ? c : 2 * c) << 4)) + 16 * h * R::kRowBytes, w);
                     if constexpr (!kCoded) {
 #pragma unroll
                         for (int r = 0; r < kHalves; ++r)
@@ -673,7 +693,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
 #pragma unroll
                     for (int j = 0; j < D / 16; ++j) {
                         uint32_t w[4];
-                        ldsm4t(vu + place<R::kRowBytes>(16 * h + (lane & 7) + ((lane >> 4) << 3), 2 * j + ((lane >> 3) & 1)), w);
+                        ldsm4t((vu ^ (2 * j << 4)) + 16 * h * R::kRowBytes, w);
                         weigh(j, w[0], w[1], w[2], w[3]);
                     }
                 } else {
@@ -683,12 +703,8 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
                     for (int c = 0; c < D / 8 / (4 * kWords); ++c) {
                         uint32_t v[4][kWords];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const int key = 16 * h + 2 * t + (k & 1) + ((k >> 1) << 3), byte = g * (D / 8) + c * 16;
-                            const uint8_t* from = stage + R::kRows + place<R::kRowBytes>(key, byte >> 4) + (byte & 15);
-                            if constexpr (kWords == 4) *reinterpret_cast<uint4*>(v[k]) = *reinterpret_cast<const uint4*>(from);
-                            else *reinterpret_cast<uint2*>(v[k]) = *reinterpret_cast<const uint2*>(from);
-                        }
+                        for (int k = 0; k < 4; ++k)        // positions 2 t, 2 t + 1, and 8 further
+                            lds(v[k], (vu ^ ((c ^ (k & 1 & R::kSwizzle)) << 4)) + (16 * h + (k & 1) + 8 * (k >> 1)) * R::kRowBytes);
 #pragma unroll
                         for (int w = 0; w < kWords; ++w)
 #pragma unroll
@@ -708,15 +724,15 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
         const bool first = first_segment;
         __syncwarp();                           // every lane has read the last stage
         more = next();
-        // the one slot that start() leaves alone; any will do where nothing follows
-        const uint32_t free_slot = more && slot != 0 ? slot - 1 : R::kStages - 1;
+        // the one slot that start() leaves alone; where nothing follows, any but the first will do
+        const uint32_t free_slot = more ? prev : R::kRing - R::kStage;
         if (more) start(seg);
 
         // ---- the four warps' parts become one: each leaves its rows in a slot of its ring.  Column c of row r lies at
         // c ^ 8 (r / 2 % 4): the lanes of a store fall on different banks
         auto at = [](int r, int c) { return r * D + (c ^ (((r >> 1) & 3) << 3)); };
-        float* mine = reinterpret_cast<float*>(ring + free_slot * R::kStage);
-        if (lane == 0) jslot[warp] = (uint32_t)(warp * R::kStages + free_slot) * R::kStage;
+        float* mine = reinterpret_cast<float*>(ring + free_slot);
+        if (lane == 0) jslot[warp] = warp * R::kRing + free_slot;
 #pragma unroll
         for (int r = 0; r < kHalves; ++r)
 #pragma unroll
@@ -1000,7 +1016,7 @@ extern "C" int kairos_paged_attention(const void* Q, long long q_b, long long q_
     int rc = kv_view(layer, &kv);
     if (rc != KAIROS_OK) return rc;
     if (B < 0 || B > 65535 || H <= 0 || H % kv.heads != 0 || table_width < 0 || table_stride < 0 ||
-        ((long long)table_width << kv.page_shift) > 0x7fffffffLL)
+        ((long long)table_width << kv.page_shift) > (1LL << 30))    // positions and those looked ahead for fit an int
         return KAIROS_ERR_SHAPE;
     const bool coded = layer->dtype == KAIROS_DTYPE_I8 || layer->dtype == KAIROS_DTYPE_E4M3;
     if ((dtype != KAIROS_DTYPE_F16 && dtype != KAIROS_DTYPE_BF16) || (!coded && layer->dtype != dtype)) {
