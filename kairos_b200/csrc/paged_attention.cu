@@ -40,7 +40,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 struct AttnShape {
     long long qb, qh, table_stride;
     int B, H, group, blocks_per_kv;         // head blocks (of 8 or 16 query heads) per kv head
-    int table_width, workers;
+    int table_width, workers, lanes;        // the even cut: workers in `lanes` equal parts, each with its own pairs
     int cluster;                            // blocks of a cluster that share one pair; 0: the even cut over all workers
     float scale_log2;
 };
@@ -49,8 +49,8 @@ struct AttnShape {
 __device__ __forceinline__ int seq_len(const int* lens, int b, int most) { return max(0, min(__ldcg(lens + b), most)); }
 
 struct Cut {
-    unsigned total, run;                    // units of all pairs, units per worker
-    int b, pair, unit;                      // where flat unit `x` lies: sequence, pair (kv head, head block) and unit of it
+    unsigned total, run;                    // units of a lane, units per worker
+    int b, pair, unit;                      // where the worker begins: sequence, pair (kv head, head block) and unit of it
     int len;                                // of that sequence
 };
 
@@ -64,9 +64,11 @@ __device__ __forceinline__ unsigned units_of(int len) { return len > 0 ? (unsign
 // needs for so many.
 constexpr unsigned kSpare = 6;
 
-// Block-wide (128 threads).  Scans the sequences' units and finds the flat unit x where worker blockIdx.x begins; returns
-// false where it has no work.  If every pair is short -- no more than kSpare units over the even run -- and there are no
-// more pairs than workers, a worker takes one whole pair (run = 0).
+// Block-wide (128 threads).  Scans the sequences' units and finds where worker blockIdx.x begins; returns false where it
+// has no work.  Pair p belongs to lane p % lanes and worker w is number w / lanes of lane w % lanes; a lane's pairs lie end
+// to end, sequence after sequence, and its workers take equal runs.  With a lane per pair of a sequence, neighbouring
+// workers read the same pages' heads at the same time.  If every pair is short -- no more than kSpare units over the even
+// run -- and there are no more pairs than workers, a worker takes one whole pair (run = 0).
 template <int kTile>
 __device__ __forceinline__ bool locate(const int* lens, const AttnShape& p, int pairs, int most, Cut* out) {
     __shared__ unsigned warp_sum[kWarps], warp_top[kWarps];
@@ -97,8 +99,10 @@ __device__ __forceinline__ bool locate(const int* lens, const AttnShape& p, int 
         total += warp_sum[w];
         top = max(top, warp_top[w]);
     }
-    total *= pairs;
-    const unsigned run = (total + p.workers - 1) / p.workers;
+    const unsigned deep = pairs / p.lanes, team = p.workers / p.lanes, rank = blockIdx.x / p.lanes;
+    const int lane = blockIdx.x - rank * p.lanes;
+    total *= deep;
+    const unsigned run = (total + team - 1) / team;
     const bool whole = top <= run + kSpare && (long long)p.B * pairs <= p.workers;
     if (whole) {
         const int b = blockIdx.x / pairs;
@@ -106,16 +110,16 @@ __device__ __forceinline__ bool locate(const int* lens, const AttnShape& p, int 
         *out = Cut{total, 0, b, (int)(blockIdx.x - b * pairs), 0, seq_len(lens, b, most)};
         return out->len > 0;
     }
-    const unsigned x = blockIdx.x * run;
+    const unsigned x = rank * run;
     if (x >= total) return false;           // the same for every thread
     unsigned before = upto - mine;
-    if (x >= before * pairs && x < upto * pairs) {
+    if (x >= before * deep && x < upto * deep) {
         for (int b = first; b < last; ++b) {
             const int len = per == 1 ? own_len : seq_len(lens, b, most);
             const unsigned n = units_of<kTile>(len);
-            if (x < (before + n) * pairs) {
-                const unsigned rest = x - before * pairs;
-                found = Cut{total, run, b, (int)(rest / n), (int)(rest % n), len};
+            if (x < (before + n) * deep) {
+                const unsigned rest = x - before * deep;
+                found = Cut{total, run, b, (int)(rest / n) * p.lanes + lane, (int)(rest % n), len};
                 break;
             }
             before += n;
@@ -324,7 +328,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
         seg.tiles = seg.take = (seg.len + kTile - 1) / kTile;
         more = seg.len > 0;                     // the same for the whole cluster; a block without tiles joins with nothing
     } else if (locate<kTile>(lens, p, pairs, most, &cut)) {
-        left = cut.run ? min(cut.run, cut.total - blockIdx.x * cut.run) : units_of<kTile>(cut.len);
+        left = cut.run ? min(cut.run, cut.total - blockIdx.x / p.lanes * cut.run) : units_of<kTile>(cut.len);
         seg = {cut.b, cut.pair, cut.unit, 0, 0, cut.len};
     }
     bool first_segment = true;
@@ -340,8 +344,8 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
     auto next = [&]() {
         do {
             if (left == 0) return false;
-            if (++seg.pair == pairs) {
-                seg.pair = 0;
+            if ((seg.pair += p.lanes) >= pairs) {
+                seg.pair = blockIdx.x % p.lanes;
                 do seg.len = seq_len(lens, ++seg.b, most); while (seg.len == 0);
             }
             seg.tile = 0;
@@ -350,7 +354,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
         return true;
     };
     if (left > 0) more = take() || next();
-    const unsigned run_end = min((blockIdx.x + 1) * cut.run, cut.total);
+    const unsigned run_end = min((blockIdx.x / p.lanes + 1) * cut.run, cut.total);
     auto record = [&](const Crossing& c) {
         *reinterpret_cast<uint4*>(Partials<kHeads, D>::crossing(ws, p.workers, blockIdx.x)) =
             make_uint4((unsigned)c.b, (unsigned)c.pair, c.slot, c.last);
@@ -761,7 +765,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
         const bool whole = done.take == done.tiles;
         const unsigned part = 2 * blockIdx.x + (first ? 0 : 1);
         if (!p.cluster && !whole && done.tile == 0 && threadIdx.x == 0)      // begins here and lies across the run's end
-            record({done.b, done.pair, part, (run_end - done.take + done.tiles - 1) / cut.run});
+            record({done.b, done.pair, part, (run_end - done.take + done.tiles - 1) / cut.run * p.lanes + blockIdx.x % p.lanes});
         for (int i = threadIdx.x; i < rows * (D / 4); i += 128) {
             const int row = i / (D / 4), c = 4 * (i - row * (D / 4));
             float top = -INFINITY;
@@ -829,8 +833,8 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
 }
 
 // Block (w, y): the pair, if any, that begins in worker w's run and lies across its end; a slice of 32 items (a head's four
-// channels) of its partial results of workers w, w + 1, ... .  The four warps share the parts, and the order in which parts
-// are added depends on nothing but their number.
+// channels) of its partial results of workers w, w + lanes, ... .  The four warps share the parts, and the order in which
+// parts are added depends on nothing but their number.
 template <typename QT, int D, int kHeads>
 __global__ void __launch_bounds__(128) paged_attention_join_kernel(QT* __restrict__ O, float* __restrict__ LSE,
                                                                    float* __restrict__ ws, const AttnShape p) {
@@ -859,12 +863,13 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(QT* __restric
         acc.w = __fmaf_rn(acc.w, keep, f * v.w);
     };
     if (row < rows) {
-        for (unsigned w = blockIdx.x + warp; w <= last; w += kAhead * kWarps) {
+        const unsigned step = kWarps * p.lanes;
+        for (unsigned w = blockIdx.x + warp * p.lanes; w <= last; w += kAhead * step) {
             float2 ml[kAhead];
             float4 v[kAhead];
 #pragma unroll
             for (int a = 0; a < kAhead; ++a) {
-                const unsigned u = w + a * kWarps;
+                const unsigned u = w + a * step;
                 if (u <= last) {
                     const unsigned slot = u == blockIdx.x ? record.z : 2 * u;
                     ml[a] = __ldcg(reinterpret_cast<const float2*>(P::ml(ws, slot) + 2 * row));
@@ -873,7 +878,7 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(QT* __restric
             }
 #pragma unroll
             for (int a = 0; a < kAhead; ++a)
-                if (w + a * kWarps <= last) add(ml[a], v[a]);
+                if (w + a * step <= last) add(ml[a], v[a]);
         }
     }
     part_o[warp][lane] = acc;
@@ -901,7 +906,7 @@ static int sm_count() {
 }
 
 struct Plan {
-    int heads_per_block, blocks_per_kv, workers, cluster;
+    int heads_per_block, blocks_per_kv, workers, lanes, cluster;
     size_t bytes;
 };
 
@@ -942,7 +947,11 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
     // and 109.1 (fp16 85.0 and 87.3, 161.3 and 167.1).  From some forty tiles on the last round's tail costs more (64
     // sequences of 1 to 4000, fp16: 91.6 and 87.6), and just over one round (320 pairs for 296 blocks) does too.
     if (cluster == 1 && 2 * pairs >= 3 * (long long)full && tiles <= 40) out->cluster = 1;
-    out->workers = (int)(out->cluster ? pairs * out->cluster : max(1LL, min((long long)full, (tiles + kEnding) * pairs)));
+    // The even cut: a lane per pair of a sequence where that leaves at most 3% of the blocks out, else one lane.
+    const long long deep = (long long)kv.heads * out->blocks_per_kv;
+    out->lanes = deep <= full && full / deep * deep * 100 >= 97LL * full ? (int)deep : 1;
+    out->workers = (int)(out->cluster ? pairs * out->cluster
+                                      : max(1LL, min((long long)full / out->lanes, (tiles + kEnding) * pairs / out->lanes)) * out->lanes);
     out->bytes = out->cluster ? 0 : (size_t)2 * out->workers * out->heads_per_block * (kv.dim + 2) * 4 + (size_t)out->workers * sizeof(Crossing);
     return KAIROS_OK;
 }
@@ -977,9 +986,9 @@ static int run_attention(const void* Q, const KvView& kv, const void* table, con
                                        static_cast<const int*>(lens), static_cast<QT*>(O), static_cast<float*>(LSE),
                                        static_cast<float*>(ws), p, status);
     if (e != cudaSuccess) return note_cuda_error(e);
-    if (!plan.cluster && plan.workers > 1) {
+    if (!plan.cluster && plan.workers > plan.lanes) {
         constexpr int kSlices = D / 4 / (32 / (8 * kHalves));
-        e = launch_chained(paged_attention_join_kernel<QT, D, 8 * kHalves>, dim3(plan.workers - 1, kSlices), dim3(128), 0, st,
+        e = launch_chained(paged_attention_join_kernel<QT, D, 8 * kHalves>, dim3(plan.workers - plan.lanes, kSlices), dim3(128), 0, st,
                            static_cast<QT*>(O), static_cast<float*>(LSE), static_cast<float*>(ws), p);
         if (e != cudaSuccess) return note_cuda_error(e);
     }
@@ -1034,7 +1043,7 @@ extern "C" int kairos_paged_attention(const void* Q, long long q_b, long long q_
     int* status = device_status_word();
     if (!status) return KAIROS_ERR_CUDA;
     const AttnShape p = {q_b, q_h, table_stride, B, H, H / kv.heads, plan.blocks_per_kv, table_width,
-                         plan.workers, plan.cluster, scale * kLog2e};
+                         plan.workers, plan.lanes, plan.cluster, scale * kLog2e};
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (dtype == KAIROS_DTYPE_F16) {
         if (layer->dtype == KAIROS_DTYPE_I8) return pick_attention<__half, WidenI8>(Q, kv, page_table, lens, O, LSE, workspace, p, plan, status, st);
