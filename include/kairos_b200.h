@@ -50,9 +50,10 @@ enum {
 int kairos_abi_version(void);
 const char* kairos_status_str(int status);
 const char* kairos_last_error(void);
-/* Status words the kernels raise when one of their bounded waits runs out (current device), including the
+/* Status words the kernels raise when one of their bounded waits runs out (KAIROS_ERR_DEVICE) or an index in device
+ * memory lies outside what it indexes (KAIROS_ERR_ARG, see the paged cache) on the current device, including the
  * word of kairos_w4a16_gemm_noalloc.  Read it after synchronising (the call itself synchronises the device
- * once that entry has been used); clear != 0 resets it.  KAIROS_OK or KAIROS_ERR_DEVICE. */
+ * once that entry has been used); clear != 0 resets it.  KAIROS_OK or one of the two. */
 int kairos_device_status(int clear);
 /* Self-test of that mechanism (no counterpart in the reference): launches one CTA that waits, through the
  * routine all pipeline kernels use, on a barrier nothing completes; the wait gives up after about a

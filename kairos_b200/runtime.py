@@ -75,7 +75,8 @@ def stream_ptr(device=None):
 
 
 def device_status(clear=True):
-    """KAIROS_OK (0) or KAIROS_ERR_DEVICE after the caller synchronised."""
+    """KAIROS_OK (0), KAIROS_ERR_DEVICE (a bounded wait ran out) or KAIROS_ERR_ARG (a page, slot or length outside its
+    range) after the caller synchronised."""
     return lib.kairos_device_status(1 if clear else 0)
 
 

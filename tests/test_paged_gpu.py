@@ -464,6 +464,8 @@ def test_attention_strides_tables_and_out():
     assert torch.equal(ops.paged_attention(q, c, wide_table[:, :table.shape[1]], n), ref)
     out = torch.full_like(ref, 7)
     assert ops.paged_attention(q, c, table, n, out=out) is out and torch.equal(out, ref)
+    own = q.clone()
+    assert ops.paged_attention(own, c, table, n, out=own) is own and torch.equal(own, ref)     # the result over the queries
     # one sequence's pages shared by the whole batch (stride 0)
     many = ops.paged_attention(q[2:].expand(4, -1, -1).contiguous(), c, table[2:].expand(4, -1), n[2:].expand(4).contiguous())
     assert all(torch.equal(m, ref[2]) for m in many)
