@@ -268,21 +268,24 @@ __device__ __forceinline__ uint32_t place(int r, int c) {
     else return r * ROWB + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
-// A warp's ring.  A stage holds 16 or 32 positions; a warp's output rows have to fit one (see the joining of warps).
-// int8, 128 channels, 128 sequences up to 8192: 16 positions x 3 stages x 4 blocks an SM 195 us, 16 x 4 x 3 199, 32 x 2 x 3
-// 201, 32 x 3 x 2 230.  fp16, one of 131071: 16 x 3 x 2 95 us, 16 x 2 x 3 101, 32 x 3 x 1 104.
+// A warp's ring.  A stage holds 16 positions, 32 where a warp's output rows of 16 heads need the room (see the joining of
+// warps); stages and blocks on an SM by what registers and measurements allow.
+// int8, 128 channels, 128 sequences up to 8192: 16 positions x 2 stages x 4 blocks an SM 178 us, 16 x 3 x 4 180 (and 3 to 9%
+// behind on smaller batches), 16 x 4 x 3 180; before the loop was cut down 16 x 3 x 4 195, 32 x 2 x 3 201, 32 x 3 x 2 230.
+// fp16, one of 131071: 16 x 3 x 2 95 us, 16 x 2 x 3 101, 32 x 3 x 1 104.  64 sequences up to 4000, 256 channels int8:
+// 16 x 2 x 2 96 us, 16 x 3 x 2 100, 32 x 3 x 1 151; 64 channels fp16 16 x 3 x 4 49, 32 x 3 x 2 58, int8 16 x 4 x 4 38, 32 x 4 x 3 41.
 template <int D, bool kCoded, int kHalves>
 struct Ring {
     static constexpr int kRowBytes = kCoded ? D : 2 * D;
     static constexpr int kChunks = kRowBytes / 16;
-    static constexpr int kSub = kRowBytes >= 256 && !kCoded ? 16 : kHalves == 1 && D == 128 ? 16 : 32;
+    static constexpr int kSub = kHalves == 1 || (kRowBytes >= 256 && !kCoded) ? 16 : 32;
     static constexpr int kTile = kSub * kWarps;                                // positions per scheduling tile
     static constexpr int kRows = kSub * kRowBytes;
-    static constexpr int kStage = 2 * kRows + (kCoded ? 2 * kSub * 4 : 0);
-    static constexpr int kStages = kRowBytes >= 128 ? 3 : 4;
+    static constexpr int kStage = (2 * kRows + (kCoded ? 2 * kSub * 4 : 0) + kRowBytes - 1) / kRowBytes * kRowBytes;
+    static constexpr int kStages = kCoded && D >= 128 && kHalves == 1 ? 2 : kRowBytes >= 128 ? 3 : 4;
     static constexpr int kRing = kStages * kStage;
     static constexpr int kBytes = kWarps * kRing + kRowBytes;                  // the rings begin at a multiple of a row
-    static constexpr int kBlocksPerSm = kBytes > 112 * 1024 ? 1 : kBytes > 74 * 1024 ? 2 : kBytes > 55 * 1024 ? 3 : 4;
+    static constexpr int kBlocksPerSm = kBytes > 112 * 1024 ? 1 : kBytes > 74 * 1024 || D == 256 ? 2 : kBytes > 55 * 1024 ? 3 : 4;
     static_assert(8 * kHalves * D * 4 <= kStage, "a warp's output rows fit one stage of its ring");
     static_assert(kStage % kRowBytes == 0, "stages begin at a multiple of a row: chunk addresses are xored into them");
     static constexpr int kSwizzle = kRowBytes >= 128 ? 7 : 0;                  // bits of a row that move its chunks (64 bytes: see place)
@@ -293,13 +296,16 @@ struct Segment {
     int b, pair, tile, tiles, take, len;
 };
 
-// QT: type of q and o; Widen: void for a cache of type QT, else how codes become fp16; kHalves: 1 (up to 8 query heads in
-// a block) or 2 (16).
-template <typename QT, typename Widen, int D, int kHalves>
-__global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHalves>::kBlocksPerSm))
+// QT: type of q and o; Widen: void for a cache of type QT, else how codes become fp16; kBlockHeads: query heads of a block,
+// 4, 8 or 16.  With 4, columns 4..7 of the products are the same heads again: their scores and weights come out the same
+// without exchange, and in the second product the first four columns carry the weights and the others their remainders, so
+// it is one instruction where 8 heads need two.
+template <typename QT, typename Widen, int D, int kBlockHeads>
+__global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kBlockHeads + 7) / 8>::kBlocksPerSm))
     paged_attention_kernel(const QT* __restrict__ Q, const KvView kv, const int* __restrict__ table, const int* __restrict__ lens,
                            QT* __restrict__ O, float* __restrict__ LSE, float* __restrict__ ws, const AttnShape p, int* status) {
-    constexpr bool kCoded = !std::is_void<Widen>::value;
+    constexpr bool kCoded = !std::is_void<Widen>::value, kTwin = kBlockHeads == 4;
+    constexpr int kHalves = (kBlockHeads + 7) / 8;
     using MT = typename std::conditional<kCoded, __half, QT>::type;
     using R = Ring<D, kCoded, kHalves>;
     constexpr int kHeads = 8 * kHalves, kSteps = R::kSub / 16, kTile = R::kTile;
@@ -442,7 +448,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
     auto start = [&](const Segment& sg) {
         head = sg.pair / p.blocks_per_kv;
         const int block = sg.pair - head * p.blocks_per_kv;
-        const int rows = min(kHeads, p.group - block * kHeads);
+        const int rows = min(kHeads, p.group - block * kHeads);            // of 4 heads a block: the whole group
         k0 = sg.tile * kTile + warp * R::kSub;
         k1 = p.cluster ? sg.len : min((sg.tile + sg.take) * kTile, sg.len);
         pages = table + (size_t)sg.b * p.table_stride;
@@ -464,8 +470,9 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
 #pragma unroll
         for (int r = 0; r < kHalves; ++r) {
             unit[r][0] = unit[r][1] = p.scale_log2;
-            const bool real = g + 8 * r < rows;
-            const QT* q = Q + (size_t)sg.b * p.qb + (size_t)(head * p.group + block * kHeads + (real ? g + 8 * r : 0)) * p.qh;
+            const int row = kTwin ? g & 3 : g + 8 * r;
+            const bool real = row < rows;
+            const QT* q = Q + (size_t)sg.b * p.qb + (size_t)(head * p.group + block * kHeads + (real ? row : 0)) * p.qh;
 #pragma unroll
             for (int s = 0; s < D / 16; ++s) {
                 uint32_t lo, hi;
@@ -688,8 +695,12 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
                         }
                         uint32_t hi, lo;
                         split(MT(), w0, w1, &hi, &lo);
-                        wb[h][r][k] = transpose8(hi);
-                        rest[h][r][k] = transpose8(lo);
+                        if constexpr (kTwin) {
+                            wb[h][r][k] = transpose8(t < 2 ? hi : lo);
+                        } else {
+                            wb[h][r][k] = transpose8(hi);
+                            rest[h][r][k] = transpose8(lo);
+                        }
                     }
 #pragma unroll
             for (int h = 0; h < kSteps; ++h) {
@@ -697,7 +708,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
 #pragma unroll
                     for (int r = 0; r < kHalves; ++r) {
                         mma(MT(), o[j][r], a0, a1, a2, a3, wb[h][r][0], wb[h][r][1]);
-                        mma(MT(), o[j][r], a0, a1, a2, a3, rest[h][r][0], rest[h][r][1]);
+                        if constexpr (!kTwin) mma(MT(), o[j][r], a0, a1, a2, a3, rest[h][r][0], rest[h][r][1]);
                     }
                 };
                 if constexpr (!kCoded) {
@@ -784,7 +795,12 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, kHa
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 const float f = exp2_fast(jm[w][row] - safe);
-                const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + jslot[w]) + at(row, c));
+                const float* from = reinterpret_cast<const float*>(smem + jslot[w]);
+                float4 v = *reinterpret_cast<const float4*>(from + at(row, c));
+                if constexpr (kTwin) {          // what the remainders gave
+                    const float4 u = *reinterpret_cast<const float4*>(from + at(row + 4, c));
+                    v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+                }
                 sum = __fmaf_rn(f, jl[w][row], sum);
                 acc.x = __fmaf_rn(f, v.x, acc.x);
                 acc.y = __fmaf_rn(f, v.y, acc.y);
@@ -921,7 +937,7 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
     const int sms = sm_count();
     if (sms <= 0) return note_cuda_error(cudaGetLastError());
     const int group = H / kv.heads;
-    out->heads_per_block = group > 8 ? 16 : 8;
+    out->heads_per_block = group > 8 ? 16 : group > 4 ? 8 : 4;
     out->blocks_per_kv = (group + out->heads_per_block - 1) / out->heads_per_block;
     const bool wide = out->heads_per_block == 16;
     int tile = 0, per_sm = 0;
@@ -959,16 +975,17 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
     out->lanes = deep <= full && full / deep * deep * 100 >= 97LL * full ? (int)deep : 1;
     out->workers = (int)(out->cluster ? pairs * out->cluster
                                       : max(1LL, min((long long)full / out->lanes, (tiles + kEnding) * pairs / out->lanes)) * out->lanes);
-    out->bytes = out->cluster ? 0 : (size_t)2 * out->workers * out->heads_per_block * (kv.dim + 2) * 4 + (size_t)out->workers * sizeof(Crossing);
+    out->bytes = out->cluster ? 0 : (size_t)2 * out->workers * max(8, out->heads_per_block) * (kv.dim + 2) * 4 + (size_t)out->workers * sizeof(Crossing);
     return KAIROS_OK;
 }
 
-template <typename QT, typename Widen, int D, int kHalves>
+template <typename QT, typename Widen, int D, int kBlockHeads>
 static int run_attention(const void* Q, const KvView& kv, const void* table, const void* lens, void* O, void* LSE, void* ws,
                          const AttnShape& p, const Plan& plan, int* status, cudaStream_t st) {
+    constexpr int kHalves = (kBlockHeads + 7) / 8;
     using R = Ring<D, !std::is_void<Widen>::value, kHalves>;
     static PerDeviceFlag flag;
-    auto kernel = paged_attention_kernel<QT, Widen, D, kHalves>;
+    auto kernel = paged_attention_kernel<QT, Widen, D, kBlockHeads>;
     const int rc = ensure_dynamic_smem(flag, kernel, R::kBytes);
     if (rc != KAIROS_OK) return rc;
     cudaLaunchConfig_t cfg = {};
@@ -1005,9 +1022,10 @@ static int run_attention(const void* Q, const KvView& kv, const void* table, con
 template <typename QT, typename Widen>
 static int pick_attention(const void* Q, const KvView& kv, const void* table, const void* lens, void* O, void* LSE, void* ws,
                           const AttnShape& p, const Plan& plan, int* status, cudaStream_t st) {
-#define KAIROS_ATTN(D)                                                                                              \
-    (plan.heads_per_block == 8 ? run_attention<QT, Widen, D, 1>(Q, kv, table, lens, O, LSE, ws, p, plan, status, st) \
-                               : run_attention<QT, Widen, D, 2>(Q, kv, table, lens, O, LSE, ws, p, plan, status, st))
+#define KAIROS_ATTN(D)                                                                                                 \
+    (plan.heads_per_block == 4 ? run_attention<QT, Widen, D, 4>(Q, kv, table, lens, O, LSE, ws, p, plan, status, st)   \
+     : plan.heads_per_block == 8 ? run_attention<QT, Widen, D, 8>(Q, kv, table, lens, O, LSE, ws, p, plan, status, st) \
+                                 : run_attention<QT, Widen, D, 16>(Q, kv, table, lens, O, LSE, ws, p, plan, status, st))
     return kv.dim == 64 ? KAIROS_ATTN(64) : kv.dim == 128 ? KAIROS_ATTN(128) : KAIROS_ATTN(256);
 #undef KAIROS_ATTN
 }
