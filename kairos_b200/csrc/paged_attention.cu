@@ -268,27 +268,33 @@ __device__ __forceinline__ uint32_t place(int r, int c) {
     else return r * ROWB + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
-// A warp's ring.  A stage holds 16 positions, 32 where a warp's output rows of 16 heads need the room (see the joining of
-// warps); stages and blocks on an SM by what registers and measurements allow.
-// int8, 128 channels, 128 sequences up to 8192: 16 positions x 2 stages x 4 blocks an SM 178 us, 16 x 3 x 4 180 (and 3 to 9%
-// behind on smaller batches), 16 x 4 x 3 180; before the loop was cut down 16 x 3 x 4 195, 32 x 2 x 3 201, 32 x 3 x 2 230.
-// fp16, one of 131071: 16 x 3 x 2 95 us, 16 x 2 x 3 101, 32 x 3 x 1 104.  64 sequences up to 4000, 256 channels int8:
-// 16 x 2 x 2 96 us, 16 x 3 x 2 100, 32 x 3 x 1 151; 64 channels fp16 16 x 3 x 4 49, 32 x 3 x 2 58, int8 16 x 4 x 4 38, 32 x 4 x 3 41.
+// A warp's ring of stages of 16 positions; stages and blocks on an SM by what registers and measurements allow.
+// int8, 128 channels, 128 sequences up to 8192: 2 stages x 4 blocks an SM 178 us, 3 x 4 180 (and 3 to 9% behind on smaller
+// batches), 4 x 3 180.  fp16, one of 131071: 3 x 2 95 us, 2 x 3 101, stages of 32 positions 3 x 1 104.  64 sequences up to
+// 4000, 256 channels int8: 2 x 2 96 us, 3 x 2 100, stages of 32 positions 3 x 1 151; 64 channels fp16 3 x 4 49, stages of 32
+// positions 3 x 2 58; int8 4 x 4 38, stages of 32 positions 4 x 3 41.
 template <int D, bool kCoded, int kHalves>
 struct Ring {
     static constexpr int kRowBytes = kCoded ? D : 2 * D;
     static constexpr int kChunks = kRowBytes / 16;
-    static constexpr int kSub = kHalves == 1 || (kRowBytes >= 256 && !kCoded) ? 16 : 32;
+    static constexpr int kSub = 16;
     static constexpr int kTile = kSub * kWarps;                                // positions per scheduling tile
     static constexpr int kRows = kSub * kRowBytes;
     static constexpr int kStage = (2 * kRows + (kCoded ? 2 * kSub * 4 : 0) + kRowBytes - 1) / kRowBytes * kRowBytes;
-    static constexpr int kStages = kCoded && D >= 128 && kHalves == 1 ? 2 : kRowBytes >= 128 ? 3 : 4;
+    static constexpr int kStages = kCoded && D >= 128 ? 2 : kRowBytes >= 128 ? 3 : 4;
     static constexpr int kRing = kStages * kStage;
     static constexpr int kBytes = kWarps * kRing + kRowBytes;                  // the rings begin at a multiple of a row
-    static constexpr int kBlocksPerSm = kBytes > 112 * 1024 ? 1 : kBytes > 74 * 1024 || D == 256 ? 2 : kBytes > 55 * 1024 ? 3 : 4;
-    static_assert(8 * kHalves * D * 4 <= kStage, "a warp's output rows fit one stage of its ring");
+    static constexpr int kFit = kBytes > 112 * 1024 ? 1 : kBytes > 74 * 1024 || D == 256 ? 2 : kBytes > 55 * 1024 ? 3 : 4;
+    static constexpr int kWide = D == 64 ? 4 : 3;                              // of 16 heads: twice the accumulators
+    static constexpr int kBlocksPerSm = kHalves == 2 && kFit > kWide ? kWide : kFit;
+    // A warp's output rows, when a pair ends, go to a free stage while the next pair is requested; where they need more than
+    // a stage they take the ring and the next pair waits.
+    static constexpr int kOut = 8 * kHalves * D * 4;
+    static constexpr bool kWaits = kOut > kStage;
+    static_assert(kOut <= kRing, "a warp's output rows fit its ring");
     static_assert(kStage % kRowBytes == 0, "stages begin at a multiple of a row: chunk addresses are xored into them");
     static constexpr int kSwizzle = kRowBytes >= 128 ? 7 : 0;                  // bits of a row that move its chunks (64 bytes: see place)
+    static constexpr int kLastOut = kWaits ? 0 : kRing - kStage;               // where the rows go when nothing follows
 };
 
 // One worker's part of one pair.
@@ -746,9 +752,9 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
         const bool first = first_segment;
         __syncwarp();                           // every lane has read the last stage
         more = next();
-        // the one slot that start() leaves alone; where nothing follows, any but the first will do
-        const uint32_t free_slot = more ? prev : R::kRing - R::kStage;
-        if (more) start(seg);
+        // the one slot that start() leaves alone
+        const uint32_t free_slot = more && !R::kWaits ? prev : R::kLastOut;
+        if (more && !R::kWaits) start(seg);
 
         // ---- the four warps' parts become one: each leaves its rows in a slot of its ring.  Column c of row r lies at
         // c ^ 8 (r / 2 % 4): the lanes of a store fall on different banks
@@ -807,8 +813,8 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
                 acc.z = __fmaf_rn(f, v.z, acc.z);
                 acc.w = __fmaf_rn(f, v.w, acc.w);
             }
-            if (p.cluster > 1) {                // warp 0's first slot: nothing follows in its ring
-                *reinterpret_cast<float4*>(smem + (row * D + c) * 4) = acc;
+            if (p.cluster > 1) {                // over warp 0's rows: nobody else reads this place
+                *reinterpret_cast<float4*>(reinterpret_cast<float*>(smem + R::kLastOut) + at(row, c)) = acc;
                 if (c == 0) jpart[row] = make_float2(top, sum);
             } else if (whole) {
                 const float inv = __fdiv_rn(1.f, sum);
@@ -830,7 +836,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
                 const int row = i / (D / 4), c = 4 * (i - row * (D / 4));
                 float top = -INFINITY, sum = 0.f;
                 float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                const uint32_t from_o = smem_u32(smem) + (row * D + c) * 4, from_ml = smem_u32(&jpart[row]);
+                const uint32_t from_o = smem_u32(smem) + R::kLastOut + at(row, c) * 4, from_ml = smem_u32(&jpart[row]);
                 for (int k = 0; k < p.cluster; ++k) top = fmaxf(top, ld_cluster2(cluster_map(from_ml, k)).x);
                 const float safe = top == -INFINITY ? 0.f : top;
                 for (int k = 0; k < p.cluster; ++k) {
@@ -851,7 +857,10 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
             cluster_arrive();
             cluster_wait();
         }
-        if (more) __syncthreads();              // the slots belong to the rings again
+        if (more) {
+            __syncthreads();                    // the slots belong to the rings again
+            if (R::kWaits) start(seg);
+        }
     }
 }
 
@@ -967,9 +976,10 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
     out->cluster = pairs * cluster <= full && (tiles + cluster - 1) / cluster <= (pairs < 32 ? 12 : 16) ? cluster : 0;
     // With many more pairs than blocks fit, blocks of their own in several rounds are balanced by their number and end a
     // pair without holding the next one up: 128 sequences of 1000 positions in int8 51.7 us and 66.4 cut, 128 of 2048 93.6
-    // and 109.1 (fp16 85.0 and 87.3, 161.3 and 167.1).  From some forty tiles on the last round's tail costs more (64
-    // sequences of 1 to 4000, fp16: 91.6 and 87.6), and just over one round (320 pairs for 296 blocks) does too.
-    if (cluster == 1 && 2 * pairs >= 3 * (long long)full && tiles <= 40) out->cluster = 1;
+    // and 109.1 (fp16 85.0 and 87.3, 161.3 and 167.1), with 16 heads a kv head 64 of 1 to 1000 (512 pairs for 444 blocks)
+    // 29.6 and 37.2.  From some forty tiles on the last round's tail costs more (64 sequences of 1 to 4000, fp16: 91.6 and
+    // 87.6), and just over one round (320 pairs for 296 blocks of 16 tiles: 37.3 and 35.4) does too.
+    if (cluster == 1 && 20 * pairs >= (tiles <= 16 ? 23 : 30) * (long long)full && tiles <= 40) out->cluster = 1;
     // The even cut: a lane per pair of a sequence where that leaves at most 3% of the blocks out, else one lane.
     const long long deep = (long long)kv.heads * out->blocks_per_kv;
     out->lanes = deep <= full && full / deep * deep * 100 >= 97LL * full ? (int)deep : 1;
