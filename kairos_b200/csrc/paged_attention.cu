@@ -6,14 +6,14 @@
 //
 // Bound.  Every cached byte is read once and meets 2 * group flops (group = query heads per kv head): below 16 flops
 // a byte, so HBM sets the pace and everything here serves to keep loads in flight:
-//   * a warp owns a ring of stages of 16 or 32 positions (8 KB of K and V rows of 128 fp16 channels), filled by 16-byte
+//   * a warp owns a ring of stages of 16 positions (8 KB of K and V rows of 128 fp16 channels), filled by 16-byte
 //     cp.async with a swizzle of its own; no block-wide barrier until a pair ends, and the next pair is requested first;
 //   * the heads that share a kv head are the eight columns of warp-level tensor instructions (m16n8k16): scores^T = K q^T
 //     (16 positions a step) and o^T = V^T w^T (16 channels), so a key is read from shared memory once for all of them and
 //     no row of a product is empty.  tcgen05 would take 128 positions by eight heads from shared or tensor memory, where
 //     codes would have to be written back once widened, and return them through tensor memory; the tensor pipe is 14%
 //     busy as it is (25% for codes), so there is nothing to gain from it;
-//   * the work goes to blocks by one of three rules (make_plan): a block or a cluster of blocks per pair, many rounds of
+//   * the work goes to blocks by one of three rules (make_plan): a block or a cluster of blocks per pair, many waves of
 //     such blocks, or an even cut on the device, whatever the lengths are.  A pair that lies across blocks of the cut
 //     leaves one partial result per block in the workspace and a second kernel joins them in the order of the blocks (no
 //     atomics: same bits every run).
@@ -35,6 +35,8 @@ namespace kairos {
 int* device_status_word();   // api.cu
 
 constexpr int kWarps = 4;
+constexpr int kSub = 16;                    // positions of a stage
+constexpr int kTile = kSub * kWarps;        // positions per scheduling tile
 // Weights are kept times 2^kLift and pass the reference by 2^kSlack at the most; with a V scale of up to twice the largest
 // so far they stay below 2^15, and fp16's smallest step is 2^-30 of a weight at the reference.
 constexpr float kLift = 6.f, kSlack = 8.f;
@@ -62,7 +64,6 @@ struct Cut {
 // The work of a pair in units: a tile of positions each, and kEnding more for ending it (joining the warps, starting the
 // next pair); none for an empty sequence.
 constexpr int kEnding = 2;                  // 1: 256 sequences of 1 to 500 positions 64.0 us for 56.4, 64 of 1 to 4000 93.9 for 88.0; 3: no gain
-template <int kTile>
 __device__ __forceinline__ unsigned units_of(int len) { return len > 0 ? (unsigned)(len + kTile - 1) / kTile + kEnding : 0; }
 
 // Units that a block may take over what an even cut gives it before cutting pays: a join costs about as long as a block
@@ -74,7 +75,6 @@ constexpr unsigned kSpare = 6;
 // to end, sequence after sequence, and its workers take equal runs.  With a lane per pair of a sequence, neighbouring
 // workers read the same pages' heads at the same time.  If every pair is short -- no more than kSpare units over the even
 // run -- and there are no more pairs than workers, a worker takes one whole pair (run = 0).
-template <int kTile>
 __device__ __forceinline__ bool locate(const int* lens, const AttnShape& p, int pairs, int most, Cut* out) {
     __shared__ unsigned warp_sum[kWarps], warp_top[kWarps];
     __shared__ Cut found;
@@ -84,7 +84,7 @@ __device__ __forceinline__ bool locate(const int* lens, const AttnShape& p, int 
     int own_len = 0;                        // the only length of this thread where there are no more sequences than threads
     for (int b = first; b < last; ++b) {
         own_len = seq_len(lens, b, most);
-        const unsigned n = units_of<kTile>(own_len);
+        const unsigned n = units_of(own_len);
         mine += n;
         top = max(top, n);
     }
@@ -121,7 +121,7 @@ __device__ __forceinline__ bool locate(const int* lens, const AttnShape& p, int 
     if (x >= before * deep && x < upto * deep) {
         for (int b = first; b < last; ++b) {
             const int len = per == 1 ? own_len : seq_len(lens, b, most);
-            const unsigned n = units_of<kTile>(len);
+            const unsigned n = units_of(len);
             if (x < (before + n) * deep) {
                 const unsigned rest = x - before * deep;
                 found = Cut{total, run, b, (int)(rest / n) * p.lanes + lane, (int)(rest % n), len};
@@ -277,8 +277,6 @@ template <int D, bool kCoded, int kHalves>
 struct Ring {
     static constexpr int kRowBytes = kCoded ? D : 2 * D;
     static constexpr int kChunks = kRowBytes / 16;
-    static constexpr int kSub = 16;
-    static constexpr int kTile = kSub * kWarps;                                // positions per scheduling tile
     static constexpr int kRows = kSub * kRowBytes;
     static constexpr int kStage = (2 * kRows + (kCoded ? 2 * kSub * 4 : 0) + kRowBytes - 1) / kRowBytes * kRowBytes;
     static constexpr int kStages = kCoded && D >= 128 ? 2 : kRowBytes >= 128 ? 3 : 4;
@@ -314,7 +312,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
     constexpr int kHalves = (kBlockHeads + 7) / 8;
     using MT = typename std::conditional<kCoded, __half, QT>::type;
     using R = Ring<D, kCoded, kHalves>;
-    constexpr int kHeads = 8 * kHalves, kSteps = R::kSub / 16, kTile = R::kTile;
+    constexpr int kHeads = 8 * kHalves;
     extern __shared__ __align__(128) uint8_t dynamic[];
     uint8_t* const smem = dynamic + ((0u - smem_u32(dynamic)) & (R::kRowBytes - 1));
     __shared__ float jm[kWarps][kHeads], jl[kWarps][kHeads];
@@ -329,7 +327,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
     Segment seg = {};
     bool more = false;
     const int stride = p.cluster ? p.cluster * kTile : kTile;      // from one of this block's tiles to the next
-    int first_pages[R::kStages - 1][kSteps];
+    int first_pages[R::kStages - 1];
     if (p.cluster) {                            // a pair per cluster, its tiles dealt to the cluster's blocks in turn
         const int place = blockIdx.x / p.cluster, rank = blockIdx.x - place * p.cluster;
         seg.b = place / pairs;
@@ -337,17 +335,15 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
         seg.tile = rank;
         // the first tiles' places do not depend on the length, so their pages are looked up together with it
 #pragma unroll
-        for (int i = 0; i < R::kStages - 1; ++i)
-#pragma unroll
-            for (int h = 0; h < kSteps; ++h) {
-                const int key = rank * kTile + warp * R::kSub + i * stride + 16 * h;
-                first_pages[i][h] = key < most ? __ldcg(table + (size_t)seg.b * p.table_stride + (key >> kv.page_shift)) : 0;
-            }
+        for (int i = 0; i < R::kStages - 1; ++i) {
+            const int key = rank * kTile + warp * kSub + i * stride;
+            first_pages[i] = key < most ? __ldcg(table + (size_t)seg.b * p.table_stride + (key >> kv.page_shift)) : 0;
+        }
         seg.len = seq_len(lens, seg.b, most);
         seg.tiles = seg.take = (seg.len + kTile - 1) / kTile;
         more = seg.len > 0;                     // the same for the whole cluster; a block without tiles joins with nothing
-    } else if (locate<kTile>(lens, p, pairs, most, &cut)) {
-        left = cut.run ? min(cut.run, cut.total - blockIdx.x / p.lanes * cut.run) : units_of<kTile>(cut.len);
+    } else if (locate(lens, p, pairs, most, &cut)) {
+        left = cut.run ? min(cut.run, cut.total - blockIdx.x / p.lanes * cut.run) : units_of(cut.len);
         seg = {cut.b, cut.pair, cut.unit, 0, 0, cut.len};
     }
     bool first_segment = true;
@@ -384,8 +380,8 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
     const uint32_t ring_u = smem_u32(ring);
     const int page_mask = (1 << kv.page_shift) - 1;
     int cur = 0, prev = R::kRing - R::kStage;   // byte offsets in the ring: the next stage to read, and the one before it
-    unsigned bad = 0;                           // per 16 positions of a slot: page outside the pool
-    int k0, k1, head;                           // this warp's positions: k0 .. k0 + kSub - 1, then `stride` further, below k1
+    unsigned bad = 0;                           // one bit per slot: its page lies outside the pool
+    int k0, k1, head;                           // this warp's positions: k0 .. k0 + 15, then `stride` further, below k1
     // Where this lane reads and writes in a stage; a chunk or row further is an xor of chunk bits or a constant.
     const uint32_t k_lane = place<R::kRowBytes>(lane & 15, lane >> 4);
     const uint32_t v_lane = R::kRows + (kCoded ? place<R::kRowBytes>(2 * t, g * (D / 8) >> 4) + (g * (D / 8) & 15)
@@ -398,54 +394,43 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
     const float* seg_scale = nullptr;
     const unsigned page_rows = (unsigned)kv.heads << kv.page_shift;
     const size_t page_bytes = (size_t)page_rows * R::kRowBytes;
-    int ahead[kSteps];                          // pages of the next stage to request
+    int ahead = 0;                              // page of the next stage to request
     uint32_t qb[D / 16][2 * kHalves];
     float unit[kHalves][2];                     // score = product * unit (* scale of the key), heads 2 t and 2 t + 1 (+ 8)
 
-    auto look = [&](int key0, int (&to)[kSteps]) {
-#pragma unroll
-        for (int h = 0; h < kSteps; ++h) {
-            const int key = key0 + 16 * h;
-            if (h == 0 || kv.page_shift < 5) to[h] = key < k1 ? __ldcg(pages + (key >> kv.page_shift)) : 0;
-            else to[h] = to[0];
-        }
-    };
-    auto request = [&](int key0, int slot, const int (&from)[kSteps]) {    // positions from key0 on, in pages `from`, into a slot
-        if (key0 < k1) {
+    auto look = [&](int key) { return key < k1 ? __ldcg(pages + (key >> kv.page_shift)) : 0; };
+    auto request = [&](int key, int slot, int from) {      // the 16 positions from `key` on, which lie in page `from`, into a slot
+        if (key < k1) {
+            const int real = k1 - key;
             const uint32_t dst = ring_u + slot;
+            const bool ok = (unsigned)from < (unsigned)kv.pages;
+            if (!ok) {
+                bad |= 1u << (slot / R::kStage);
+                *status = KAIROS_ERR_ARG;
+            }
+            const unsigned page = ok ? (unsigned)from : 0u, in_page = (unsigned)(key & page_mask);
+            const size_t off = (size_t)page * page_bytes + in_page * R::kRowBytes;
+            const uint8_t* ks = seg_k + off;
+            const uint8_t* vs = seg_v + off;
+            if (ok && real >= kSub) {
 #pragma unroll
-            for (int h = 0; h < kSteps; ++h) {
-                const int key = key0 + 16 * h, real = k1 - key;
-                const bool ok = (unsigned)from[h] < (unsigned)kv.pages;
-                if (!ok && real > 0) {
-                    bad |= 1u << (slot / R::kStage * kSteps + h);
-                    *status = KAIROS_ERR_ARG;
+                for (int n = 0; n < R::kChunks / 2; ++n) {
+                    const uint32_t to = ((dst + cp_lane) ^ ((n * kCpRows & R::kSwizzle) << 4)) + n * kCpRows * R::kRowBytes;
+                    cp16(to, ks + 512 * n);
+                    cp16(to + R::kRows, vs + 512 * n);
                 }
-                const unsigned page = ok ? (unsigned)from[h] : 0u, in_page = (unsigned)(key & page_mask);
-                const size_t off = (size_t)page * page_bytes + in_page * R::kRowBytes;
-                const uint8_t* ks = seg_k + off;
-                const uint8_t* vs = seg_v + off;
-                if (ok && real >= 16) {
+            } else {                            // rows behind the end, or of no page, are zeros: 0 * weight stays 0
 #pragma unroll
-                    for (int n = 0; n < R::kChunks / 2; ++n) {
-                        const uint32_t to = ((dst + cp_lane) ^ ((n * kCpRows & R::kSwizzle) << 4)) + (16 * h + n * kCpRows) * R::kRowBytes;
-                        cp16(to, ks + 512 * n);
-                        cp16(to + R::kRows, vs + 512 * n);
-                    }
-                } else {                        // rows behind the end, or of no page, are zeros: 0 * weight stays 0
-#pragma unroll
-                    for (int n = 0; n < R::kChunks / 2; ++n) {
-                        const uint32_t to = ((dst + cp_lane) ^ ((n * kCpRows & R::kSwizzle) << 4)) + (16 * h + n * kCpRows) * R::kRowBytes;
-                        const bool there = ok && n * kCpRows + lane / R::kChunks < real;
-                        cp16(to, ks + 512 * n, there);
-                        cp16(to + R::kRows, vs + 512 * n, there);
-                    }
+                for (int n = 0; n < R::kChunks / 2; ++n) {
+                    const uint32_t to = ((dst + cp_lane) ^ ((n * kCpRows & R::kSwizzle) << 4)) + n * kCpRows * R::kRowBytes;
+                    const bool there = ok && n * kCpRows + lane / R::kChunks < real;
+                    cp16(to, ks + 512 * n, there);
+                    cp16(to + R::kRows, vs + 512 * n, there);
                 }
-                if constexpr (kCoded) {         // lanes 0..3: scales of K, 4..7: of V
-                    if (lane < 8)
-                        cp16(dst + 2 * R::kRows + (lane >> 2) * (R::kSub * 4) + h * 64 + (lane & 3) * 16,
-                             seg_scale + ((size_t)page * page_rows + in_page), ok && real > 0);
-                }
+            }
+            if constexpr (kCoded) {             // lanes 0..3: scales of K, 4..7: of V
+                if (lane < 8)
+                    cp16(dst + 2 * R::kRows + (lane >> 2) * (kSub * 4) + (lane & 3) * 16, seg_scale + ((size_t)page * page_rows + in_page), ok);
             }
         }
         cp_commit();
@@ -455,7 +440,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
         head = sg.pair / p.blocks_per_kv;
         const int block = sg.pair - head * p.blocks_per_kv;
         const int rows = min(kHeads, p.group - block * kHeads);            // of 4 heads a block: the whole group
-        k0 = sg.tile * kTile + warp * R::kSub;
+        k0 = sg.tile * kTile + warp * kSub;
         k1 = p.cluster ? sg.len : min((sg.tile + sg.take) * kTile, sg.len);
         pages = table + (size_t)sg.b * p.table_stride;
         const unsigned head_row = (unsigned)head << kv.page_shift;
@@ -463,11 +448,11 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
         seg_v = static_cast<const uint8_t*>(kv.v) + (size_t)head_row * R::kRowBytes + lane * 16;
         if constexpr (kCoded) seg_scale = (lane < 4 ? kv.ks : kv.vs) + head_row + (lane & 3) * 4;
         int slot = cur;
-        if (!p.cluster) look(k0, first_pages[0]);
+        if (!p.cluster) first_pages[0] = look(k0);
 #pragma unroll
         for (int i = 0; i < R::kStages - 1; ++i) {
-            if (i + 1 == R::kStages - 1) look(k0 + (i + 1) * stride, ahead);
-            else if (!p.cluster) look(k0 + (i + 1) * stride, first_pages[i + 1]);
+            if (i + 1 == R::kStages - 1) ahead = look(k0 + (i + 1) * stride);
+            else if (!p.cluster) first_pages[i + 1] = look(k0 + (i + 1) * stride);
             request(k0 + i * stride, slot, first_pages[i]);
             slot = slot == R::kRing - R::kStage ? 0 : slot + R::kStage;
         }
@@ -552,107 +537,79 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
             cp_wait<R::kStages - 2>();
             __syncwarp();                       // every lane's copies have landed; the stage before has been read
             request(pos + (R::kStages - 1) * stride, prev, ahead);
-            look(pos + R::kStages * stride, ahead);
+            ahead = look(pos + R::kStages * stride);
             const uint32_t ku = ring_u + cur + k_lane, vu = ring_u + cur + v_lane;
-            const uint8_t* stage = ring + cur;
+            const float* scales = reinterpret_cast<const float*>(ring + cur + 2 * R::kRows);
             const int real = k1 - pos;
-            const bool full = real >= R::kSub && bad == 0;      // the same in all lanes
-            unsigned gone = 0;
+            const bool full = real >= kSub && bad == 0;         // the same in all lanes
+            bool gone = false;                                  // the page lies outside the pool
             if (!full) {
-                const int shift = cur / R::kStage * kSteps;
-                gone = (bad >> shift) & ((1u << kSteps) - 1);
-                bad &= ~(gone << shift);
+                const int slot = cur / R::kStage;
+                gone = (bad >> slot) & 1u;
+                bad &= ~(1u << slot);
             }
             prev = cur;
             cur = cur == R::kRing - R::kStage ? 0 : cur + R::kStage;
 
-            // scores^T of step h: positions g and g + 8, heads 2 t and 2 t + 1: [0], [1] and [2], [3]
-            float s[kSteps][kHalves][4] = {};
+            // scores^T: positions g and g + 8, heads 2 t and 2 t + 1: [0], [1] and [2], [3]
+            float s[kHalves][4] = {};
 #pragma unroll
-            for (int c = 0; c < D / 16; c += kCoded ? 2 : 1)
+            for (int c = 0; c < D / 16; c += kCoded ? 2 : 1) {
+                uint32_t w[4];                  // uncoded: one step of 16 channels; coded: two
+                ldsm4(ku ^ ((kCoded ? c : 2 * c) << 4), w);
+                if constexpr (!kCoded) {
 #pragma unroll
-                for (int h = 0; h < kSteps; ++h) {
-                    uint32_t w[4];              // uncoded: one step of channels; coded: two
-                    ldsm4((ku ^ ((kCoded ? c : 2 * c) << 4)) + 16 * h * R::kRowBytes, w);
-                    if constexpr (!kCoded) {
+                    for (int r = 0; r < kHalves; ++r) mma(MT(), s[r], w[0], w[1], w[2], w[3], qb[c][2 * r], qb[c][2 * r + 1]);
+                } else {
+#pragma unroll
+                    for (int d = 0; d < 2; ++d) {
+                        uint32_t a[4];
+                        Widen::run(w[2 * d], &a[0], &a[2]);
+                        Widen::run(w[2 * d + 1], &a[1], &a[3]);
 #pragma unroll
                         for (int r = 0; r < kHalves; ++r)
-                            mma(MT(), s[h][r], w[0], w[1], w[2], w[3], qb[c][2 * r], qb[c][2 * r + 1]);
-                    } else {
-#pragma unroll
-                        for (int d = 0; d < 2; ++d) {
-                            uint32_t a[4];
-                            Widen::run(w[2 * d], &a[0], &a[2]);
-                            Widen::run(w[2 * d + 1], &a[1], &a[3]);
-#pragma unroll
-                            for (int r = 0; r < kHalves; ++r)
-                                mma(MT(), s[h][r], a[0], a[1], a[2], a[3], qb[c + d][2 * r], qb[c + d][2 * r + 1]);
-                        }
+                            mma(MT(), s[r], a[0], a[1], a[2], a[3], qb[c + d][2 * r], qb[c + d][2 * r + 1]);
                     }
                 }
-            // positions g, g + 8 of each step: the scale of V, and which of them are no positions at all
-            float vs[kSteps][2];
-            unsigned dead = 0;
+            }
+            // positions g, g + 8: the scale of V, and which of them are no positions at all
+            float vs[2];
+            bool dead[2] = {false, false};
             if (!full) {
 #pragma unroll
-                for (int h = 0; h < kSteps; ++h)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                        if (16 * h + 8 * k + g >= real || ((gone >> h) & 1u)) dead |= 1u << (2 * h + k);
+                for (int k = 0; k < 2; ++k) dead[k] = 8 * k + g >= real || gone;
             }
             bool move = false;
             if constexpr (kCoded) {
-                const float* sc = reinterpret_cast<const float*>(stage + 2 * R::kRows);
 #pragma unroll
-                for (int h = 0; h < kSteps; ++h)
+                for (int k = 0; k < 2; ++k) {
+                    const float ks = scales[8 * k + g];
+                    vs[k] = scales[kSub + 8 * k + g];
+                    if (dead[k]) vs[k] = 0.f;   // scales behind the end may be anything, NaN too
+                    move |= fabsf(vs[k]) > 2.f * vtop;
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const float ks = sc[16 * h + 8 * k + g];
-                        vs[h][k] = sc[R::kSub + 16 * h + 8 * k + g];
-#pragma unroll
-                        for (int r = 0; r < kHalves; ++r) s[h][r][2 * k] *= ks, s[h][r][2 * k + 1] *= ks;
-                    }
-                if (!full) {                    // scales behind the end may be anything, NaN too
-#pragma unroll
-                    for (int h = 0; h < kSteps; ++h)
-#pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            if ((dead >> (2 * h + k)) & 1u) vs[h][k] = 0.f;
+                    for (int r = 0; r < kHalves; ++r) s[r][2 * k] *= ks, s[r][2 * k + 1] *= ks;
                 }
-#pragma unroll
-                for (int h = 0; h < kSteps; ++h) move |= fabsf(vs[h][0]) > 2.f * vtop || fabsf(vs[h][1]) > 2.f * vtop;
             }
-            float x[kSteps][kHalves][4];        // exponents
+            float x[kHalves][4];                // exponents
             auto exponents = [&]() {
 #pragma unroll
-                for (int h = 0; h < kSteps; ++h)
+                for (int r = 0; r < kHalves; ++r)
 #pragma unroll
-                    for (int r = 0; r < kHalves; ++r)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x[h][r][e] = __fmaf_rn(s[h][r][e], unit[r][e & 1], -base[r][e & 1]);
-                if (!full) {
-#pragma unroll
-                    for (int h = 0; h < kSteps; ++h)
-#pragma unroll
-                        for (int r = 0; r < kHalves; ++r)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if ((dead >> (2 * h + (e >> 1))) & 1u) x[h][r][e] = -INFINITY;
-                }
+                    for (int e = 0; e < 4; ++e) {
+                        x[r][e] = __fmaf_rn(s[r][e], unit[r][e & 1], -base[r][e & 1]);
+                        if (dead[e >> 1]) x[r][e] = -INFINITY;
+                    }
             };
             exponents();
 #pragma unroll
             for (int r = 0; r < kHalves; ++r)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int h = 0; h < kSteps; ++h) move |= x[h][r][e] > kLift + kSlack;
+                for (int e = 0; e < 4; ++e) move |= x[r][e] > kLift + kSlack;
             if (__any_sync(0xffffffffu, move)) {
                 float grow = 1.f;
                 if constexpr (kCoded) {
-                    float top = 0.f;
-#pragma unroll
-                    for (int h = 0; h < kSteps; ++h) top = fmaxf(top, fmaxf(fabsf(vs[h][0]), fabsf(vs[h][1])));
+                    float top = fmaxf(fabsf(vs[0]), fabsf(vs[1]));
 #pragma unroll
                     for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
                     if (top > vtop) {
@@ -665,12 +622,8 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
                 for (int r = 0; r < kHalves; ++r)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float top = -INFINITY;
-#pragma unroll
-                        for (int h = 0; h < kSteps; ++h)
-#pragma unroll
-                            for (int k = 0; k < 4; k += 2)
-                                if (!((dead >> (2 * h + (k >> 1))) & 1u)) top = fmaxf(top, s[h][r][e + k] * unit[r][e]);
+                        float top = dead[0] ? -INFINITY : s[r][e] * unit[r][e];
+                        if (!dead[1]) top = fmaxf(top, s[r][e + 2] * unit[r][e]);
 #pragma unroll
                         for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
                         top = fmaxf(m[r][e], top);
@@ -685,64 +638,59 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
                 exponents();
             }
             // weights as the second operand of o^T += V^T w^T: positions 2 t, 2 t + 1 (and 8 further) of head g
-            uint32_t wb[kSteps][kHalves][2], rest[kSteps][kHalves][2];
+            uint32_t wb[kHalves][2], rest[kHalves][2];
 #pragma unroll
-            for (int h = 0; h < kSteps; ++h)
+            for (int r = 0; r < kHalves; ++r)
 #pragma unroll
-                for (int r = 0; r < kHalves; ++r)
+                for (int k = 0; k < 2; ++k) {
+                    float w0 = exp2_fast(x[r][2 * k]), w1 = exp2_fast(x[r][2 * k + 1]);
+                    l[r][0] += w0;
+                    l[r][1] += w1;
+                    if constexpr (kCoded) {
+                        const float f = vs[k] * vinv;
+                        w0 *= f, w1 *= f;
+                    }
+                    uint32_t hi, lo;
+                    split(MT(), w0, w1, &hi, &lo);
+                    if constexpr (kTwin) {
+                        wb[r][k] = transpose8(t < 2 ? hi : lo);
+                    } else {
+                        wb[r][k] = transpose8(hi);
+                        rest[r][k] = transpose8(lo);
+                    }
+                }
+            auto weigh = [&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        float w0 = exp2_fast(x[h][r][2 * k]), w1 = exp2_fast(x[h][r][2 * k + 1]);
-                        l[r][0] += w0;
-                        l[r][1] += w1;
-                        if constexpr (kCoded) {
-                            const float f = vs[h][k] * vinv;
-                            w0 *= f, w1 *= f;
+                for (int r = 0; r < kHalves; ++r) {
+                    mma(MT(), o[j][r], a0, a1, a2, a3, wb[r][0], wb[r][1]);
+                    if constexpr (!kTwin) mma(MT(), o[j][r], a0, a1, a2, a3, rest[r][0], rest[r][1]);
+                }
+            };
+            if constexpr (!kCoded) {
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) {
+                    uint32_t w[4];
+                    ldsm4t(vu ^ (2 * j << 4), w);
+                    weigh(j, w[0], w[1], w[2], w[3]);
+                }
+            } else {
+                // a thread's bytes of a row are the D / 8 channels from g * D / 8 on
+                constexpr int kWords = D / 32 < 4 ? D / 32 : 4;        // words per access: 2 (8 bytes) or 4 (16 bytes)
+#pragma unroll
+                for (int c = 0; c < D / 8 / (4 * kWords); ++c) {
+                    uint32_t v[4][kWords];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)            // positions 2 t, 2 t + 1, and 8 further
+                        lds(v[k], (vu ^ ((c ^ (k & 1 & R::kSwizzle)) << 4)) + ((k & 1) + 8 * (k >> 1)) * R::kRowBytes);
+#pragma unroll
+                    for (int w = 0; w < kWords; ++w)
+#pragma unroll
+                        for (int d = 0; d < 2; ++d) {
+                            uint32_t a0, a1, a2, a3;
+                            Widen::run(__byte_perm(v[0][w], v[1][w], d ? 0x7362 : 0x5140), &a0, &a1);
+                            Widen::run(__byte_perm(v[2][w], v[3][w], d ? 0x7362 : 0x5140), &a2, &a3);
+                            weigh((c * kWords + w) * 2 + d, a0, a1, a2, a3);
                         }
-                        uint32_t hi, lo;
-                        split(MT(), w0, w1, &hi, &lo);
-                        if constexpr (kTwin) {
-                            wb[h][r][k] = transpose8(t < 2 ? hi : lo);
-                        } else {
-                            wb[h][r][k] = transpose8(hi);
-                            rest[h][r][k] = transpose8(lo);
-                        }
-                    }
-#pragma unroll
-            for (int h = 0; h < kSteps; ++h) {
-                auto weigh = [&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-#pragma unroll
-                    for (int r = 0; r < kHalves; ++r) {
-                        mma(MT(), o[j][r], a0, a1, a2, a3, wb[h][r][0], wb[h][r][1]);
-                        if constexpr (!kTwin) mma(MT(), o[j][r], a0, a1, a2, a3, rest[h][r][0], rest[h][r][1]);
-                    }
-                };
-                if constexpr (!kCoded) {
-#pragma unroll
-                    for (int j = 0; j < D / 16; ++j) {
-                        uint32_t w[4];
-                        ldsm4t((vu ^ (2 * j << 4)) + 16 * h * R::kRowBytes, w);
-                        weigh(j, w[0], w[1], w[2], w[3]);
-                    }
-                } else {
-                    // a thread's bytes of a row are the D / 8 channels from g * D / 8 on
-                    constexpr int kWords = D / 32 < 4 ? D / 32 : 4;    // words per access: 2 (8 bytes) or 4 (16 bytes)
-#pragma unroll
-                    for (int c = 0; c < D / 8 / (4 * kWords); ++c) {
-                        uint32_t v[4][kWords];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)        // positions 2 t, 2 t + 1, and 8 further
-                            lds(v[k], (vu ^ ((c ^ (k & 1 & R::kSwizzle)) << 4)) + (16 * h + (k & 1) + 8 * (k >> 1)) * R::kRowBytes);
-#pragma unroll
-                        for (int w = 0; w < kWords; ++w)
-#pragma unroll
-                            for (int d = 0; d < 2; ++d) {
-                                uint32_t a0, a1, a2, a3;
-                                Widen::run(__byte_perm(v[0][w], v[1][w], d ? 0x7362 : 0x5140), &a0, &a1);
-                                Widen::run(__byte_perm(v[2][w], v[3][w], d ? 0x7362 : 0x5140), &a2, &a3);
-                                weigh((c * kWords + w) * 2 + d, a0, a1, a2, a3);
-                            }
-                    }
                 }
             }
         }
@@ -949,17 +897,12 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
     out->heads_per_block = group > 8 ? 16 : group > 4 ? 8 : 4;
     out->blocks_per_kv = (group + out->heads_per_block - 1) / out->heads_per_block;
     const bool wide = out->heads_per_block == 16;
-    int tile = 0, per_sm = 0;
-#define KAIROS_RING(D)                                                                          \
-    (wide ? (tile = coded ? Ring<D, true, 2>::kTile : Ring<D, false, 2>::kTile,                 \
-             per_sm = coded ? Ring<D, true, 2>::kBlocksPerSm : Ring<D, false, 2>::kBlocksPerSm) \
-          : (tile = coded ? Ring<D, true, 1>::kTile : Ring<D, false, 1>::kTile,                 \
-             per_sm = coded ? Ring<D, true, 1>::kBlocksPerSm : Ring<D, false, 1>::kBlocksPerSm))
-    if (kv.dim == 64) KAIROS_RING(64);
-    else if (kv.dim == 128) KAIROS_RING(128);
-    else KAIROS_RING(256);
-#undef KAIROS_RING
-    const long long tiles = (((long long)table_width << kv.page_shift) + tile - 1) / tile;
+#define KAIROS_PER_SM(D)                                                                       \
+    (wide ? (coded ? Ring<D, true, 2>::kBlocksPerSm : Ring<D, false, 2>::kBlocksPerSm)         \
+          : (coded ? Ring<D, true, 1>::kBlocksPerSm : Ring<D, false, 1>::kBlocksPerSm))
+    const int per_sm = kv.dim == 64 ? KAIROS_PER_SM(64) : kv.dim == 128 ? KAIROS_PER_SM(128) : KAIROS_PER_SM(256);
+#undef KAIROS_PER_SM
+    const long long tiles = (((long long)table_width << kv.page_shift) + kTile - 1) / kTile;
     const long long pairs = (long long)B * kv.heads * out->blocks_per_kv;
     if ((tiles + kEnding) * pairs > 0x7fffffffLL) return KAIROS_ERR_SHAPE;
     const int full = sms * per_sm;
@@ -967,18 +910,17 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
     // meet in shared memory: one launch, no scan of the lengths, no workspace.  Otherwise the device cuts the work by the
     // lengths, which costs some 8 us more but keeps every block busy whatever they are.  Up to four tiles go to one block, more
     // are shared by two tiles a block: 256 positions take 5.1 us in one block and in four, 512 take 7.0 in one, 6.6 in two
-    // and 5.9 in four.  Sixteen at the most (twelve
-    // where pairs are few): in fp16, 32 sequences of 1024 positions take 24.0 us in blocks of their own and 27.9 cut (18.1
+    // and 5.9 in four.  Sixteen at the most (twelve where pairs are few): in fp16, 32 sequences of 1024 positions take 24.0 us in blocks of their own and 27.9 cut (18.1
     // and 22.7 with lengths from 32 to 1024), 16 of 2048 in clusters of two 25.0 and 29.9 (19.5 and 20.4), 16 of 4096
     // 44.0 and 49.4 (33.0 and 31.4), one of 8192 in clusters of eight 15.9 and 14.0.
     int cluster = 1;
     while (cluster < 8 && pairs * cluster * 2 <= full && tiles > 4 && tiles > 2 * cluster) cluster *= 2;
     out->cluster = pairs * cluster <= full && (tiles + cluster - 1) / cluster <= (pairs < 32 ? 12 : 16) ? cluster : 0;
-    // With many more pairs than blocks fit, blocks of their own in several rounds are balanced by their number and end a
+    // With many more pairs than blocks fit, blocks of their own in several waves are balanced by their number and end a
     // pair without holding the next one up: 128 sequences of 1000 positions in int8 51.7 us and 66.4 cut, 128 of 2048 93.6
     // and 109.1 (fp16 85.0 and 87.3, 161.3 and 167.1), with 16 heads a kv head 64 of 1 to 1000 (512 pairs for 444 blocks)
-    // 29.6 and 37.2.  From some forty tiles on the last round's tail costs more (64 sequences of 1 to 4000, fp16: 91.6 and
-    // 87.6), and just over one round (320 pairs for 296 blocks of 16 tiles: 37.3 and 35.4) does too.
+    // 29.6 and 37.2.  From some forty tiles on the last wave's tail costs more (64 sequences of 1 to 4000, fp16: 91.6 and
+    // 87.6), and just over one wave (320 pairs for 296 blocks of 16 tiles: 37.3 and 35.4) does too.
     if (cluster == 1 && 20 * pairs >= (tiles <= 16 ? 23 : 30) * (long long)full && tiles <= 40) out->cluster = 1;
     // The even cut: a lane per pair of a sequence where that leaves at most 3% of the blocks out, else one lane.
     const long long deep = (long long)kv.heads * out->blocks_per_kv;
