@@ -9,31 +9,7 @@
 
 namespace kairos {
 
-// Eight consecutive elements of a row as fp32, in one or two 16-byte accesses.
-__device__ __forceinline__ void load8(const __half* p, float (&f)[8]) {
-    const uint4 v = __ldcg(reinterpret_cast<const uint4*>(p));
-    const __half2* h = reinterpret_cast<const __half2*>(&v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 t = __half22float2(h[i]);
-        f[2 * i] = t.x;
-        f[2 * i + 1] = t.y;
-    }
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&f)[8]) {
-    const uint4 v = __ldcg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[2 * i] = __uint_as_float(w[i] << 16);
-        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-}
-__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
-    const float4 a = __ldcg(reinterpret_cast<const float4*>(p)), b = __ldcg(reinterpret_cast<const float4*>(p) + 1);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-}
+// Eight consecutive elements of a row from fp32, rounded once, in one or two 16-byte accesses.
 __device__ __forceinline__ void store8(__half* p, const float (&f)[8]) {
     uint4 v;
     __half2* h = reinterpret_cast<__half2*>(&v);
