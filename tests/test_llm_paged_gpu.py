@@ -21,7 +21,7 @@ def model():
     kb.DynamicLinear.context = runtime.Context('cuda', cache_bytes=None)
     m = llm.Decoder(cfg, 'cuda')
     prof = kb.Profiler(m.linear_shapes())
-    prof.load_table({s: [(4, 'w4a16_gemv'), (30720, 'w4a16_gemm')] for s in m.linear_shapes()})
+    prof.load_table({s: [(4, 'w4a16_gemv'), (30000, 'w4a16_gemm')] for s in m.linear_shapes()})
     kb.DynamicLinear.prof = prof
     yield m
     kb.DynamicLinear.context = None
