@@ -89,14 +89,16 @@ struct WriteShape {
 
 // Codes = void: the cache holds the activation's own type.  One block takes `tokens_per_block` tokens; the D / 16 cells of
 // a row go to neighbouring threads of one warp, so the row's maximum is a few shuffles.  A thread requests its first cells
-// before the block computes the tokens' angles, once for all heads, into shared memory.
+// before the block computes the tokens' angles, once for all heads, into shared memory beside their slots (each read where
+// its rows are stored: 2% slower).
 template <typename T, typename Codes, int D>
 __global__ void __launch_bounds__(256, 4) rope_paged_kv_kernel(const T* __restrict__ QKV, const long long* __restrict__ positions,
                                                             const long long* __restrict__ slots,
                                                             const unsigned long long* __restrict__ steps, const KvView kv,
                                                             T* __restrict__ Q, const WriteShape p, int* status) {
-    constexpr int kLanes = D / 16, kStep = 256 / kLanes, kU = kCells<T>;
+    constexpr int kLanes = D / 16, kU = kCells<T>;
     __shared__ __align__(16) float cs[kTablePairs], sn[kTablePairs];
+    __shared__ long long to_slot[kBlockTokens];
     chain_release();
     chain_wait();
     const int t0 = blockIdx.x * p.tokens_per_block;
@@ -110,18 +112,19 @@ __global__ void __launch_bounds__(256, 4) rope_paged_kv_kernel(const T* __restri
         *head = k - *t * per + (q ? 0 : p.H);
     };
     const long long capacity = (long long)kv.pages << kv.page_shift;
-    const int at = threadIdx.x / kLanes, j = threadIdx.x % kLanes;
+    const int at = threadIdx.x / kLanes, j = threadIdx.x % kLanes, step = blockDim.x / kLanes;
     const Cell cell = cell_of(j, p.rot, p.layout);
-    for (int base = 0; base < rows; base += kU * kStep) {
+    for (int base = 0; base < rows; base += kU * step) {
         RawCell<T> raw[kU];
+        int ts[kU], heads[kU];
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-            int t, head;
-            split(min(base + u * kStep + at, rows - 1), &t, &head);        // whole warps stay together
-            raw[u].load(QKV + (size_t)(t0 + t) * p.row_stride + head * D, cell);
+            split(min(base + u * step + at, rows - 1), &ts[u], &heads[u]);  // whole warps stay together
+            raw[u].load(QKV + (size_t)(t0 + ts[u]) * p.row_stride + heads[u] * D, cell);
         }
         if (base == 0) {
-            for (int i = threadIdx.x; i < here * pairs; i += 256) {
+            if (threadIdx.x < here) to_slot[threadIdx.x] = __ldcg(slots + t0 + threadIdx.x);
+            for (int i = threadIdx.x; i < here * pairs; i += blockDim.x) {
                 const int t = div_small(i, p.by_pairs), pair = i - t * pairs;
                 float c, s;
                 turn_of(__ldcg(positions + t0 + t), __ldg(steps + pair), p.magnitude, &c, &s);
@@ -132,10 +135,7 @@ __global__ void __launch_bounds__(256, 4) rope_paged_kv_kernel(const T* __restri
         }
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-            const int r = base + u * kStep + at;
-            const bool live = r < rows;
-            int t, head;
-            split(min(r, rows - 1), &t, &head);
+            const int t = ts[u], head = heads[u];
             float a[8], b[8];
             RawCell<T>::widen(raw[u].w[0], a);
             RawCell<T>::widen(raw[u].w[1], b);
@@ -144,14 +144,14 @@ __global__ void __launch_bounds__(256, 4) rope_paged_kv_kernel(const T* __restri
             if constexpr (!std::is_void<Codes>::value) {
                 if (__any_sync(0xffffffffu, head >= p.H)) amax = row_amax(a, b, kLanes);
             }
-            if (!live) continue;
+            if (base + u * step + at >= rows) continue;
             if (head < p.H) {
                 T* q = Q + ((size_t)(t0 + t) * p.H + head) * D;
                 store8(q + cell.first, a);
                 store8(q + cell.second, b);
                 continue;
             }
-            const long long slot = __ldcg(slots + t0 + t);
+            const long long slot = to_slot[t];
             if (slot < 0) continue;                        // padding
             if (slot >= capacity) {
                 *status = KAIROS_ERR_ARG;
@@ -243,12 +243,13 @@ __global__ void __launch_bounds__(256) paged_kv_read_kernel(const KvView kv, con
 template <typename T, typename Codes, int D>
 static int run_write(const void* QKV, const void* positions, const void* slots, const void* steps, const KvView& kv, void* Q,
                      WriteShape p, int* status, cudaStream_t st) {
-    p.tokens_per_block = rows_tokens(p.T, p.H + 2 * kv.heads, p.rot, kCells<T> * (256 / (D / 16)), 128);
+    const RowBlocks form = row_blocks(p.T, p.H + 2 * kv.heads, p.rot, 128 / (D / 16), kCells<T>, 64);
+    p.tokens_per_block = form.tokens;
     p.by_q = div_magic(p.H);
     p.by_kv = div_magic(2 * kv.heads);
     p.by_pairs = div_magic(max(1, p.rot / 2));
     const cudaError_t e = launch_chained(
-        rope_paged_kv_kernel<T, Codes, D>, dim3((unsigned)((p.T + p.tokens_per_block - 1) / p.tokens_per_block)), dim3(256), 0,
+        rope_paged_kv_kernel<T, Codes, D>, dim3((unsigned)((p.T + p.tokens_per_block - 1) / p.tokens_per_block)), dim3(form.threads), 0,
         st, static_cast<const T*>(QKV), static_cast<const long long*>(positions), static_cast<const long long*>(slots),
         static_cast<const unsigned long long*>(steps), kv, static_cast<T*>(Q), p, status);
     if (e != cudaSuccess) return note_cuda_error(e);

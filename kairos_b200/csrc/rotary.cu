@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(256, 4) rotary_kernel(const T* X, T* Y, const 
     const int here = (int)min((long long)p.tokens_per_block, p.tokens - t0);
     const int pairs = p.rot >> 1, lanes = p.D >> 4, rows = here * p.H;
     const int at = div_small((int)threadIdx.x, p.by_lanes), j = (int)threadIdx.x - at * lanes;
-    const int step = div_small(256, p.by_lanes);        // rows in one go; threads behind the last whole row idle
+    const int step = div_small(blockDim.x, p.by_lanes);        // rows in one go; threads behind the last whole row idle
     const bool idle = at >= step;
     const Cell cell = cell_of(j, p.rot, p.layout);
     auto place = [&](int r, long long sb, long long ss, long long sh) {
@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(256, 4) rotary_kernel(const T* X, T* Y, const 
             if (r < rows && !idle) raw[u].load(X + place(r, p.xb, p.xs, p.xh), cell);
         }
         if (base == 0) {
-            for (int i = threadIdx.x; i < here * pairs; i += 256) {
+            for (int i = threadIdx.x; i < here * pairs; i += blockDim.x) {
                 const int t = div_small(i, p.by_pairs), pair = i - t * pairs;
                 const long long token = t0 + t, b = p.S == p.tokens ? 0 : (unsigned)token / (unsigned)p.S;
                 float c, s;
@@ -115,12 +115,13 @@ static int run_rotary(const void* X, void* Y, const void* positions, const void*
     const unsigned long long* st64 = static_cast<const unsigned long long*>(steps);
     cudaError_t e;
     if (wide) {
-        p.tokens_per_block = rows_tokens(p.tokens, p.H, p.rot, kCells<T> * (256 / (p.D / 16)), sizeof(T) == 4 ? 64 : 128);
+        const RowBlocks form = row_blocks(p.tokens, p.H, p.rot, 128 / (p.D / 16), kCells<T>, sizeof(T) == 4 ? 32 : 64);
+        p.tokens_per_block = form.tokens;
         p.by_heads = div_magic(p.H);
         p.by_pairs = div_magic(max(1, p.rot / 2));
         p.by_lanes = div_magic(p.D / 16);
         const long long blocks = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
-        e = launch_chained(rotary_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, x, y, pos, st64, p);
+        e = launch_chained(rotary_kernel<T>, dim3((unsigned)blocks), dim3(form.threads), 0, st, x, y, pos, st64, p);
     } else {
         const long long total = p.tokens * p.H * ((p.D + 1) / 2);
         const long long blocks = min((total + 255) / 256, (long long)1 << 20);

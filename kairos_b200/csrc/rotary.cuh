@@ -135,25 +135,32 @@ struct RawCell {
         }
     }
 };
-// Cells that a thread has under way: 64 bytes of loads, which with four blocks of 256 threads on an SM keeps 64 KB of
-// loads in flight.  Twice as many with two or three blocks measured 4 to 20% slower (16381 x 32 heads of 128 in bf16: 51 us
-// against 47), half as many with six blocks 60%.
+// Cells that a thread has under way: 64 bytes of loads, which with 1024 threads on an SM keeps 64 KB of loads in flight.
+// Twice as many with 512 or 768 threads measured 4 to 20% slower (16381 x 32 heads of 128 in bf16: 51 us against 47), half
+// as many with 1536 threads 60%.
 template <typename T>
 constexpr int kCells = sizeof(T) == 4 ? 1 : 2;
 
 constexpr int kTablePairs = 2048;   // pairs whose cos and sin a block keeps: 16 KB of shared memory
+constexpr int kBlockTokens = 64;    // tokens of a block, at most
 
 // i / d for i, d below 2^16 by one multiplication; `magic` = ceil(2^32 / d).
 inline unsigned div_magic(int d) { return d == 1 ? 0u : (unsigned)((0x100000000ull + d - 1) / d); }
 __device__ __forceinline__ int div_small(int i, unsigned magic) { return magic ? (int)__umulhi((unsigned)i, magic) : i; }
 
-// Tokens of a block: about `target` rows (heads of tokens) or up to twice as many, so that they fill whole batches of
-// `batch` rows (what its threads have under way together) best, where there are enough tokens for every SM to have two such
-// blocks; else one token, so that a decode step spreads over the SMs.  128 rows of 16-bit values, 64 of fp32 ones: half and
-// twice as many measured up to 25% and 14% slower.  The angles of a block's tokens fit its table.
-inline int rows_tokens(long long tokens, int rows, int rot, int batch, int target) {
-    if (tokens * rows < 2 * 148 * target) return 1;
-    const int most = min(64, rot ? kTablePairs / (rot / 2) : 64);
+// Tokens and threads of a block.  Where every SM gets four of them or more: 128 threads and about `target` rows (heads of
+// tokens) or up to twice as many, so that they fill whole batches (what the threads have under way together; `per_step`
+// rows take 128 threads, `deep` of those a batch) best.  64 rows of 16-bit values, 32 of fp32 ones; 256 threads with twice
+// the rows measured 5 to 9% slower (a block's barrier and its last stores hold up more loads), 1.5 times the rows the same.
+// Else one token, so that a decode step spreads over the SMs, and 256 threads: 64 tokens of 48 heads 2.2 us against 2.7 with
+// 128.  The angles of a block's tokens fit its table.
+struct RowBlocks {
+    int tokens, threads;
+};
+inline RowBlocks row_blocks(long long tokens, int rows, int rot, int per_step, int deep, int target) {
+    if (tokens * rows < 4 * 148 * target) return {1, 256};
+    const int batch = per_step * deep;
+    const int most = min(kBlockTokens, rot ? kTablePairs / (rot / 2) : kBlockTokens);
     int best = 1;
     long long best_done = 0, best_room = 1;                 // rows of a block over the rows of its batches
     for (int tb = 1; tb <= most && (tb == 1 || tb * rows <= 2 * target); ++tb) {
@@ -161,7 +168,7 @@ inline int rows_tokens(long long tokens, int rows, int rot, int batch, int targe
         if (8 * done < 7 * target && tb < most && (tb + 1) * rows <= 2 * target) continue;
         if (done * best_room > best_done * room) best = tb, best_done = done, best_room = room;
     }
-    return best;
+    return {best, 128};
 }
 
 inline bool rotary_plan_ok(const kairos_rotary_plan* p, int D) {
