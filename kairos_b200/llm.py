@@ -479,9 +479,10 @@ class Decoder(torch.nn.Module):
         keys = range(self.batch)
         if not keep:
             for i in keys:
-                if self.lengths[i]:
+                if self.paged.pages(i):
                     self.paged.release(i)
             self.lengths = [0] * self.batch
+            self.lens.zero_()                # both empty, also where the pages do not suffice below
         self._grow(counts)
         starts, totals = self.lengths, [a + n for a, n in zip(self.lengths, counts)]
         self.slots, self.positions = self.paged.slots(keys, counts, starts)

@@ -105,6 +105,10 @@ class PagedKVCache:
         self._pages[key] = pages + [self._take() for _ in range(more)]
         return self._pages[key]
 
+    def pages(self, key):
+        """The pages of sequence `key` in the order of its positions, none where it is unknown."""
+        return list(self._pages.get(key, ()))
+
     def release(self, key):
         """Takes the pages of sequence `key` back.  Work that still reads them has to be ordered before their next use,
         which it is on one stream."""

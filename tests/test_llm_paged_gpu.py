@@ -115,3 +115,16 @@ def test_pages_and_lengths_run_out_loudly(model):
     model.allocate(2, 64)
     with pytest.raises(ValueError):
         model.prefill(torch.stack([prompt(4, 1)] * 2), keep=True)
+
+
+def test_a_refused_prompt_leaves_empty_sequences(model):
+    import kairos_b200 as kb
+    model.allocate_paged(2, 64, page_size=16, num_pages=3)
+    model.prefill([prompt(20, 1), prompt(10, 2)])
+    with pytest.raises(kb.KairosError):                          # the first prompt gets two pages, the second needs two
+        model.prefill([prompt(32, 3), prompt(20, 4)])
+    assert model.lengths == model.lens.tolist() == [0, 0]
+    got = model.prefill([prompt(5, 5), prompt(32, 6)], return_logits=True).clone()      # fits once those are back
+    assert model.paged.free_pages == 0
+    model.allocate_paged(2, 64, page_size=16)
+    assert close(got, model.prefill([prompt(5, 5), prompt(32, 6)], return_logits=True))

@@ -193,3 +193,13 @@ def test_c_refuses_rotary(kw, code):
 def test_empty_calls_need_no_device():
     assert attention(layer(), b=0) == 0 and write(layer(), t=0) == 0 and turn(s=0) == 0 and turn(h=0) == 0
     assert lib.kairos_paged_kv_read(ctypes.addressof(layer()), P, P, P, 0, 0, None) == 0
+
+
+def test_pages_of_a_sequence_are_a_copy():
+    c = cache()
+    assert c.pages('a') == []
+    c.reserve('a', 17)
+    held = c.pages('a')
+    assert held == c.page_table(['a'])[0].tolist() and len(held) == 2
+    held.append(5)
+    assert len(c.pages('a')) == 2 and c.free_pages == 4
