@@ -128,8 +128,9 @@ __global__ void __launch_bounds__(256, 4) rope_paged_kv_kernel(const T* __restri
                 const int t = div_small(i, p.by_pairs), pair = i - t * pairs;
                 float c, s;
                 turn_of(__ldcg(positions + t0 + t), __ldg(steps + pair), p.magnitude, &c, &s);
-                cs[i] = c;
-                sn[i] = s;
+                const int to = t * pairs + table_place(pair, pairs);
+                cs[to] = c;
+                sn[to] = s;
             }
             __syncthreads();
         }
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(256, 4) rope_paged_kv_kernel(const T* __restri
             float a[8], b[8];
             RawCell<T>::widen(raw[u].w[0], a);
             RawCell<T>::widen(raw[u].w[1], b);
-            if (cell.pair >= 0 && head < p.H + kv.heads) turn_cell(a, b, cs + t * pairs, sn + t * pairs, cell.pair, p.layout);
+            if (cell.pair >= 0 && head < p.H + kv.heads) turn_cell(a, b, cs + t * pairs, sn + t * pairs, cell.pair, pairs, p.layout);
             float amax = 0.f;
             if constexpr (!std::is_void<Codes>::value) {
                 if (__any_sync(0xffffffffu, head >= p.H)) amax = row_amax(a, b, kLanes);

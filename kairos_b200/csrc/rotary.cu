@@ -49,8 +49,9 @@ __global__ void __launch_bounds__(256, 4) rotary_kernel(const T* X, T* Y, const 
                 const long long token = t0 + t, b = p.S == p.tokens ? 0 : (unsigned)token / (unsigned)p.S;
                 float c, s;
                 turn_of(__ldcg(positions + b * p.pb + (token - b * p.S) * p.ps), __ldg(steps + pair), p.magnitude, &c, &s);
-                cs[i] = c;
-                sn[i] = s * p.sign;
+                const int to = t * pairs + table_place(pair, pairs);
+                cs[to] = c;
+                sn[to] = s * p.sign;
             }
             __syncthreads();
         }
@@ -62,7 +63,7 @@ __global__ void __launch_bounds__(256, 4) rotary_kernel(const T* X, T* Y, const 
             RawCell<T>::widen(raw[u].w[0], a);
             RawCell<T>::widen(raw[u].w[1], b);
             const int t = div_small(r, p.by_heads);
-            if (cell.pair >= 0) turn_cell(a, b, cs + t * pairs, sn + t * pairs, cell.pair, p.layout);
+            if (cell.pair >= 0) turn_cell(a, b, cs + t * pairs, sn + t * pairs, cell.pair, pairs, p.layout);
             T* y = Y + place(r, p.yb, p.ys, p.yh);
             store8(y + cell.first, a);
             store8(y + cell.second, b);

@@ -85,14 +85,21 @@ __device__ __forceinline__ Cell cell_of(int j, int rot, int layout) {
     c.pair = j < turning ? 8 * j : -1;
     return c;
 }
-// Turns the cell's eight pairs by the table entries cs / sn (fp32 cos and sin, indexed by pair).
-__device__ __forceinline__ void turn_cell(float (&a)[8], float (&b)[8], const float* cs, const float* sn, int pair,
+// Where a token's table of `pairs` angles (a multiple of 8) holds a pair: the first four of every eight, then the other
+// fours, so that neighbouring cells read neighbouring 16 bytes without bank conflicts (4099 x 28 fp32 heads 20.3 us against
+// 20.9 in order).
+__device__ __forceinline__ int table_place(int pair, int pairs) {
+    return (pair & 4 ? pairs >> 1 : 0) + (pair >> 3) * 4 + (pair & 3);
+}
+// Turns the cell's eight pairs from `pair` on by a token's table cs / sn (fp32 cos and sin).
+__device__ __forceinline__ void turn_cell(float (&a)[8], float (&b)[8], const float* cs, const float* sn, int pair, int pairs,
                                           int layout) {
     float c[8], s[8];
-    *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(cs + pair);
-    *reinterpret_cast<float4*>(c + 4) = *reinterpret_cast<const float4*>(cs + pair + 4);
-    *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(sn + pair);
-    *reinterpret_cast<float4*>(s + 4) = *reinterpret_cast<const float4*>(sn + pair + 4);
+    const int low = pair >> 1, high = low + (pairs >> 1);
+    *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(cs + low);
+    *reinterpret_cast<float4*>(c + 4) = *reinterpret_cast<const float4*>(cs + high);
+    *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(sn + low);
+    *reinterpret_cast<float4*>(s + 4) = *reinterpret_cast<const float4*>(sn + high);
     if (layout == 0) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) turn_pair(a[i], b[i], c[i], s[i]);
