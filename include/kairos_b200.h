@@ -264,8 +264,8 @@ int kairos_rotary(const void* X, long long x_b, long long x_s, long long x_h, vo
  * cache at slots[t] = page * page_size + offset (int64).  A 16-bit cache has QKV's type; rows of an I8 / E4M3 cache
  * are quantized from the fp32 rotated values (code = nearest-even of row / scale).  A row with an infinity or NaN
  * gets scale NaN.  slots[t] < 0 marks padding: nothing is stored for it (its q row is).  slots[t] past the pool is
- * not stored either and raises the device status word (KAIROS_ERR_ARG).  Slots must be distinct.
- * rot % 16 == 0. */
+ * not stored either and raises the device status word (KAIROS_ERR_ARG).  Slots must be distinct,
+ * and Q_out must not overlap QKV.  rot % 16 == 0. */
 int kairos_rope_paged_kv(const void* QKV, long long row_stride, const void* positions, const void* slots,
                          const kairos_rotary_plan* plan, const kairos_kv_layer* kv, void* Q_out, int T, int H, int dtype,
                          kairos_stream_t stream);
@@ -275,7 +275,7 @@ int kairos_paged_kv_read(const kairos_kv_layer* kv, const void* slots, void* K_o
                          kairos_stream_t stream);
 /* Attention of one new token per sequence: O[b,h,:] = sum_j softmax_j(scale * Q[b,h,:] . K[j,:]) V[j,:] over the
  * sequence's lens[b] positions, position j at offset j % page_size of page page_table[b, j / page_size].
- * Q [B, H, D] F16 / BF16 with element strides {b, h} (multiples of 8); O dense [B, H, D] of the same type; a 16-bit cache has Q's
+ * Q [B, H, D] F16 / BF16 with element strides {b, h} (multiples of 8); O dense [B, H, D] of the same type (it may be Q); a 16-bit cache has Q's
  * type.  table_width * page_size <= 2^30 and H % kv_heads == 0 (head h reads kv head h / (H / kv_heads)).  LSE [B, H] fp32 (natural logarithm of the
  * softmax's denominator) when not null.  lens[b] <= 0: O = 0, LSE = -inf.  Entries of the table behind the end may
  * hold anything.  A page outside the pool is left out of the sum, lens[b] is cut to table_width * page_size, and both

@@ -320,8 +320,9 @@ def rotary(x, positions, rotary, transpose=False, out=None):
         raise _bad(positions, 'positions', 'int64', index)
     if out is None:
         out = torch.empty_like(x)
-    elif out.shape != shape or out.dtype != x.dtype or out.get_device() != index or out.stride(-1) != 1:
-        raise _bad(out, 'out', f'{x.dtype} {tuple(shape)} with a dense last dimension', index)
+    elif out.shape != shape or out.dtype != x.dtype or out.get_device() != index or out.stride(-1) != 1 or \
+            any(step == 0 and n > 1 for step, n in zip(out.stride(), shape)):
+        raise _bad(out, 'out', f'{x.dtype} {tuple(shape)} with a dense last dimension and a place for every element', index)
     to, at = out.stride(), positions
     if dims == 3:
         b, xb, yb, pb, (s, h, d) = 1, 0, 0, 0, shape
@@ -346,7 +347,7 @@ def rope_paged_kv(qkv, positions, slots, rotary, cache, layer=0, q_out=None):
     """One pass over the fused activation qkv [T, (H + 2 kv_heads) * D] (fp16 / bf16, rows may be strided): returns the
     turned q heads [T, H, D], and stores the turned k heads and the v heads at ``slots`` [T] of the cache's `layer`, in
     the cache's type (int8 / e4m3 rows are quantized from fp32).  positions and slots are int64 [T]; a negative slot is
-    padding and stores nothing; slots must be distinct."""
+    padding and stores nothing; slots must be distinct, and q_out must not overlap qkv."""
     d, shape, code, index = cache.head_dim, qkv.shape, _HALVES.get(qkv.dtype), qkv.get_device()
     if code is None or len(shape) != 2 or shape[1] % d or qkv.stride(1) != 1:
         raise _bad(qkv, 'qkv', f'fp16 or bf16 [tokens, heads * {d}] with dense rows', index)

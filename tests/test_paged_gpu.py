@@ -648,3 +648,16 @@ def test_operators_together(dtype, kv):
     x = qkv.view(3, -1, d)[:, h + hkv:].double()
     assert ((v.double() - x).abs() <= held64(x, kv) * (1 + 1e-5) + 1e-12).all()
     assert status() == 0
+
+
+def test_rotary_refuses_a_result_that_overlaps_itself():
+    import kairos_b200 as kb
+    from kairos_b200 import ops
+    r, one, pos = kb.Rotary(64), randn((1, 2, 64), 1), torch.arange(3, device=DEV)
+    x = one.expand(3, 2, 64)                                    # broadcast inputs are fine, broadcast results are not
+    assert_turned(ops.rotary(x, pos, r), x, pos, r)
+    with pytest.raises(ValueError):
+        ops.rotary(x, pos, r, out=x)
+    with pytest.raises(ValueError):
+        ops.rotary(x, pos, r, out=torch.empty((3, 1, 64), dtype=F16, device=DEV).expand(3, 2, 64))
+    assert ops.rotary(one, pos[:1], r, out=torch.empty_like(one).expand(1, 2, 64)).shape == one.shape
