@@ -911,13 +911,14 @@ static int make_plan(const KvView& kv, bool coded, int B, int H, int table_width
     // meet in shared memory: one launch, no scan of the lengths, no workspace.  Otherwise the device cuts the work by the
     // lengths, which costs 2 to 4 us more but keeps every block busy whatever they are.  Up to four tiles go to one block, more
     // are shared by two tiles a block: 256 positions take 5.0 us in one block and 5.1 in four, 512 take 6.6 in one or two and
-    // 5.6 in four.  Sixteen at the most (twelve where pairs are few): in fp16, 32 sequences of 1024 positions take 23.6 us in
-    // blocks of their own and 27.8 cut (17.5 and 20.3 with lengths from 32 to 1024), 16 of 2048 in clusters of two 24.6 and
-    // 28.9 (19.0 and 19.6), but 16 of 256 to 4096 32.5 and 30.1 (43.4 and 48.0 where all have 4096), one of 8192 in clusters
-    // of eight 15.5 and 12.6.
+    // 5.6 in four.  A single block takes twenty at the most: in fp16, 32 sequences of 1280 positions take 28.3 us in blocks of
+    // their own and 32.4 cut (20.7 and 22.7 with lengths from 1 to 1280, but one of 1280 and 31 of 160 14.7 and 11.1; of 1536:
+    // 33.2 and 37.3, 23.9 and 25.0, 19.0 and 11.5).  In clusters sixteen (twelve where pairs are few): 16 of 2048 in clusters of
+    // two 24.6 and 28.9 (19.0 and 19.6 with lengths from 128 on), but 16 of 256 to 4096 32.5 and 30.1 (43.4 and 48.0 where all
+    // have 4096), one of 8192 in clusters of eight 15.5 and 12.6.
     int cluster = 1;
     while (cluster < 8 && pairs * cluster * 2 <= full && tiles > 4 && tiles > 2 * cluster) cluster *= 2;
-    out->cluster = pairs * cluster <= full && (tiles + cluster - 1) / cluster <= (pairs < 32 ? 12 : 16) ? cluster : 0;
+    out->cluster = pairs * cluster <= full && (tiles + cluster - 1) / cluster <= (cluster == 1 ? 20 : pairs < 32 ? 12 : 16) ? cluster : 0;
     // With many more pairs than blocks fit, blocks of their own in several waves are balanced by their number and end a
     // pair without holding the next one up: 128 sequences of 1000 positions in int8 50.3 us and 58.4 cut, 128 of 2048 92.8
     // and 97.7 (fp16 84.8 and 85.4, 160.9 and 162.2), with 16 heads a kv head 64 of 1 to 1000 in int8 (512 pairs for 444
