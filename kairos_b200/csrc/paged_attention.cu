@@ -192,6 +192,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// What a row's sum is divided by.  Where no position was left (every page outside the pool) the row is an empty one: zeros, and
+// a logarithm of -inf; NaN among the inputs stays NaN.
+__device__ __forceinline__ float inverse_sum(float top, float sum) {
+    return top == -INFINITY && sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+}
 // A thread-block cluster: barrier halves, and the shared memory of block `rank` at the address that `a` has in this one.
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -766,7 +771,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
                 *reinterpret_cast<float4*>(reinterpret_cast<float*>(smem + R::kLastOut) + at(row, c)) = acc;
                 if (c == 0) jpart[row] = make_float2(top, sum);
             } else if (whole) {
-                const float inv = __fdiv_rn(1.f, sum);
+                const float inv = inverse_sum(top, sum);
                 const size_t to = (size_t)done.b * p.H + q0 + row;
                 put4(O + to * D + c, acc, inv);
                 if (LSE && c == 0) LSE[to] = (top + __log2f(sum) - kLift) * kLn2;
@@ -799,7 +804,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
                     acc.w = __fmaf_rn(f, v.w, acc.w);
                 }
                 const size_t to = (size_t)done.b * p.H + q0 + row;
-                put4(O + to * D + c, acc, __fdiv_rn(1.f, sum));
+                put4(O + to * D + c, acc, inverse_sum(top, sum));
                 if (LSE && c == 0) LSE[to] = (top + __log2f(sum) - kLift) * kLn2;
             }
             __syncwarp();
@@ -869,7 +874,7 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(QT* __restric
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) add(part_ml[w][lane], part_o[w][lane]);
     const size_t at = (size_t)b * p.H + head * p.group + block * kHeads + row;
-    put4(O + at * D + c, acc, __fdiv_rn(1.f, sum));
+    put4(O + at * D + c, acc, inverse_sum(top, sum));
     if (LSE && c == 0) LSE[at] = (top + __log2f(sum) - kLift) * kLn2;
 }
 
