@@ -27,6 +27,7 @@
 // (value and remainder): rounding them to 16 bits alone would add an error as large as the output's own rounding.
 // The reference m of the exponent need not be the maximum: it moves (and o and l are rescaled) only when a score
 // passes it by 2^kSlack, so most stages need neither a reduction over lanes nor a rescaling.
+#include <cfloat>
 #include <type_traits>
 
 #include "paged_kv.cuh"
@@ -40,9 +41,10 @@ constexpr int kSub = 16;                    // positions of a stage
 constexpr int kTile = kSub * kWarps;        // positions per scheduling tile
 // Weights are kept times 2^kLift and pass the reference by 2^kSlack at the most; with a V scale of up to twice the largest
 // so far they stay below 2^15, and fp16's smallest step is 2^-30 of a weight at the reference.
-constexpr float kLift = 6.f, kSlack = 8.f;
-// Reference (less kLift) of a head before its first score: any score passes it.
-constexpr float kUnset = -1e30f;
+constexpr float kLift = 6.f, kSlack = 8.f, kMost = 16384.f;         // kMost = 2^(kLift + kSlack)
+// Reference of a head before its first score: any score passes it.  References are finite, so that differences of two are
+// never NaN; a head that has seen no score has a sum of 0.
+constexpr float kUnset = -FLT_MAX;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnShape {
@@ -194,9 +196,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 // What a row's sum is divided by.  Where no position was left (every page outside the pool) the row is an empty one: zeros, and
 // a logarithm of -inf; NaN among the inputs stays NaN.
-__device__ __forceinline__ float inverse_sum(float top, float sum) {
-    return top == -INFINITY && sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-}
+__device__ __forceinline__ float inverse_sum(float sum) { return sum == 0.f ? 0.f : __fdiv_rn(1.f, sum); }
 // A thread-block cluster: barrier halves, and the shared memory of block `rank` at the address that `a` has in this one.
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -532,11 +532,12 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
         settle();
         // o[j][r]: channels 16 j + g and + 8 (coded: g * D / 8 + 2 j and + 1) of heads 2 t, 2 t + 1 (+ 8 r)
         float o[D / 16][kHalves][4] = {};
-        float m[kHalves][2], base[kHalves][2], l[kHalves][2], vtop = 7.888609052210118e-31f, vinv = 1.2676506002282294e30f;   // 2^-100, 2^100
+        // l and o are sums of weights 2^(s - base)
+        float base[kHalves][2], l[kHalves][2], vtop = 7.888609052210118e-31f, vinv = 1.2676506002282294e30f;   // 2^-100, 2^100
 #pragma unroll
         for (int r = 0; r < kHalves; ++r)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) m[r][e] = -INFINITY, base[r][e] = kUnset, l[r][e] = 0.f;
+            for (int e = 0; e < 2; ++e) base[r][e] = kUnset, l[r][e] = 0.f;
 
 #pragma unroll 1
         for (int pos = k0; pos < k1; pos += stride) {
@@ -597,21 +598,24 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
                     for (int r = 0; r < kHalves; ++r) s[r][2 * k] *= ks, s[r][2 * k + 1] *= ks;
                 }
             }
-            float x[kHalves][4];                // exponents
-            auto exponents = [&]() {
-#pragma unroll
-                for (int r = 0; r < kHalves; ++r)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[r][e] = __fmaf_rn(s[r][e], unit[r][e & 1], -base[r][e & 1]);
-                        if (dead[e >> 1]) x[r][e] = -INFINITY;
-                    }
-            };
-            exponents();
+            // In units of log2 e, rounded to fp32 before the reference is taken off: a score of any size less itself is 0, where
+            // the exact product less its rounding can be any number once scores pass 2^27.
 #pragma unroll
             for (int r = 0; r < kHalves; ++r)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) move |= x[r][e] > kLift + kSlack;
+                for (int e = 0; e < 4; ++e) s[r][e] = dead[e >> 1] ? -INFINITY : s[r][e] * unit[r][e & 1];
+            float w[kHalves][4];
+            auto weights = [&]() {
+#pragma unroll
+                for (int r = 0; r < kHalves; ++r)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[r][e] = exp2_fast(s[r][e] - base[r][e & 1]);
+            };
+            weights();
+#pragma unroll
+            for (int r = 0; r < kHalves; ++r)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) move |= w[r][e] > kMost;
             if (__any_sync(0xffffffffu, move)) {
                 float grow = 1.f;
                 if constexpr (kCoded) {
@@ -628,20 +632,19 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
                 for (int r = 0; r < kHalves; ++r)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float top = dead[0] ? -INFINITY : s[r][e] * unit[r][e];
-                        if (!dead[1]) top = fmaxf(top, s[r][e + 2] * unit[r][e]);
+                        float top = fmaxf(s[r][e], s[r][e + 2]);
 #pragma unroll
                         for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-                        top = fmaxf(m[r][e], top);
-                        const float safe = top == -INFINITY ? 0.f : top;
-                        const float keep = exp2_fast(m[r][e] - safe);
-                        m[r][e] = top;
-                        base[r][e] = top == -INFINITY ? kUnset : top - kLift;
+                        float to = top - kLift;
+                        if (top - to > kLift + kSlack) to = top;        // where fp32 no longer resolves kLift
+                        to = fmaxf(base[r][e], to);
+                        const float keep = exp2_fast(base[r][e] - to);
+                        base[r][e] = to;
                         l[r][e] *= keep;
 #pragma unroll
                         for (int j = 0; j < D / 16; ++j) o[j][r][e] *= keep * grow, o[j][r][e + 2] *= keep * grow;
                     }
-                exponents();
+                weights();
             }
             // weights as the second operand of o^T += V^T w^T: positions 2 t, 2 t + 1 (and 8 further) of head g
             uint32_t wb[kHalves][2], rest[kHalves][2];
@@ -649,7 +652,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
             for (int r = 0; r < kHalves; ++r)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    float w0 = exp2_fast(x[r][2 * k]), w1 = exp2_fast(x[r][2 * k + 1]);
+                    float w0 = w[r][2 * k], w1 = w[r][2 * k + 1];
                     l[r][0] += w0;
                     l[r][1] += w1;
                     if constexpr (kCoded) {
@@ -723,7 +726,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
                 float sum = l[r][e];
 #pragma unroll
                 for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-                if (g == 0) jm[warp][row] = m[r][e], jl[warp][row] = sum;
+                if (g == 0) jm[warp][row] = base[r][e], jl[warp][row] = sum;
                 if constexpr (kCoded) {
 #pragma unroll
                     for (int j = 0; j < D / 16; j += 2)
@@ -746,15 +749,14 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
             record({done.b, done.pair, part, (run_end - done.take + done.tiles - 1) / cut.run * p.lanes + blockIdx.x % p.lanes});
         for (int i = threadIdx.x; i < rows * (D / 4); i += 128) {
             const int row = i / (D / 4), c = 4 * (i - row * (D / 4));
-            float top = -INFINITY;
+            float top = kUnset;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) top = fmaxf(top, jm[w][row]);
-            const float safe = top == -INFINITY ? 0.f : top;
             float sum = 0.f;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const float f = exp2_fast(jm[w][row] - safe);
+                const float f = exp2_fast(jm[w][row] - top);
                 const float* from = reinterpret_cast<const float*>(smem + jslot[w]);
                 float4 v = *reinterpret_cast<const float4*>(from + at(row, c));
                 if constexpr (kTwin) {          // what the remainders gave
@@ -771,10 +773,10 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
                 *reinterpret_cast<float4*>(reinterpret_cast<float*>(smem + R::kLastOut) + at(row, c)) = acc;
                 if (c == 0) jpart[row] = make_float2(top, sum);
             } else if (whole) {
-                const float inv = inverse_sum(top, sum);
+                const float inv = inverse_sum(sum);
                 const size_t to = (size_t)done.b * p.H + q0 + row;
                 put4(O + to * D + c, acc, inv);
-                if (LSE && c == 0) LSE[to] = (top + __log2f(sum) - kLift) * kLn2;
+                if (LSE && c == 0) LSE[to] = (top + log2f(sum)) * kLn2;
             } else {
                 *reinterpret_cast<float4*>(Partials<kHeads, D>::o(ws, part) + row * D + c) = acc;
                 if (c == 0) *reinterpret_cast<float2*>(Partials<kHeads, D>::ml(ws, part) + 2 * row) = make_float2(top, sum);
@@ -788,15 +790,14 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
             cluster_wait();
             for (int i = threadIdx.x + 128 * (blockIdx.x % p.cluster); i < rows * (D / 4); i += 128 * p.cluster) {
                 const int row = i / (D / 4), c = 4 * (i - row * (D / 4));
-                float top = -INFINITY, sum = 0.f;
+                float top = kUnset, sum = 0.f;
                 float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
                 const uint32_t from_o = smem_u32(smem) + R::kLastOut + at(row, c) * 4, from_ml = smem_u32(&jpart[row]);
                 for (int k = 0; k < p.cluster; ++k) top = fmaxf(top, ld_cluster2(cluster_map(from_ml, k)).x);
-                const float safe = top == -INFINITY ? 0.f : top;
                 for (int k = 0; k < p.cluster; ++k) {
                     const float2 ml = ld_cluster2(cluster_map(from_ml, k));
                     const float4 v = ld_cluster4(cluster_map(from_o, k));
-                    const float f = exp2_fast(ml.x - safe);
+                    const float f = exp2_fast(ml.x - top);
                     sum = __fmaf_rn(f, ml.y, sum);
                     acc.x = __fmaf_rn(f, v.x, acc.x);
                     acc.y = __fmaf_rn(f, v.y, acc.y);
@@ -804,8 +805,8 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
                     acc.w = __fmaf_rn(f, v.w, acc.w);
                 }
                 const size_t to = (size_t)done.b * p.H + q0 + row;
-                put4(O + to * D + c, acc, inverse_sum(top, sum));
-                if (LSE && c == 0) LSE[to] = (top + __log2f(sum) - kLift) * kLn2;
+                put4(O + to * D + c, acc, inverse_sum(sum));
+                if (LSE && c == 0) LSE[to] = (top + log2f(sum)) * kLn2;
             }
             __syncwarp();
             cluster_arrive();
@@ -836,11 +837,10 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(QT* __restric
     const int b = (int)record.x, pair = (int)record.y, head = pair / p.blocks_per_kv, block = pair - head * p.blocks_per_kv;
     const int rows = min(kHeads, p.group - block * kHeads);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane / kPer, c = 4 * (blockIdx.y * kPer + lane % kPer);
-    float top = -INFINITY, sum = 0.f;
+    float top = kUnset, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [&](const float2 ml, const float4 v) {
-        const float next = fmaxf(top, ml.x), safe = next == -INFINITY ? 0.f : next;
-        const float keep = exp2_fast(top - safe), f = exp2_fast(ml.x - safe);
+        const float next = fmaxf(top, ml.x), keep = exp2_fast(top - next), f = exp2_fast(ml.x - next);
         top = next;
         sum = __fmaf_rn(sum, keep, f * ml.y);
         acc.x = __fmaf_rn(acc.x, keep, f * v.x);
@@ -874,8 +874,8 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(QT* __restric
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) add(part_ml[w][lane], part_o[w][lane]);
     const size_t at = (size_t)b * p.H + head * p.group + block * kHeads + row;
-    put4(O + at * D + c, acc, inverse_sum(top, sum));
-    if (LSE && c == 0) LSE[at] = (top + __log2f(sum) - kLift) * kLn2;
+    put4(O + at * D + c, acc, inverse_sum(sum));
+    if (LSE && c == 0) LSE[at] = (top + log2f(sum)) * kLn2;
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------

@@ -40,3 +40,54 @@ def test_padded_rows_of_one_position_and_no_page(dtype, kv):
     got, lse = ops.paged_attention(q, c, table, n, return_lse=True)
     assert status() == -8
     check_attention(c, q, table, [60, 0, 0], got, lse)
+
+
+def level_case(dtype, kv, lens, special, width=0):
+    """Keys that are 1 in channel 0 and nothing elsewhere, 2 at position special[i] of sequence i; queries 1 in channel 0."""
+    c, q, table, n = attention_case(dtype, kv, lens, 8, 2, 64, 16, seed=3)
+    q.zero_()
+    q[..., 0] = 1
+    top = {I8: 127.0, E4M3: 448.0}.get(kv, 1.0)
+    row = torch.zeros(64, device=DEV)
+    row[0] = top
+    for i, m in enumerate(lens):
+        for j in range(m):
+            page, at = table[i, j // 16].item(), j % 16
+            factor = 2.0 if j == special[i] else 1.0
+            if c.k_scale is None:
+                c.k[0, page, :, at] = (row * factor).to(kv)
+            else:
+                c.k[0, page, :, at].view(torch.uint8).copy_(row.to(kv).view(torch.uint8).expand(2, -1))
+                c.k_scale[0, page, :, at] = factor / top
+    wide = torch.full((len(lens), max(width, table.shape[1])), -1, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    return c, q, wide, n
+
+
+@pytest.mark.parametrize('dtype,kv', TYPES)
+@pytest.mark.parametrize('special', [(0, 0), (3, 149), (100, 40)])
+@pytest.mark.parametrize('width', [0, 2000])
+def test_scores_of_any_size(dtype, kv, special, width):
+    """Scores of +-2^8 to +-2^126: where one is twice the others, either it has all of the weight or the others share it
+    evenly, whatever fp32 makes of them, since equal scores stay equal.  n / 16 + 64 additions, 8 U for weights and scale
+    factors, 2^-16 for the weights' halves, as in check_attention."""
+    from kairos_b200 import ops
+    lens = [200, 150]
+    c, q, table, n = level_case(dtype, kv, lens, special, width)
+    v64 = c.v[0].float().double() if c.v_scale is None else c.v[0].float().double() * c.v_scale[0].double()[..., None]
+    for power in (8, 20, 26, 27, 28, 29, 30, 31, 40, 100, 126):
+        for sign in (1, -1):
+            if power == 126 and sign == 1:
+                continue                                        # the doubled score is past fp32
+            got, lse = ops.paged_attention(q, c, table, n, scale=sign * 2.0 ** power, return_lse=True)
+            for i, m in enumerate(lens):
+                at = torch.arange(m, device=DEV)
+                v = v64[table[i].long()[at // 16], :, at % 16]
+                mine = at == special[i] if sign > 0 else at != special[i]
+                ref, size = v[mine].mean(0), v[mine].abs().mean(0)
+                tol = EPS[dtype] * ref.abs() + TINY[dtype] + size * ((m / 16 + 64) * 2 * U + 8 * U + 2.0 ** -16)
+                assert ((got[i].view(2, 4, 64).double() - ref[:, None]).abs() <= tol[:, None]).all(), (power, sign, i)
+                level = (2.0 if sign > 0 else -1.0) * 2.0 ** power + math.log(mine.sum().item())
+                # codes: 127 * (1 / 127) and the sum of D products are off by 2 U each at the most
+                assert ((lse[i].double() - level).abs() <= (m / 16 + 64) * 2 * U + 12 * U * (1 + abs(level))).all(), (power, sign, i)
+    assert status() == 0
