@@ -39,12 +39,21 @@ int* device_status_word();   // api.cu
 constexpr int kWarps = 4;
 constexpr int kSub = 16;                    // positions of a stage
 constexpr int kTile = kSub * kWarps;        // positions per scheduling tile
-// Weights are kept times 2^kLift and pass the reference by 2^kSlack at the most; with a V scale of up to twice the largest
-// so far they stay below 2^15, and fp16's smallest step is 2^-30 of a weight at the reference.
+// Weights are kept times 2^kLift and pass the reference by 2^kSlack at the most, so that they stay below 2^15, and fp16's
+// smallest step is 2^-30 of a weight at the reference.
 constexpr float kLift = 6.f, kSlack = 8.f, kMost = 16384.f;         // kMost = 2^(kLift + kSlack)
 // Reference of a head before its first score: any score passes it.  References are finite, so that differences of two are
 // never NaN; a head that has seen no score has a sum of 0.
 constexpr float kUnset = -FLT_MAX;
+// Coded caches: what enters the second product is weight * V scale, and each head keeps a power of two of its own under it: the
+// largest product so far lies between 2^8 and 2^9 when the power is set and below 2^15 until the next time, so fp16's smallest
+// step is 2^-32 of it.  A row's scale alone sets nothing: one that is 2^60 times the others', with a weight of 2^-90, takes
+// no bits from them.  (2^12 in place of 2^8 moves the power more often: 64 sequences up to 4000 positions in int8, 16 heads a
+// kv head, 51.2 us from 48.2.)
+constexpr int kLargest = 8;
+constexpr float kOver = 32768.f;
+// Inverse of a power of two.
+__device__ __forceinline__ float inverse_pow2(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnShape {
@@ -194,6 +203,21 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Two fp32 operations in one instruction: what the loop does to the scores of heads 2 t and 2 t + 1 of a position (rows of 64
+// int8 channels, 64 sequences up to 4000 positions: 37.6 us, 38.3 with an instruction each).
+__device__ __forceinline__ uint64_t bits2(const float2& a) { return (uint64_t)__float_as_uint(a.y) << 32 | __float_as_uint(a.x); }
+__device__ __forceinline__ float2 from_bits2(uint64_t a) { return make_float2(__uint_as_float((uint32_t)a), __uint_as_float((uint32_t)(a >> 32))); }
+__device__ __forceinline__ float2 mul2(const float2& a, const float2& b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+    return from_bits2(r);
+}
+__device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+    return from_bits2(r);
+}
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
 // What a row's sum is divided by.  Where no position was left (every page outside the pool) the row is an empty one: zeros, and
 // a logarithm of -inf; NaN among the inputs stays NaN.
 __device__ __forceinline__ float inverse_sum(float sum) { return sum == 0.f ? 0.f : __fdiv_rn(1.f, sum); }
@@ -402,7 +426,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
     const size_t page_bytes = (size_t)page_rows * R::kRowBytes;
     int ahead = 0;                              // page of the next stage to request
     uint32_t qb[D / 16][2 * kHalves];
-    float unit[kHalves][2];                     // score = product * unit (* scale of the key), heads 2 t and 2 t + 1 (+ 8)
+    float2 unit[kHalves];                       // score = product * unit (* scale of the key), heads 2 t and 2 t + 1 (+ 8)
 
     auto look = [&](int key) { return key < k1 ? __ldcg(pages + (key >> kv.page_shift)) : 0; };
     auto request = [&](int key, int slot, int from) {      // the 16 positions from `key` on, which lie in page `from`, into a slot
@@ -466,7 +490,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
         // words lie: a thread's four channels are 4 t .. 4 t + 3.
 #pragma unroll
         for (int r = 0; r < kHalves; ++r) {
-            unit[r][0] = unit[r][1] = p.scale_log2;
+            unit[r] = both(p.scale_log2);
             const int row = kTwin ? g & 3 : g + 8 * r;
             const bool real = row < rows;
             const QT* q = Q + (size_t)sg.b * p.qb + (size_t)(head * p.group + block * kHeads + (real ? row : 0)) * p.qh;
@@ -503,8 +527,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
                 const int e2 = top > 0.f && top <= 3e38f ? max(-110, min(126, (int)(__float_as_uint(top) >> 23) - 127)) : 13;
                 const float up = __uint_as_float((uint32_t)(127 + 13 - e2) << 23);
                 const float back = p.scale_log2 * __uint_as_float((uint32_t)(127 - 13 + e2) << 23);
-                unit[r][0] = __shfl_sync(0xffffffffu, back, 8 * t);
-                unit[r][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+                unit[r] = make_float2(__shfl_sync(0xffffffffu, back, 8 * t), __shfl_sync(0xffffffffu, back, 8 * t + 4));
 #pragma unroll
                 for (int s = 0; s < D / 16; ++s)
 #pragma unroll
@@ -532,12 +555,11 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
         settle();
         // o[j][r]: channels 16 j + g and + 8 (coded: g * D / 8 + 2 j and + 1) of heads 2 t, 2 t + 1 (+ 8 r)
         float o[D / 16][kHalves][4] = {};
-        // l and o are sums of weights 2^(s - base)
-        float base[kHalves][2], l[kHalves][2], vtop = 7.888609052210118e-31f, vinv = 1.2676506002282294e30f;   // 2^-100, 2^100
+        // l and o are sums of weights 2^(s + back); heads 2 t and 2 t + 1.  Coded: the power of two that products are kept times,
+        // at first 2^122
+        float2 back[kHalves], l[kHalves], shift[kHalves];
 #pragma unroll
-        for (int r = 0; r < kHalves; ++r)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) base[r][e] = kUnset, l[r][e] = 0.f;
+        for (int r = 0; r < kHalves; ++r) back[r] = both(-kUnset), l[r] = both(0.f), shift[r] = both(5.316911983139664e36f);
 
 #pragma unroll 1
         for (int pos = k0; pos < k1; pos += stride) {
@@ -579,88 +601,110 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
                     }
                 }
             }
-            // positions g, g + 8: the scale of V, and which of them are no positions at all
+            // positions g, g + 8 (k): the scale of V; where there is no position, 0 and a score of -inf.  Scores are in units of
+            // log2 e, rounded to fp32 before the reference is taken off: a score of any size less itself is 0, where the exact
+            // product less its rounding can be any number once scores pass 2^27.
+            float2 x[kHalves][2];
             float vs[2];
-            bool dead[2] = {false, false};
-            if (!full) {
 #pragma unroll
-                for (int k = 0; k < 2; ++k) dead[k] = 8 * k + g >= real || gone;
-            }
-            bool move = false;
-            if constexpr (kCoded) {
+            for (int k = 0; k < 2; ++k) {
+                if constexpr (kCoded) vs[k] = scales[kSub + 8 * k + g];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const float ks = scales[8 * k + g];
-                    vs[k] = scales[kSub + 8 * k + g];
-                    if (dead[k]) vs[k] = 0.f;   // scales behind the end may be anything, NaN too
-                    move |= fabsf(vs[k]) > 2.f * vtop;
-#pragma unroll
-                    for (int r = 0; r < kHalves; ++r) s[r][2 * k] *= ks, s[r][2 * k + 1] *= ks;
+                for (int r = 0; r < kHalves; ++r) {
+                    x[r][k] = make_float2(s[r][2 * k], s[r][2 * k + 1]);
+                    if constexpr (kCoded) x[r][k] = mul2(x[r][k], both(scales[8 * k + g]));
+                    x[r][k] = mul2(x[r][k], unit[r]);
                 }
             }
-            // In units of log2 e, rounded to fp32 before the reference is taken off: a score of any size less itself is 0, where
-            // the exact product less its rounding can be any number once scores pass 2^27.
+            if (!full) {
 #pragma unroll
-            for (int r = 0; r < kHalves; ++r)
+                for (int k = 0; k < 2; ++k)
+                    if (8 * k + g >= real || gone) {
+                        vs[k] = 0.f;            // scales behind the end may be anything, NaN too
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[r][e] = dead[e >> 1] ? -INFINITY : s[r][e] * unit[r][e & 1];
-            float w[kHalves][4];
+                        for (int r = 0; r < kHalves; ++r) x[r][k] = both(-INFINITY);
+                    }
+            }
+            float2 w[kHalves][2], wv[kHalves][2];           // weights, and what enters the second product
             auto weights = [&]() {
 #pragma unroll
                 for (int r = 0; r < kHalves; ++r)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) w[r][e] = exp2_fast(s[r][e] - base[r][e & 1]);
+                    for (int k = 0; k < 2; ++k) {
+                        const float2 y = add2(x[r][k], back[r]);
+                        w[r][k] = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                        wv[r][k] = kCoded ? mul2(w[r][k], both(vs[k])) : w[r][k];
+                    }
             };
+            auto shifted = [&](int r, int k) { return kCoded ? mul2(wv[r][k], shift[r]) : wv[r][k]; };
             weights();
+            bool move = false;
 #pragma unroll
             for (int r = 0; r < kHalves; ++r)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) move |= w[r][e] > kMost;
+                for (int k = 0; k < 2; ++k) {
+                    move |= w[r][k].x > kMost || w[r][k].y > kMost;
+                    if constexpr (kCoded) {
+                        const float2 v = shifted(r, k);
+                        move |= fabsf(v.x) > kOver || fabsf(v.y) > kOver;
+                    }
+                }
             if (__any_sync(0xffffffffu, move)) {
-                float grow = 1.f;
-                if constexpr (kCoded) {
-                    float top = fmaxf(fabsf(vs[0]), fabsf(vs[1]));
+                float keep[kHalves][2];
+                auto top_of = [](float a, float b) {        // over the positions of the stage
+                    float top = fmaxf(a, b);
 #pragma unroll
-                    for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-                    if (top > vtop) {
-                        grow = __fdividef(vtop, top);
-                        vtop = top;
-                        vinv = __frcp_rn(top);
+                    for (int i = 4; i < 32; i <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+                    return top;
+                };
+                // a new reference for a head that needs one; what the sums before are multiplied by
+                auto refer = [](float top, float& back) {
+                    if (!(top + back > kLift + kSlack)) return 1.f;
+                    float to = top - kLift;
+                    if (top - to > kLift + kSlack) to = top;            // where fp32 no longer resolves kLift
+                    const float keep = exp2_fast(-back - to);
+                    back = -to;
+                    return keep;
+                };
+#pragma unroll
+                for (int r = 0; r < kHalves; ++r) {
+                    keep[r][0] = refer(top_of(x[r][0].x, x[r][1].x), back[r].x);
+                    keep[r][1] = refer(top_of(x[r][0].y, x[r][1].y), back[r].y);
+                    l[r] = mul2(l[r], make_float2(keep[r][0], keep[r][1]));
+                }
+                weights();
+                if constexpr (kCoded) {
+                    auto raise = [](float top, float& keep, float& shift) {
+                        // never above the largest product so far, as the new reference leaves it
+                        const float was = inverse_pow2(shift);
+                        top = fmaxf(top, was * (float)(1 << kLargest) * keep);
+                        const int exponent = max(-110, min(126, (int)(__float_as_uint(top) >> 23) - 127));
+                        shift = __uint_as_float((uint32_t)(127 + kLargest - exponent) << 23);
+                        keep = keep * shift * was;
+                    };
+#pragma unroll
+                    for (int r = 0; r < kHalves; ++r) {
+                        raise(top_of(fabsf(wv[r][0].x), fabsf(wv[r][1].x)), keep[r][0], shift[r].x);
+                        raise(top_of(fabsf(wv[r][0].y), fabsf(wv[r][1].y)), keep[r][1], shift[r].y);
                     }
                 }
 #pragma unroll
                 for (int r = 0; r < kHalves; ++r)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float top = fmaxf(s[r][e], s[r][e + 2]);
+                    for (int e = 0; e < 2; ++e)
 #pragma unroll
-                        for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-                        float to = top - kLift;
-                        if (top - to > kLift + kSlack) to = top;        // where fp32 no longer resolves kLift
-                        to = fmaxf(base[r][e], to);
-                        const float keep = exp2_fast(base[r][e] - to);
-                        base[r][e] = to;
-                        l[r][e] *= keep;
-#pragma unroll
-                        for (int j = 0; j < D / 16; ++j) o[j][r][e] *= keep * grow, o[j][r][e + 2] *= keep * grow;
-                    }
-                weights();
+                        for (int j = 0; j < D / 16; ++j) o[j][r][e] *= keep[r][e], o[j][r][e + 2] *= keep[r][e];
             }
-            // weights as the second operand of o^T += V^T w^T: positions 2 t, 2 t + 1 (and 8 further) of head g
+            // the second operand of o^T += V^T w^T: positions 2 t, 2 t + 1 (and 8 further) of head g
             uint32_t wb[kHalves][2], rest[kHalves][2];
 #pragma unroll
             for (int r = 0; r < kHalves; ++r)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    float w0 = w[r][2 * k], w1 = w[r][2 * k + 1];
-                    l[r][0] += w0;
-                    l[r][1] += w1;
-                    if constexpr (kCoded) {
-                        const float f = vs[k] * vinv;
-                        w0 *= f, w1 *= f;
-                    }
+                    l[r] = add2(l[r], w[r][k]);
+                    const float2 v = shifted(r, k);
                     uint32_t hi, lo;
-                    split(MT(), w0, w1, &hi, &lo);
+                    split(MT(), v.x, v.y, &hi, &lo);
                     if constexpr (kTwin) {
                         wb[r][k] = transpose8(t < 2 ? hi : lo);
                     } else {
@@ -723,15 +767,16 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int row = 8 * r + 2 * t + e;
-                float sum = l[r][e];
+                float sum = e ? l[r].y : l[r].x;
 #pragma unroll
                 for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-                if (g == 0) jm[warp][row] = base[r][e], jl[warp][row] = sum;
+                if (g == 0) jm[warp][row] = e ? -back[r].y : -back[r].x, jl[warp][row] = sum;
                 if constexpr (kCoded) {
+                    const float down = inverse_pow2(e ? shift[r].y : shift[r].x);
 #pragma unroll
                     for (int j = 0; j < D / 16; j += 2)
                         *reinterpret_cast<float4*>(mine + at(row, g * (D / 8) + 2 * j)) =
-                            make_float4(o[j][r][e] * vtop, o[j][r][e + 2] * vtop, o[j + 1][r][e] * vtop, o[j + 1][r][e + 2] * vtop);
+                            make_float4(o[j][r][e] * down, o[j][r][e + 2] * down, o[j + 1][r][e] * down, o[j + 1][r][e + 2] * down);
                 } else {
 #pragma unroll
                     for (int j = 0; j < D / 16; ++j) {

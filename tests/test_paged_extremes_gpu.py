@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from test_paged_gpu import (BF16, DEV, E4M3, EPS, F16, F32, I8, TINY, TYPES, U, assert_turned, attention_case, check_attention, gen,
-                            randn, status)
+                            randn, status, values64)
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +91,45 @@ def test_scores_of_any_size(dtype, kv, special, width):
                 # codes: 127 * (1 / 127) and the sum of D products are off by 2 U each at the most
                 assert ((lse[i].double() - level).abs() <= (m / 16 + 64) * 2 * U + 12 * U * (1 + abs(level))).all(), (power, sign, i)
     assert status() == 0
+
+
+@pytest.mark.parametrize('dtype,kv', [(F16, I8), (BF16, I8), (F16, E4M3), (BF16, E4M3)])
+@pytest.mark.parametrize('h,hkv', [(8, 2), (5, 1), (40, 2)])
+@pytest.mark.parametrize('ratio', [16, 24, 40, 60, 100])
+@pytest.mark.parametrize('where', ['first', 'middle', 'last'])
+def test_a_large_scale_of_no_weight_takes_nothing_from_the_others(dtype, kv, h, hkv, ratio, where):
+    """One row of V a step of 2^ratio above the rest, its score so far below (ratio ln 2 + 20) that it adds e^-20 of the sum:
+    the others keep the bits of their weights.
+
+    Beside what check_attention counts: a head's products of weight and scale are kept times a power of two that leaves the
+    largest of them, P, at 2^8 or more, as two fp16 numbers, the second of which has steps of 2^-24: half a step is 2^-33 P
+    for each position, times its code.  (It shows in a channel where the row that has all of the weight has a code of 0.)"""
+    from kairos_b200 import ops
+    lens = [300, 70, 1000]
+    c, q, table, n = attention_case(dtype, kv, lens, h, hkv, 64, 16, seed=4)
+    q[..., 0] = 4
+    top = {I8: 127.0, E4M3: 448.0}[kv]
+    low = torch.zeros(64, device=DEV)
+    low[0] = -top
+    for i, m in enumerate(lens):
+        j = {'first': 0, 'middle': m // 2 + 3, 'last': m - 1}[where]
+        page, at = table[i, j // 16].item(), j % 16
+        c.k[0, page, :, at].view(torch.uint8).copy_(low.to(kv).view(torch.uint8).expand(hkv, -1))
+        c.k_scale[0, page, :, at] = (ratio * math.log(2) + 20) / (4 * top)
+        c.v_scale[0, page, :, at] *= 2.0 ** ratio
+    got, lse = ops.paged_attention(q, c, table, n, scale=1.0, return_lse=True)
+    codes, (k64, _) = c.v[0].float().double(), values64(c)
+    for i, m in enumerate(lens):
+        at = torch.arange(m, device=DEV)
+        pages = table[i].long()[at // 16]
+        k, code, scale = (x[pages, :, at % 16].repeat_interleave(h // hkv, 1) for x in (k64, codes, c.v_scale[0].double()))
+        s = torch.einsum('hd,nhd->hn', q[i].double(), k)
+        p = torch.softmax(s, -1) * scale.t()                                    # products [H, n]
+        ref, size = torch.einsum('hn,nhd->hd', p, code), torch.einsum('hn,nhd->hd', p, code.abs())
+        ds = torch.einsum('hd,nhd->hn', q[i].double().abs(), k.abs()).amax(-1) * 72 * 2 * U
+        add = (m / 16 + 64) * 2 * U
+        tol = EPS[dtype] * ref.abs() + TINY[dtype] + size * (2 * ds[:, None] + add + 8 * U + 2.0 ** -16) + \
+            2.0 ** -33 * p.amax(-1)[:, None] * code.abs().sum(0)
+        assert ((got[i].double() - ref).abs() <= tol).all(), (i, ((got[i].double() - ref).abs() / tol).max().item())
+        level = torch.logsumexp(s, -1)
+        assert ((lse[i].double() - level).abs() <= ds + add + 8 * U * (1 + level.abs())).all()
