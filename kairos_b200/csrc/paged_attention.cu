@@ -39,9 +39,14 @@ int* device_status_word();   // api.cu
 constexpr int kWarps = 4;
 constexpr int kSub = 16;                    // positions of a stage
 constexpr int kTile = kSub * kWarps;        // positions per scheduling tile
-// Weights are kept times 2^kLift and pass the reference by 2^kSlack at the most, so that they stay below 2^15, and fp16's
-// smallest step is 2^-30 of a weight at the reference.
-constexpr float kLift = 6.f, kSlack = 8.f, kMost = 16384.f;         // kMost = 2^(kLift + kSlack)
+// Weights are kept times 2^lift and pass the reference by 2^kSlack at the most.  Over fp16 rows they are fp16 numbers themselves:
+// below 2^15, and the smallest step is 2^-30 of a weight at the reference.  Over bf16 rows and codes nothing but fp32 bounds
+// them, and they are kept small instead, so that sums of values up to bf16's largest stay finite.
+constexpr float kSlack = 8.f;
+template <typename QT, bool kCoded>
+constexpr float kLiftOf = !kCoded && std::is_same<QT, __half>::value ? 6.f : -16.f;
+template <typename QT, bool kCoded>
+constexpr float kMostOf = !kCoded && std::is_same<QT, __half>::value ? 16384.f : 1.f / 256.f;      // 2^(lift + kSlack)
 // Reference of a head before its first score: any score passes it.  References are finite, so that differences of two are
 // never NaN; a head that has seen no score has a sum of 0.
 constexpr float kUnset = -FLT_MAX;
@@ -343,6 +348,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
     using MT = typename std::conditional<kCoded, __half, QT>::type;
     using R = Ring<D, kCoded, kHalves>;
     constexpr int kHeads = 8 * kHalves;
+    constexpr float kLift = kLiftOf<QT, kCoded>, kMost = kMostOf<QT, kCoded>;
     extern __shared__ __align__(128) uint8_t dynamic[];
     uint8_t* const smem = dynamic + ((0u - smem_u32(dynamic)) & (R::kRowBytes - 1));
     __shared__ float jm[kWarps][kHeads], jl[kWarps][kHeads];
@@ -556,10 +562,10 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
         // o[j][r]: channels 16 j + g and + 8 (coded: g * D / 8 + 2 j and + 1) of heads 2 t, 2 t + 1 (+ 8 r)
         float o[D / 16][kHalves][4] = {};
         // l and o are sums of weights 2^(s + back); heads 2 t and 2 t + 1.  Coded: the power of two that products are kept times,
-        // at first 2^122
+        // at first 2^126
         float2 back[kHalves], l[kHalves], shift[kHalves];
 #pragma unroll
-        for (int r = 0; r < kHalves; ++r) back[r] = both(-kUnset), l[r] = both(0.f), shift[r] = both(5.316911983139664e36f);
+        for (int r = 0; r < kHalves; ++r) back[r] = both(-kUnset), l[r] = both(0.f), shift[r] = both(8.507059173023462e37f);
 
 #pragma unroll 1
         for (int pos = k0; pos < k1; pos += stride) {
@@ -678,7 +684,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
                         // never above the largest product so far, as the new reference leaves it
                         const float was = inverse_pow2(shift);
                         top = fmaxf(top, was * (float)(1 << kLargest) * keep);
-                        const int exponent = max(-110, min(126, (int)(__float_as_uint(top) >> 23) - 127));
+                        const int exponent = max(-118, min(126, (int)(__float_as_uint(top) >> 23) - 127));
                         shift = __uint_as_float((uint32_t)(127 + kLargest - exponent) << 23);
                         keep = keep * shift * was;
                     };

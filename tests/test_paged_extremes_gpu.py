@@ -133,3 +133,22 @@ def test_a_large_scale_of_no_weight_takes_nothing_from_the_others(dtype, kv, h, 
         assert ((got[i].double() - ref).abs() <= tol).all(), (i, ((got[i].double() - ref).abs() / tol).max().item())
         level = torch.logsumexp(s, -1)
         assert ((lse[i].double() - level).abs() <= ds + add + 8 * U * (1 + level.abs())).all()
+
+
+@pytest.mark.parametrize('kv', [BF16, I8, E4M3])
+@pytest.mark.parametrize('power', [121, 110, 60, -60, -80])
+@pytest.mark.parametrize('width', [0, 2000])
+def test_values_near_the_ends_of_bf16(kv, power, width):
+    """Values up to 2^125 and down to 2^-80: weighted sums of them stay inside fp32."""
+    from kairos_b200 import ops
+    lens = [300, 1, 40, 1500]
+    c, q, table, n = attention_case(BF16, kv, lens, 8, 2, 64, 16, seed=4)
+    seen = torch.isfinite(c.v.float()).all(-1) if c.v_scale is None else torch.isfinite(c.v_scale)
+    if c.v_scale is None:
+        c.v[seen] *= 2.0 ** power
+    else:
+        c.v_scale[seen] *= 2.0 ** power
+    wide = torch.full((4, max(width, table.shape[1])), -1, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    got = ops.paged_attention(q, c, wide, n)
+    check_attention(c, q, table, lens, got)
