@@ -39,14 +39,15 @@ int* device_status_word();   // api.cu
 constexpr int kWarps = 4;
 constexpr int kSub = 16;                    // positions of a stage
 constexpr int kTile = kSub * kWarps;        // positions per scheduling tile
-// Weights are kept times 2^lift and pass the reference by 2^kSlack at the most.  Over fp16 rows they are fp16 numbers themselves:
-// below 2^15, and the smallest step is 2^-30 of a weight at the reference.  Over bf16 rows and codes nothing but fp32 bounds
-// them, and they are kept small instead, so that sums of values up to bf16's largest stay finite.
-constexpr float kSlack = 8.f;
-template <typename QT, bool kCoded>
-constexpr float kLiftOf = !kCoded && std::is_same<QT, __half>::value ? 6.f : -16.f;
-template <typename QT, bool kCoded>
-constexpr float kMostOf = !kCoded && std::is_same<QT, __half>::value ? 16384.f : 1.f / 256.f;      // 2^(lift + kSlack)
+// Weights are kept times 2^lift and pass the reference by 2^slack at the most.  Over fp16 rows they are fp16 numbers themselves
+// and stay below 2^15; the smallest step is 2^-36 of a weight at the reference (a slack of 2^8 and steps of 2^-30 measure the
+// same within 0.2%).  Over bf16 rows and codes nothing but fp32 bounds them, and they are kept small instead, so that sums of
+// values up to bf16's largest stay finite.
+template <bool kHalfRows>
+struct Span {
+    static constexpr float kLift = kHalfRows ? 12.f : -16.f, kSlack = kHalfRows ? 3.f : 8.f;
+    static constexpr float kMost = kHalfRows ? 32768.f : 1.f / 256.f;      // 2^(lift + slack)
+};
 // Reference of a head before its first score: any score passes it.  References are finite, so that differences of two are
 // never NaN; a head that has seen no score has a sum of 0.
 constexpr float kUnset = -FLT_MAX;
@@ -348,7 +349,8 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
     using MT = typename std::conditional<kCoded, __half, QT>::type;
     using R = Ring<D, kCoded, kHalves>;
     constexpr int kHeads = 8 * kHalves;
-    constexpr float kLift = kLiftOf<QT, kCoded>, kMost = kMostOf<QT, kCoded>;
+    using W = Span<!kCoded && std::is_same<QT, __half>::value>;
+    constexpr float kLift = W::kLift, kSlack = W::kSlack, kMost = W::kMost;
     extern __shared__ __align__(128) uint8_t dynamic[];
     uint8_t* const smem = dynamic + ((0u - smem_u32(dynamic)) & (R::kRowBytes - 1));
     __shared__ float jm[kWarps][kHeads], jl[kWarps][kHeads];

@@ -152,3 +152,31 @@ def test_values_near_the_ends_of_bf16(kv, power, width):
     wide[:, :table.shape[1]] = table
     got = ops.paged_attention(q, c, wide, n)
     check_attention(c, q, table, lens, got)
+
+
+@pytest.mark.parametrize('h,hkv', [(8, 1), (4, 1), (16, 1)])
+@pytest.mark.parametrize('gap', [10.0, 18.0, 22.0])
+def test_small_weights_over_fp16_rows_beside_a_large_one(h, hkv, gap):
+    """One position with all but e^-gap of the weight and values of zero: what the others add is held to 2^-37 of the largest
+    weight for each of them (the halves of a weight are fp16 numbers, 2^12 at the reference, which is within 2^3 of the
+    largest), beside the errors that check_attention counts."""
+    from kairos_b200 import ops
+    m = 5000
+    c, q, table, n = attention_case(F16, F16, [m], h, hkv, 64, 16, seed=4)
+    q.zero_()
+    q[..., 0] = 1
+    at = torch.arange(m, device=DEV)
+    pages = table[0].long()[at // 16]
+    c.k[0, pages, :, at % 16] = 0
+    c.v[0, pages, :, at % 16] = c.v[0, pages, :, at % 16].abs() * 1024
+    c.k[0, pages[7], :, 7, 0] = gap
+    c.v[0, pages[7], :, 7] = 0
+    got = ops.paged_attention(q, c, table, n, scale=1.0)
+    v = c.v[0, pages, :, at % 16].double()
+    s = torch.zeros(m, dtype=torch.float64, device=DEV)
+    s[7] = gap
+    p = torch.softmax(s, 0)
+    ref = torch.einsum('n,nhd->hd', p, v)
+    tol = EPS[F16] * ref + TINY[F16] + ref * (2 * gap * 72 * 2 * U + (m / 16 + 64) * 2 * U + 8 * U + 2.0 ** -16) + \
+        2.0 ** -37 * v.sum(0) * p.max()
+    assert ((got[0].view(hkv, h, 64).double() - ref[:, None]).abs() <= tol[:, None]).all()
