@@ -275,11 +275,16 @@ int kairos_paged_kv_read(const kairos_kv_layer* kv, const void* slots, void* K_o
                          kairos_stream_t stream);
 /* Attention of one new token per sequence: O[b,h,:] = sum_j softmax_j(scale * Q[b,h,:] . K[j,:]) V[j,:] over the
  * sequence's lens[b] positions, position j at offset j % page_size of page page_table[b, j / page_size].
- * Q [B, H, D] F16 / BF16 with element strides {b, h} (multiples of 8); O dense [B, H, D] of the same type (it may be Q); a 16-bit cache has Q's
- * type.  table_width * page_size <= 2^30 and H % kv_heads == 0 (head h reads kv head h / (H / kv_heads)).  LSE [B, H] fp32 (natural logarithm of the
- * softmax's denominator) when not null.  lens[b] <= 0: O = 0, LSE = -inf.  Entries of the table behind the end may
- * hold anything.  A page outside the pool is left out of the sum (a row that is left with no position is an empty one: O = 0,
- * LSE = -inf), lens[b] is cut to table_width * page_size, and both raise the status word (KAIROS_ERR_ARG).  Scores, softmax sums and outputs are accumulated in fp32.
+ * Q [B, H, D] F16 / BF16 with element strides {b, h} (multiples of 8); O dense [B, H, D] of the same type (it may be Q); a
+ * 16-bit cache has Q's type.  table_width * page_size <= 2^30 and H % kv_heads == 0 (head h reads kv head
+ * h / (H / kv_heads)).  LSE [B, H] fp32 (natural logarithm of the softmax's denominator) when not null.  lens[b] <= 0:
+ * O = 0, LSE = -inf.  Entries of the table behind the end may hold anything.  A page outside the pool is left out of the
+ * sum (a row that is left with no position is an empty one: O = 0, LSE = -inf), lens[b] is cut to
+ * table_width * page_size, and both raise the status word (KAIROS_ERR_ARG).
+ * Scores, softmax sums and outputs are accumulated in fp32.  The weight that multiplies a row of V is held in two 16-bit
+ * numbers: to 2^-16 of itself over BF16 rows; to 2^-22 of itself or 2^-37 of the head's largest weight, whichever is more,
+ * over F16 rows; over codes weight times V scale is, to 2^-22 of itself or 2^-33 of the largest such product.  BF16 queries
+ * over codes are held to 2^-38 of the head's largest value.
  * `workspace` of kairos_paged_attention_workspace_bytes() is scratch of this call alone (contents need no
  * initialisation): calls that may overlap need workspaces of their own. */
 size_t kairos_paged_attention_workspace_bytes(const kairos_kv_layer* kv, int B, int H, int table_width);

@@ -23,10 +23,14 @@
 // 400 warp instructions per 16 positions, 176 of them widening codes, take 63% of the issue slots.  Rows of 64 int8 channels,
 // half the bytes for more than half the instructions, reach 5.4 TB/s (128 sequences of 8192: 210 us).
 //
-// Precision.  Scores, maxima, sums and outputs are fp32.  The weights enter the second product as TWO 16-bit numbers
-// (value and remainder): rounding them to 16 bits alone would add an error as large as the output's own rounding.
-// The reference m of the exponent need not be the maximum: it moves (and o and l are rescaled) only when a score
-// passes it by 2^kSlack, so most stages need neither a reduction over lanes nor a rescaling.
+// Precision.  Scores, references, sums and outputs are fp32.  What has fewer bits, since tensor instructions take 16-bit
+// operands, and why that is enough beside an output of 11 (fp16) or 8 bits (bf16):
+//   * the weights of the second product (over codes: weight times V scale) are TWO 16-bit numbers, value and remainder; one alone
+//     would add an error as large as the output's own rounding.  Over bf16 rows they are off by 2^-16 of each weight; over fp16 rows
+//     2^-22 of each, but no less than 2^-37 of the head's largest; over codes the same with 2^-33 of the largest product;
+//   * bf16 queries over codes become fp16 times a power of two per head: exact to 2^-38 of the head's largest value.
+// Exponentials are ex2.approx (2 U); an argument below -126 gives 0.  The reference need not be the maximum: it moves (and o and
+// l are rescaled) only when a score passes it by 2^slack, so most stages need neither a reduction over lanes nor a rescaling.
 #include <cfloat>
 #include <type_traits>
 
