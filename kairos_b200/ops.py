@@ -306,10 +306,51 @@ def _bad(t, name, want, index):
                       f'on {t.device}')
 
 
+def _rows(shape, strides):
+    """Where the rows of a tensor with a dense last dimension begin, in elements, in ascending order."""
+    at = torch.zeros(1, dtype=_int64)
+    for n, step in zip(shape[:-1], strides[:-1]):
+        at = (at[:, None] + torch.arange(n) * step).flatten()
+    return at.sort().values
+
+
+def _distinct(shape, strides):
+    """Whether every element of a tensor with a dense last dimension has a place of its own.  It has if each dimension steps
+    over all that the smaller ones reach; else the rows' places decide."""
+    reach = 0
+    for step, n in sorted((step, n) for step, n in zip(strides, shape) if n > 1):
+        if step <= reach:
+            return bool((_rows(shape, strides).diff() >= shape[-1]).all())
+        reach += (n - 1) * step
+    return True
+
+
+def _disjoint(shape, a, b, offset):
+    """Whether a tensor of strides `a` and one of strides `b` that begins `offset` elements behind it, both with a dense last
+    dimension, have no element in common."""
+    if 0 in shape:
+        return True
+    ends = [sum((n - 1) * step for n, step in zip(shape, strides)) for strides in (a, b)]
+    if offset > ends[0] or -offset > ends[1]:
+        return True
+    dims = sorted((step, n) for step, n in zip(a, shape) if n > 1)
+    if dims and dims == sorted((step, n) for step, n in zip(b, shape) if n > 1):
+        # slices of one activation: both stay within a part of each step of the largest dimension
+        step, reach = dims[-1][0], sum((n - 1) * step for step, n in dims[:-1])
+        if step and reach < offset % step < step - reach:
+            return True
+    first, second = _rows(shape, a), _rows(shape, b) + offset
+    near = torch.searchsorted(first, second)                  # the rows of `a` on either side of each row of `b`
+    behind = first[near.clamp(max=len(first) - 1)] - second
+    before = second - first[(near - 1).clamp(min=0)]
+    d = shape[-1]
+    return not bool((((near < len(first)) & (behind < d)) | ((near > 0) & (before < d))).any())
+
+
 def rotary(x, positions, rotary, transpose=False, out=None):
     """Heads [T, H, D] or [B, S, H, D] (fp16, bf16 or fp32; dense last dimension, any other strides) turned by their
     int64 positions, [T] or broadcastable to [B, S], with the plan of a :class:`Rotary`.  ``transpose`` turns back with the same
-    magnitude: the gradient of x from that of the result.  ``out`` may be x."""
+    magnitude: the gradient of x from that of the result.  ``out`` may be x, and must not overlap it otherwise."""
     shape, strides, code, index = x.shape, x.stride(), _FLOATS.get(x.dtype), x.get_device()
     dims = len(shape)
     if code is None or not 3 <= dims <= 4 or shape[-1] != rotary.head_dim or strides[-1] != 1:
@@ -321,8 +362,12 @@ def rotary(x, positions, rotary, transpose=False, out=None):
     if out is None:
         out = torch.empty_like(x)
     elif out.shape != shape or out.dtype != x.dtype or out.get_device() != index or out.stride(-1) != 1 or \
-            any(step == 0 and n > 1 for step, n in zip(out.stride(), shape)):
+            not _distinct(shape, out.stride()):
         raise _bad(out, 'out', f'{x.dtype} {tuple(shape)} with a dense last dimension and a place for every element', index)
+    elif out is not x and not (out.data_ptr() == x.data_ptr() and
+                               all(a == b or n == 1 for a, b, n in zip(out.stride(), strides, shape))) and \
+            not _disjoint(shape, strides, out.stride(), (out.data_ptr() - x.data_ptr()) // x.element_size()):
+        raise ValueError('out: overlaps x without being it')
     to, at = out.stride(), positions
     if dims == 3:
         b, xb, yb, pb, (s, h, d) = 1, 0, 0, 0, shape

@@ -203,3 +203,33 @@ def test_pages_of_a_sequence_are_a_copy():
     assert held == c.page_table(['a'])[0].tolist() and len(held) == 2
     held.append(5)
     assert len(c.pages('a')) == 2 and c.free_pages == 4
+
+
+# ---- results that would overlap ----------------------------------------------------------------------
+LAYOUTS = [((3, 2, 4), (8, 4, 1)), ((3, 2, 4), (0, 4, 1)), ((3, 2, 4), (8, 2, 1)), ((3, 2, 4), (4, 12, 1)), ((3, 2, 4), (4, 4, 1)),
+           ((2, 3, 4), (12, 4, 1)), ((2, 3, 4), (6, 4, 1)), ((3, 2, 2), (4, 6, 1)), ((3, 2, 2), (3, 2, 1)), ((1, 2, 4), (0, 4, 1)),
+           ((2, 3, 2, 4), (40, 8, 4, 1)), ((2, 3, 2, 4), (24, 4, 12, 1)), ((2, 3, 2, 4), (4, 8, 24, 1)), ((0, 2, 4), (0, 0, 1)),
+           ((2, 2, 1), (2, 1, 1)), ((2, 2, 1), (1, 1, 1))]
+
+
+def elements(shape, strides, offset=0):
+    at = [offset]
+    for n, step in zip(shape, strides):
+        at = [a + i * step for a in at for i in range(n)]
+    return at
+
+
+@pytest.mark.parametrize('shape,strides', LAYOUTS)
+def test_results_whose_elements_share_a_place(shape, strides):
+    at = elements(shape, strides)
+    assert ops._distinct(shape, strides) == (len(set(at)) == len(at))
+
+
+@pytest.mark.parametrize('shape,strides', [x for x in LAYOUTS if 0 not in x[0]])
+def test_results_that_overlap_their_input(shape, strides):
+    for s, other in LAYOUTS:
+        if s != shape:
+            continue
+        first = set(elements(shape, strides))
+        for offset in range(-70, 71):
+            assert ops._disjoint(shape, strides, other, offset) == first.isdisjoint(elements(shape, other, offset)), (other, offset)

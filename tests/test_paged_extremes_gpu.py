@@ -180,3 +180,24 @@ def test_small_weights_over_fp16_rows_beside_a_large_one(h, hkv, gap):
     tol = EPS[F16] * ref + TINY[F16] + ref * (2 * gap * 72 * 2 * U + (m / 16 + 64) * 2 * U + 8 * U + 2.0 ** -16) + \
         2.0 ** -37 * v.sum(0) * p.max()
     assert ((got[0].view(hkv, h, 64).double() - ref[:, None]).abs() <= tol[:, None]).all()
+
+
+def test_rotary_refuses_results_that_overlap():
+    import kairos_b200 as kb
+    from kairos_b200 import ops
+    r, pos = kb.Rotary(64), torch.arange(5, device=DEV)
+    flat = randn((5 * 40 * 64,), 1)
+    x = flat.as_strided((5, 3, 64), (40 * 64, 64, 1))
+    for out in (flat.as_strided((5, 3, 64), (40 * 64, 32, 1)), flat.as_strided((5, 3, 64), (64, 64, 1)),
+                flat[8:].as_strided((5, 3, 64), (40 * 64, 64, 1)), flat[128:].as_strided((5, 3, 64), (40 * 64, 64, 1)),
+                flat.as_strided((5, 3, 64), (40 * 64, 128, 1)), flat[576:].as_strided((5, 3, 64), (8 * 64, 64, 1))):
+        kept = flat.clone()
+        with pytest.raises(ValueError):
+            ops.rotary(x, pos, r, out=out)
+        assert torch.equal(flat, kept)
+    # beside x in the same rows, in the gaps between them (320 + 512 k .. 192 further ends at 2560, where x goes on), and x itself
+    # by another view
+    for out in (flat[320:].as_strided((5, 3, 64), (8 * 64, 64, 1)), flat[192:].as_strided((5, 3, 64), (40 * 64, 64, 1)), flat[20 * 64:].as_strided((5, 3, 64), (40 * 64, 256, 1)), x[:]):
+        kept = x.clone()
+        assert ops.rotary(x, pos, r, out=out) is out
+        assert_turned(out, kept, pos, r)
