@@ -201,3 +201,30 @@ def test_rotary_refuses_results_that_overlap():
         kept = x.clone()
         assert ops.rotary(x, pos, r, out=out) is out
         assert_turned(out, kept, pos, r)
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16, F32])
+def test_rotary_into_a_result_of_other_strides(dtype):
+    """x and the result have strides of their own, in 16-byte and in element-wise accesses; what lies around the result stays."""
+    import kairos_b200 as kb
+    from kairos_b200 import ops
+    r = kb.Rotary(64, 48, layout='interleaved')
+    wide = randn((4, 9, 12, 64), 1, dtype)
+    odd = randn((4, 9, 12, 65), 2, dtype)
+    for x in (wide[:, :, 2:9], wide.transpose(1, 2)[:, :9, :7], odd[..., 1:][:, :, 2:9], wide[:, ::1, ::2][:, :, :5]):
+        b, s, h, _ = x.shape
+        pos = torch.randint(0, 9999, (b, s), generator=gen(3), device=DEV)
+        for room, view in ((torch.empty((s, h, b, 64), device=DEV), lambda t: t.permute(2, 0, 1, 3)),
+                           (torch.empty((b, s + 2, h + 3, 64 + 16), device=DEV), lambda t: t[:, 1:-1, 2:-1, 8:72]),
+                           (torch.empty((b, h, s, 64 + 3), device=DEV), lambda t: t.transpose(1, 2)[..., 1:65]),
+                           (torch.empty((b * 3, s * 2, h, 64), device=DEV), lambda t: t[1::3, ::2])):
+            room = torch.full_like(room, 7, dtype=dtype)
+            out, kept = view(room), room.clone()
+            assert ops.rotary(x, pos, r, out=out) is out
+            assert_turned(out, x, pos, r)
+            view(kept).copy_(out)
+            assert torch.equal(room, kept)
+        if b > 1:
+            three = torch.full((s, 2 * h, 64), 7, dtype=dtype, device=DEV)                     # [T, H, D]
+            assert_turned(ops.rotary(x[1], pos[1], r, out=three[:, 1::2]), x[1], pos[1], r)
+            assert (three[:, ::2] == 7).all()
