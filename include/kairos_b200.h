@@ -254,9 +254,9 @@ typedef struct {
 } kairos_rotary_plan;
 /* Y[b,s,h,:] = turned X[b,s,h,:]; X and Y are F16 / BF16 / F32 with element strides {b, s, h} and a dense last
  * dimension (D <= 512); Y may be X, must not overlap it otherwise, and no two of its elements share a place.  positions:
- * int64 with element strides {b, s} (0 broadcasts).  transpose != 0
- * turns the other way with the same magnitude: the transposed operator, i.e. the gradient of X from that of Y.
- * Rows that are 16-byte aligned with D % 16 == 0 and rot % 16 == 0 move in 16-byte accesses, others element-wise. */
+ * int64 with element strides {b, s} (0 broadcasts).  transpose != 0 turns the other way with the same magnitude: the
+ * transposed operator, i.e. the gradient of X from that of Y.  Rows that are 16-byte aligned with D % 16 == 0 and
+ * rot % 16 == 0 move in 16-byte accesses, others element-wise. */
 int kairos_rotary(const void* X, long long x_b, long long x_s, long long x_h, void* Y, long long y_b, long long y_s,
                   long long y_h, const void* positions, long long pos_b, long long pos_s, const kairos_rotary_plan* plan,
                   int dtype, int transpose, int B, int S, int H, int D, kairos_stream_t stream);

@@ -361,6 +361,8 @@ def rotary(x, positions, rotary, transpose=False, out=None):
         raise _bad(positions, 'positions', 'int64', index)
     if out is None:
         out = torch.empty_like(x)
+        if out.stride(-1) != 1:                 # overlapping windows: another dimension came out as the dense one
+            out = x.new_empty(shape)
     elif out.shape != shape or out.dtype != x.dtype or out.get_device() != index or out.stride(-1) != 1 or \
             not _distinct(shape, out.stride()):
         raise _bad(out, 'out', f'{x.dtype} {tuple(shape)} with a dense last dimension and a place for every element', index)

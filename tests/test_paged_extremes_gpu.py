@@ -228,3 +228,19 @@ def test_rotary_into_a_result_of_other_strides(dtype):
             three = torch.full((s, 2 * h, 64), 7, dtype=dtype, device=DEV)                     # [T, H, D]
             assert_turned(ops.rotary(x[1], pos[1], r, out=three[:, 1::2]), x[1], pos[1], r)
             assert (three[:, ::2] == 7).all()
+
+
+def test_rotary_of_overlapping_windows():
+    """An input whose heads are windows of one row, a step of one element apart: more heads than channels, so that a result
+    allocated after the input's strides would not have a dense last dimension."""
+    import kairos_b200 as kb
+    from kairos_b200 import ops
+    r = kb.Rotary(64)
+    for dtype in (F16, F32):
+        flat = randn((3000,), 1, dtype)
+        for shape, strides in (((2, 200, 64), (300, 1, 1)), ((3, 7, 4, 64), (1, 0, 300, 1)), ((100, 7, 1, 64), (1, 0, 300, 1))):
+            x = flat.as_strided(shape, strides)
+            pos = torch.randint(0, 999, shape[:-2], generator=gen(3), device=DEV)
+            got = ops.rotary(x, pos, r)
+            assert got.stride(-1) == 1
+            assert_turned(got, x, pos, r)
