@@ -243,9 +243,10 @@ typedef struct {
 /* Rotary positions.  Pair i of the first `rot` channels of a head (channels i and i + rot / 2 in layout 0, "half";
  * 2 i and 2 i + 1 in layout 1, "interleaved") is turned by position * f_i and multiplied by `magnitude`; the
  * channels behind `rot` pass unchanged.  f_i is given as a binary fraction of a full turn:
- * steps[i] = round(f_i / (2 pi) * 2^64), uint64 in device memory.  position * step modulo 2^64 IS the angle, so a
- * position of any size (negative ones included) has an angle that is exact to 2^-32 turns: no table, no far-position
- * error. */
+ * steps[i] = round(f_i / (2 pi) * 2^64), uint64 in device memory.  position * step modulo 2^64 is the angle of a position of
+ * any size (negative ones included), with no reduction that could lose it: off by 2^-32 turns at the most for the bits that
+ * are dropped, and by 2^-65 turns for each position for the step's own rounding (2^-32 turns at 2^33, where the step is
+ * rounded from more digits than a 64-bit float has). */
 typedef struct {
     const void* steps; /* uint64 [rot / 2] */
     float magnitude;

@@ -36,7 +36,7 @@ __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bf
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 
 // cos and sin of position * step, step being a binary fraction of a full turn (2^64 = one turn).  The product
-// modulo 2^64 is the angle without any rounding, however far the position.  Its upper 32 bits split into the nearest
+// modulo 2^64 is the angle without any rounding but the step's own (2^-65 turns for each position).  Its upper 32 bits split into the nearest
 // quarter turn and a signed rest of at most an eighth of a turn, whose sine and cosine are their Taylor series to x^9 and
 // x^8: what is left out is below 1.8e-9 and 2.5e-8 at pi / 4, under the half step 3e-8 of fp32.  Dropping the lower
 // 32 bits moves the angle by less than 1.5e-9.  A third of the instructions of a general sine and cosine, which has to

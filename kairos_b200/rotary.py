@@ -3,12 +3,17 @@ from __future__ import annotations
 
 import ctypes
 import math
+from decimal import Context, Decimal, localcontext
 
 import torch
 
 from ._lib import RotaryPlan
 
 LAYOUTS = {'half': 0, 'interleaved': 1}
+# Frequencies are computed with 50 decimal digits: a step of the kernels is a fraction of 64 bits that far positions multiply, so
+# 64-bit floats would leave 2^-56 turns a position in the fast pairs.
+_DIGITS = Context(prec=50)
+_TWO_PI = 2 * Decimal('3.14159265358979323846264338327950288419716939937510582097')
 
 
 class Rotary:
@@ -25,8 +30,8 @@ class Rotary:
                 Peng et al., "YaRN: efficient context window extension of large language models" (2023): a ramp over
                 the pair index between the two, and a magnitude on the turned channels.
 
-    `frequencies` holds the radians per position of every pair (float64).  The kernels take them as 64-bit binary
-    fractions of a turn, so no angle loses precision with the position."""
+    `frequencies` holds the radians per position of every pair (float64).  The kernels take them as 64-bit binary fractions of
+    a turn, rounded from 50 digits: an angle is off by 2^-65 turns for each position (2^-32 turns at position 2^33)."""
 
     def __init__(self, head_dim, rot_dim=None, theta=10000.0, layout='half', scaling=None, device='cuda'):
         rot = head_dim if rot_dim is None else rot_dim
@@ -34,11 +39,13 @@ class Rotary:
             raise ValueError(f'rot_dim must be even and between 2 and the head dimension {head_dim}, got {rot}')
         if layout not in LAYOUTS:
             raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
-        if not theta > 1:
+        if not 1 < theta < math.inf:
             raise ValueError(f'theta must be above 1, got {theta}')
         self.head_dim, self.rot_dim, self.layout, self.theta = head_dim, rot, layout, float(theta)
-        self.frequencies, self.magnitude = self._scaled(rot, float(theta), scaling)
-        turns = [int(round(f / (2 * math.pi) * 2.0 ** 64)) % (1 << 64) for f in self.frequencies.tolist()]
+        with localcontext(_DIGITS):
+            exact, self.magnitude = self._scaled(rot, float(theta), scaling)
+            turns = [round(f / _TWO_PI * (1 << 64)) % (1 << 64) for f in exact]
+        self.frequencies = torch.tensor([float(f) for f in exact], dtype=torch.float64)
         signed = [t - (1 << 64) if t >= 1 << 63 else t for t in turns]
         self.steps = torch.tensor(signed, dtype=torch.int64, device=device)
         self.index = self.steps.get_device() if self.steps.is_cuda else -1
@@ -47,14 +54,20 @@ class Rotary:
 
     @staticmethod
     def _scaled(rot, theta, scaling):
-        pair = torch.arange(rot // 2, dtype=torch.float64)
-        freq = theta ** (-2.0 * pair / rot)
+        def power(base):          # base^(-2 i / rot) for every pair i
+            each, powers = (-2 * base.ln() / rot).exp(), [Decimal(1)]
+            while len(powers) < rot // 2:
+                powers.append(powers[-1] * each)
+            return powers
+
+        freq = power(Decimal(theta))
         if scaling is None:
             return freq, 1.0
         opt = dict(scaling)
         kind, factor = opt.pop('type', None), float(opt.pop('factor', 0.0))
-        if not factor >= 1:
+        if not 1 <= factor < math.inf:
             raise ValueError(f'rotary scaling needs a factor of at least 1, got {factor}')
+        by = Decimal(factor)
 
         def take(name, default=None):
             value = opt.pop(name, default)
@@ -62,17 +75,19 @@ class Rotary:
                 raise ValueError(f'rotary scaling {kind!r} needs {name!r}')
             return float(value)
 
+        def blend(keep):          # keep = 1: the pair's own speed, 0: slowed by the factor
+            return [f * (k + (1 - k) / by) for f, k in zip(freq, (min(max(k, Decimal(0)), Decimal(1)) for k in keep))]
+
         magnitude = 1.0
         if kind == 'linear':
-            freq = freq / factor
+            freq = [f / by for f in freq]
         elif kind == 'ntk':
-            freq = (theta * factor ** (rot / max(2, rot - 2))) ** (-2.0 * pair / rot)
+            freq = power(Decimal(theta) * (by.ln() * rot / max(2, rot - 2)).exp())
         elif kind == 'llama3':
             trained, low, high = take('original_max'), take('low_freq_factor', 1.0), take('high_freq_factor', 4.0)
             if not high > low:
                 raise ValueError('rotary scaling: high_freq_factor must be above low_freq_factor')
-            keep = ((trained * freq / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
-            freq = freq * (keep + (1 - keep) / factor)
+            freq = blend([(Decimal(trained) * f / _TWO_PI - Decimal(low)) / (Decimal(high) - Decimal(low)) for f in freq])
         elif kind == 'yarn':
             trained, fast, slow = take('original_max'), take('beta_fast', 32.0), take('beta_slow', 1.0)
             magnitude = take('magnitude', 0.1 * math.log(factor) + 1)
@@ -80,8 +95,7 @@ class Rotary:
             def pair_of(turns):       # the pair that makes so many turns within the trained length
                 return rot * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(theta))
             lo, hi = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rot - 1)
-            ramp = ((pair - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
-            freq = freq * (1 - ramp + ramp / factor)
+            freq = blend([1 - (i - lo) / max(Decimal(hi - lo), Decimal('1e-3')) for i in range(rot // 2)])
         else:
             raise ValueError(f"rotary scaling type must be 'linear', 'ntk', 'llama3' or 'yarn', got {kind!r}")
         if opt:

@@ -2,6 +2,7 @@
 operators' argument checks and of the C entry points (which refuse before anything is launched)."""
 import ctypes
 import math
+from decimal import Context, Decimal, localcontext
 
 import pytest
 import torch
@@ -233,3 +234,52 @@ def test_results_that_overlap_their_input(shape, strides):
         first = set(elements(shape, strides))
         for offset in range(-70, 71):
             assert ops._disjoint(shape, strides, other, offset) == first.isdisjoint(elements(shape, other, offset)), (other, offset)
+
+
+# ---- the kernels' steps against the definition in 60 digits -----------------------------------------------
+def two_pi():
+    def arctan_inverse(x):                                    # of 1 / x, by its series
+        total, term, n = Decimal(0), 1 / Decimal(x), 0
+        while abs(term) > Decimal('1e-70'):
+            total += term / (2 * n + 1) * (-1) ** n
+            term, n = term / (x * x), n + 1
+        return total
+    return 8 * (4 * arctan_inverse(5) - arctan_inverse(239))  # Machin
+
+
+def frequencies60(rot, theta, scaling):
+    """Radians a position, from the definitions of the scalings."""
+    kind, s = (scaling or {}).get('type'), Decimal((scaling or {}).get('factor', 1))
+    theta = Decimal(theta)
+    if kind == 'ntk':
+        theta = theta * s ** (Decimal(rot) / max(2, rot - 2))
+    out = []
+    for i in range(rot // 2):
+        f = theta ** (Decimal(-2 * i) / rot)
+        if kind == 'linear':
+            f = f / s
+        elif kind == 'llama3':                                # trained 8192, low 1, high 4
+            wavelength = two_pi() / f
+            part = (Decimal(8192) / wavelength - 1) / 3
+            f = f if wavelength < 2048 else f / s if wavelength > 8192 else (1 - part) * f / s + part * f
+        elif kind == 'yarn':                                  # trained 32768, 32 and 1 turns
+            at = [Decimal(rot) / 2 * (32768 / (two_pi() * t)).ln() / theta.ln() for t in (32, 1)]
+            first, last = max(0, math.floor(at[0])), min(rot - 1, math.ceil(at[1]))
+            part = min(Decimal(1), max(Decimal(0), (Decimal(i) - first) / (last - first)))
+            f = part * f / s + (1 - part) * f
+        out.append(f)
+    return out
+
+
+@pytest.mark.parametrize('rot', [2, 20, 64, 128])
+@pytest.mark.parametrize('theta', [10000.0, 5e5, 1234567.891])
+@pytest.mark.parametrize('scaling', [None, dict(type='linear', factor=3), dict(type='ntk', factor=4), dict(type='llama3', factor=8, original_max=8192),
+                                     dict(type='yarn', factor=2.5, original_max=32768)])
+def test_steps_are_rounded_once(rot, theta, scaling):
+    """Half a step of 2^-64 turns, so that a far position multiplies nothing else; the frequencies half a step of fp64."""
+    with localcontext(Context(prec=60)):
+        r = kb.Rotary(128, rot, theta=theta, scaling=scaling, device='cpu')
+        for step, kept, f in zip(r.steps.tolist(), r.frequencies.tolist(), frequencies60(rot, theta, scaling)):
+            off = (step - f / two_pi() * (1 << 64)) % (1 << 64)
+            assert min(off, (1 << 64) - off) <= Decimal('0.5000001')
+            assert abs(Decimal(kept) - f) <= f * Decimal(2) ** -53

@@ -2,10 +2,12 @@
 to, scores of any size, V scales and values far apart, results in memory of another layout.  Helpers and the counting of
 roundings are those of test_paged_gpu."""
 import math
+from decimal import Context, localcontext
 
 import pytest
 import torch
 
+from test_paged_cpu import frequencies60, two_pi
 from test_paged_gpu import (BF16, DEV, E4M3, EPS, F16, F32, I8, TINY, TYPES, U, assert_turned, attention_case, check_attention, gen,
                             randn, status, values64)
 
@@ -244,3 +246,26 @@ def test_rotary_of_overlapping_windows():
             got = ops.rotary(x, pos, r)
             assert got.stride(-1) == 1
             assert_turned(got, x, pos, r)
+
+
+@pytest.mark.parametrize('scaling', [None, dict(type='linear', factor=3.0)])
+@pytest.mark.parametrize('layout', ['half', 'interleaved'])
+def test_angles_of_far_positions(scaling, layout):
+    """Against angles from theta in 60 digits, not from the plan's own steps.  Beside the fp32 errors of assert_turned (8 U) the
+    angle is off by 2^-32 turns for the bits that are dropped and 2^-65 turns for each position."""
+    import kairos_b200 as kb
+    from kairos_b200 import ops
+    r = kb.Rotary(128, theta=5e5, layout=layout, scaling=scaling)
+    places = [1, 1000, (1 << 24) + 1, (1 << 33) + 12345, -(1 << 33) - 7, (1 << 40) + 3, -(1 << 44)]
+    pos = torch.tensor(places, device=DEV)
+    x = randn((len(places), 3, 128), 1, F32)
+    with localcontext(Context(prec=60)):
+        steps = [f / two_pi() for f in frequencies60(128, 5e5, scaling)]
+        angle = torch.tensor([[float(p * f % 1) * 2 * math.pi for f in steps] for p in places], dtype=torch.float64, device=DEV)
+    c, s = torch.cos(angle)[:, None], torch.sin(angle)[:, None]
+    i = torch.arange(64, device=DEV)
+    first, second = (i, i + 64) if layout == 'half' else (2 * i, 2 * i + 1)
+    a, b = x.double()[..., first], x.double()[..., second]
+    got = ops.rotary(x, pos, r).double()
+    tol = (a.abs() + b.abs()) * (9 * U + 2 * math.pi * (2.0 ** -32 + pos.abs().double() * 2.0 ** -65))[:, None, None]
+    assert ((got[..., first] - (a * c - b * s)).abs() <= tol).all() and ((got[..., second] - (b * c + a * s)).abs() <= tol).all()
