@@ -33,7 +33,10 @@ def main():
                     help='tensor parallel: measure a second time with the small all-reduces through NCCL')
     ap.add_argument('--glue', default='cuda', choices=['cuda', 'torch'], help="'torch' = stock torch ops around the linears")
     ap.add_argument('--kv', default='contiguous', choices=['contiguous', 'float16', 'int8', 'fp8_e4m3'],
-                    help='a paged key-value cache of that type with the library\'s decode attention, instead of the contiguous one')
+                    help='a paged key-value cache of that type with the library\'s decode attention, instead of the contiguous one '
+                         '(its prefill is eager)')
+    ap.add_argument('--eager-prefill', action='store_true',
+                    help='no graph for the prefill over the contiguous cache either, to compare its ttft with a paged cache\'s')
     args = ap.parse_args()
 
     import torch
@@ -69,7 +72,8 @@ def main():
                       'weights_gb': round(sum(b.numel() * b.element_size() for b in model.buffers()) / 2**30, 2)}))
     def sweep(label):
         for b in [int(v) for v in args.batches.split(',')]:
-            r = llm.measure_ttft_tpot(model, b, args.prompt, args.new, kv_dtype=None if args.kv == 'contiguous' else args.kv)
+            r = llm.measure_ttft_tpot(model, b, args.prompt, args.new, kv_dtype=None if args.kv == 'contiguous' else args.kv,
+                                      prefill_graph=not args.eager_prefill)
             r.update({'model': model.cfg.name, 'kv': args.kv, 'tp': world, 'small_allreduce': label, 'cache': ctx.stats(),
                       'peak_gb': round(torch.cuda.max_memory_allocated() / 2**30, 2)})
             say(json.dumps(r), flush=True)

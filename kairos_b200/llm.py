@@ -503,7 +503,8 @@ class Decoder(torch.nn.Module):
         """tokens [B, S] -> next token ids [B, 1]; fills the KV cache for positions 0..S-1.
 
         With a paged cache the prompts may differ in length (a list of token vectors) and, with `keep`, continue what the
-        sequences already hold (a prompt in chunks, another turn of a conversation); such a prefill runs eagerly.
+        sequences already hold (a prompt in chunks, another turn of a conversation).  Over a paged cache every prefill runs
+        eagerly, with use_graph too: its slots and lengths come from the host.
 
         use_graph: replay a CUDA graph captured for this (B, S) (the ~500 launches of a prefill are then off
         the host's critical path); the prompt is copied into the graph's static token buffer.  The graph is
@@ -605,8 +606,9 @@ class Decoder(torch.nn.Module):
         self.graph.replay()
 
     @torch.no_grad()
-    def generate(self, tokens, max_new_tokens, use_graph=True):
-        nxt = self.prefill(tokens, use_graph=use_graph)
+    def generate(self, tokens, max_new_tokens, use_graph=True, prefill_graph=None):
+        """Greedy tokens [B, max_new_tokens].  prefill_graph: see `prefill` (default: as use_graph)."""
+        nxt = self.prefill(tokens, use_graph=use_graph if prefill_graph is None else prefill_graph)
         out = [nxt]
         for _ in range(max_new_tokens - 1):
             self.tok.copy_(nxt)
@@ -617,12 +619,15 @@ class Decoder(torch.nn.Module):
 
 
 @torch.no_grad()
-def measure_ttft_tpot(model, batch, prompt_len=1024, new_tokens=512, warmup=2, ttft_times=5, seed=0, kv_dtype=None):
+def measure_ttft_tpot(model, batch, prompt_len=1024, new_tokens=512, warmup=2, ttft_times=5, seed=0, kv_dtype=None,
+                      prefill_graph=True):
     """TTFT = mean wall time of prefill + first token over `ttft_times` runs; TPOT = (time of a full
     generation - TTFT) / (new_tokens - 1); throughput = batch * new_tokens / (TTFT + (new_tokens-1) * TPOT)
     (utils/perf_eval.py:236-275 and kairos/main_ablation.py:111-125 of the reference).  kv_dtype: over a paged cache of
-    that type instead of the contiguous one."""
+    that type instead of the contiguous one.  The prefill over the contiguous cache is a captured graph (prefill_graph) or
+    eager, over a paged one always eager: 'prefill' in the result says which, and only alike ones compare."""
     dev = model.device
+    prefill_graph = prefill_graph and kv_dtype is None
     gen = torch.Generator(device=dev).manual_seed(seed)
     tokens = torch.randint(0, model.cfg.vocab, (batch, prompt_len), generator=gen, device=dev)
     if kv_dtype is None:
@@ -630,21 +635,21 @@ def measure_ttft_tpot(model, batch, prompt_len=1024, new_tokens=512, warmup=2, t
     else:
         model.allocate_paged(batch, prompt_len + new_tokens + 8, kv_dtype)
     for _ in range(warmup):
-        model.generate(tokens, 4)
+        model.generate(tokens, 4, prefill_graph=prefill_graph)
     torch.cuda.synchronize()
     t0 = time.perf_counter()
     for _ in range(ttft_times):
-        model.prefill(tokens, use_graph=True)
+        model.prefill(tokens, use_graph=prefill_graph)
         torch.cuda.synchronize()
     ttft = (time.perf_counter() - t0) / ttft_times
     torch.cuda.synchronize()
     t0 = time.perf_counter()
-    out = model.generate(tokens, new_tokens)
+    out = model.generate(tokens, new_tokens, prefill_graph=prefill_graph)
     torch.cuda.synchronize()
     total = time.perf_counter() - t0
     tpot = (total - ttft) / (new_tokens - 1)
-    return {'batch': batch, 'prompt_len': prompt_len, 'new_tokens': int(out.shape[1]), 'ttft_ms': 1e3 * ttft,
-            'tpot_ms': 1e3 * tpot, 'tokens_per_s': batch * new_tokens / (ttft + (new_tokens - 1) * tpot)}
+    return {'batch': batch, 'prompt_len': prompt_len, 'prefill': 'graph' if prefill_graph else 'eager',
+            'new_tokens': int(out.shape[1]), 'ttft_ms': 1e3 * ttft, 'tpot_ms': 1e3 * tpot, 'tokens_per_s': batch * new_tokens / (ttft + (new_tokens - 1) * tpot)}
 
 
 def build_lut(shapes, device='cuda', m_grid=None, cache='warm', n=20):

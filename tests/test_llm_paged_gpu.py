@@ -128,3 +128,11 @@ def test_a_refused_prompt_leaves_empty_sequences(model):
     assert model.paged.free_pages == 0
     model.allocate_paged(2, 64, page_size=16)
     assert close(got, model.prefill([prompt(5, 5), prompt(32, 6)], return_logits=True))
+
+
+def test_measurements_say_how_the_prefill_ran(model):
+    from kairos_b200 import llm
+    short = dict(prompt_len=8, new_tokens=3, warmup=1, ttft_times=1)
+    for kw, want, graphs in ((dict(), 'graph', 1), (dict(prefill_graph=False), 'eager', 0), (dict(kv_dtype='int8'), 'eager', 0)):
+        assert llm.measure_ttft_tpot(model, 2, **short, **kw)['prefill'] == want
+        assert len(model._prefill_graphs) == graphs
