@@ -292,7 +292,7 @@ class Decoder(torch.nn.Module):
         process group must not be destroyed while such a graph is alive (its teardown then never returns):
         call this, synchronize, and only then ``destroy_process_group``."""
         import gc
-        self.graph = None
+        self.graph = self._graph_logits = None
         self._prefill_graphs = {}
         gc.collect()
         torch.cuda.synchronize(self.device)
@@ -563,10 +563,12 @@ class Decoder(torch.nn.Module):
             self.graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(self.graph, stream=side):
                 self._paged_decode_body()
+            self._graph_logits = self.logits
             self.lens.copy_(before)
             torch.cuda.synchronize()
         if use_graph:
             self.graph.replay()
+            self.logits = self._graph_logits                      # an eager step in between left its own
         else:
             self._paged_decode_body()
         self.lengths = [n + 1 for n in self.lengths]
@@ -580,7 +582,8 @@ class Decoder(torch.nn.Module):
 
     @torch.no_grad()
     def decode_step(self, use_graph=True):
-        """One token for every sequence: reads self.tok, writes self.next_tok, advances self.pos (paged: self.lens)."""
+        """One token for every sequence: reads self.tok, writes self.next_tok and self.logits, advances self.pos (paged:
+        self.lens)."""
         if self.paged is not None:
             self._paged_decode_step(use_graph)
             return
@@ -600,10 +603,12 @@ class Decoder(torch.nn.Module):
             self.graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(self.graph, stream=side):
                 self._decode_body()
+            self._graph_logits = self.logits
             self.pos.copy_(pos0)
             self.mask.copy_(mask0)
             torch.cuda.synchronize()
         self.graph.replay()
+        self.logits = self._graph_logits                          # an eager step in between left its own
 
     @torch.no_grad()
     def generate(self, tokens, max_new_tokens, use_graph=True, prefill_graph=None):

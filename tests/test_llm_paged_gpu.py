@@ -136,3 +136,19 @@ def test_measurements_say_how_the_prefill_ran(model):
     for kw, want, graphs in ((dict(), 'graph', 1), (dict(prefill_graph=False), 'eager', 0), (dict(kv_dtype='int8'), 'eager', 0)):
         assert llm.measure_ttft_tpot(model, 2, **short, **kw)['prefill'] == want
         assert len(model._prefill_graphs) == graphs
+
+
+@pytest.mark.parametrize('paged', [False, True])
+def test_logits_are_those_of_the_last_step(model, paged):
+    """Captured and eager steps in turn: the logits follow whichever ran last."""
+    feed = torch.stack([prompt(8, 5), prompt(8, 6)])
+    runs = []
+    for modes in ([False] * 8, [True, False, True, True, False, False, True, True]):
+        model.allocate_paged(2, 32, page_size=16) if paged else model.allocate(2, 32)
+        model.prefill(torch.stack([prompt(7, 1), prompt(7, 2)]))
+        out = []
+        for i, graph in enumerate(modes):
+            out += steps(model, feed[:, i:i + 1], 1, graph)
+            assert torch.equal(model.next_tok[:, 0], out[-1].argmax(-1))
+        runs.append(out)
+    assert all(close(a, b) for a, b in zip(*runs))
