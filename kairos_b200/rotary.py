@@ -10,10 +10,11 @@ import torch
 from ._lib import RotaryPlan
 
 LAYOUTS = {'half': 0, 'interleaved': 1}
-# Frequencies are computed with 50 decimal digits: a step of the kernels is a fraction of 64 bits that far positions multiply, so
+# Frequencies are computed with 40 decimal digits: a step of the kernels is a fraction of 64 bits that far positions multiply, so
 # 64-bit floats would leave 2^-56 turns a position in the fast pairs.
-_DIGITS = Context(prec=50)
-_TWO_PI = 2 * Decimal('3.14159265358979323846264338327950288419716939937510582097')
+_DIGITS = Context(prec=40)
+_TWO_PI = Decimal('6.2831853071795864769252867665590057683943388')
+_PER_RADIAN = _DIGITS.divide(Decimal(1 << 64), _TWO_PI)         # of a turn in 64 bits
 
 
 class Rotary:
@@ -31,7 +32,7 @@ class Rotary:
                 the pair index between the two, and a magnitude on the turned channels.
 
     `frequencies` holds the radians per position of every pair (float64).  The kernels take them as 64-bit binary fractions of
-    a turn, rounded from 50 digits: an angle is off by 2^-65 turns for each position (2^-32 turns at position 2^33)."""
+    a turn, rounded from 40 digits: an angle is off by 2^-65 turns for each position (2^-32 turns at position 2^33)."""
 
     def __init__(self, head_dim, rot_dim=None, theta=10000.0, layout='half', scaling=None, device='cuda'):
         rot = head_dim if rot_dim is None else rot_dim
@@ -44,7 +45,7 @@ class Rotary:
         self.head_dim, self.rot_dim, self.layout, self.theta = head_dim, rot, layout, float(theta)
         with localcontext(_DIGITS):
             exact, self.magnitude = self._scaled(rot, float(theta), scaling)
-            turns = [round(f / _TWO_PI * (1 << 64)) % (1 << 64) for f in exact]
+            turns = [round(f * _PER_RADIAN) % (1 << 64) for f in exact]
         self.frequencies = torch.tensor([float(f) for f in exact], dtype=torch.float64)
         signed = [t - (1 << 64) if t >= 1 << 63 else t for t in turns]
         self.steps = torch.tensor(signed, dtype=torch.int64, device=device)
@@ -75,8 +76,9 @@ class Rotary:
                 raise ValueError(f'rotary scaling {kind!r} needs {name!r}')
             return float(value)
 
-        def blend(keep):          # keep = 1: the pair's own speed, 0: slowed by the factor
-            return [f * (k + (1 - k) / by) for f, k in zip(freq, (min(max(k, Decimal(0)), Decimal(1)) for k in keep))]
+        def blend(keep):          # keep = 1 and above: the pair's own speed, 0 and below: slowed by the factor
+            slow = 1 / by
+            return [f if k >= 1 else f * slow if k <= 0 else f * (k + (1 - k) * slow) for f, k in zip(freq, keep)]
 
         magnitude = 1.0
         if kind == 'linear':
@@ -87,7 +89,8 @@ class Rotary:
             trained, low, high = take('original_max'), take('low_freq_factor', 1.0), take('high_freq_factor', 4.0)
             if not high > low:
                 raise ValueError('rotary scaling: high_freq_factor must be above low_freq_factor')
-            freq = blend([(Decimal(trained) * f / _TWO_PI - Decimal(low)) / (Decimal(high) - Decimal(low)) for f in freq])
+            rate, offset = Decimal(trained) / _TWO_PI / (Decimal(high) - Decimal(low)), Decimal(low) / (Decimal(high) - Decimal(low))
+            freq = blend([rate * f - offset for f in freq])
         elif kind == 'yarn':
             trained, fast, slow = take('original_max'), take('beta_fast', 32.0), take('beta_slow', 1.0)
             magnitude = take('magnitude', 0.1 * math.log(factor) + 1)
@@ -95,7 +98,8 @@ class Rotary:
             def pair_of(turns):       # the pair that makes so many turns within the trained length
                 return rot * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(theta))
             lo, hi = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rot - 1)
-            freq = blend([1 - (i - lo) / max(Decimal(hi - lo), Decimal('1e-3')) for i in range(rot // 2)])
+            rate = 1 / max(Decimal(hi - lo), Decimal('1e-3'))
+            freq = blend([1 - (i - lo) * rate for i in range(rot // 2)])
         else:
             raise ValueError(f"rotary scaling type must be 'linear', 'ntk', 'llama3' or 'yarn', got {kind!r}")
         if opt:
