@@ -4,8 +4,10 @@
 // l = sum_j 2^(s_j - m), m = max_j s_j, in ONE pass over the cache: m, l and o are kept for the keys seen so far and
 // multiplied by 2^(m_old - m_new) where the maximum moves.  Parts of a sequence are joined by the same rule.
 //
-// Bound.  Every cached byte is read once and meets 2 * group flops (group = query heads per kv head): below 16 flops
-// a byte, so HBM sets the pace and everything here serves to keep loads in flight:
+// Bound.  With up to 16 query heads per kv head every cached byte is read once and meets 2 * group flops (group = query heads
+// per kv head): below 16 flops a byte, so HBM sets the pace and everything here serves to keep loads in flight.  Each further
+// 16 heads are blocks of their own that ask for the pages again (64 sequences up to 4000 positions, 4 kv heads of 128: 16 heads a
+// kv head 56 us, 32 75, 48 101 over fp16 rows, 48, 78 and 105 over int8 ones).
 //   * a warp owns a ring of stages of 16 positions (8 KB of K and V rows of 128 fp16 channels), filled by 16-byte
 //     cp.async with a swizzle of its own; no block-wide barrier until a pair ends, and the next pair is requested first;
 //   * the heads that share a kv head are the eight columns of warp-level tensor instructions (m16n8k16): scores^T = K q^T
@@ -17,11 +19,12 @@
 //     such blocks, or an even cut on the device, whatever the lengths are.  A pair that lies across blocks of the cut
 //     leaves one partial result per block in the workspace and a second kernel joins them in the order of the blocks (no
 //     atomics: same bits every run).
-// Measured on B200: one sequence of 131071 bf16 positions, 8 kv heads: 84.4 us = 6.36 TB/s (0.97 of the copy rate); 128
-// sequences of 2048 fp16 positions 161 us = 6.7 TB/s, in int8 92.8 us = 6.0 TB/s; 128 of 1 to 8192 in int8 176 us = 6.3 TB/s;
-// 2 x 1024 positions 6.6 us; 64 positions 3.5 us (2.2 us is an empty launch).  For codes the instruction stream comes next:
-// 400 warp instructions per 16 positions, 176 of them widening codes, take 63% of the issue slots.  Rows of 64 int8 channels,
-// half the bytes for more than half the instructions, reach 5.4 TB/s (128 sequences of 8192: 210 us).
+// Measured on B200, six to twelve calls in a graph: one sequence of 131071 bf16 positions, 8 kv heads: 84.9 us = 6.33 TB/s (0.97
+// of the copy rate); 128 sequences of 2048 fp16 positions 161 us = 6.7 TB/s, in int8 92.5 us = 6.0 TB/s; 128 of 1 to 8192 in int8
+// 177 us = 6.3 TB/s (back to back for a second, under the power cap, 203); 2 x 1024 positions 6.6 us; 64 positions 3.5 us (2.2 us
+// is an empty launch).  For codes the instruction stream comes next: 383 warp instructions per 16 positions, 176 of them widening
+// codes, take 60% of the issue slots.  Rows of 64 int8 channels, half the bytes for more than half the instructions, reach
+// 5.4 TB/s (128 sequences of 8192: 210 us).
 //
 // Precision.  Scores, references, sums and outputs are fp32.  What has fewer bits, since tensor instructions take 16-bit
 // operands, and why that is enough beside an output of 11 (fp16) or 8 bits (bf16):
@@ -309,7 +312,8 @@ __device__ __forceinline__ uint32_t place(int r, int c) {
 }
 
 // A warp's ring of stages of 16 positions; stages and blocks on an SM by what registers and measurements allow.
-// int8, 128 channels, 128 sequences up to 8192: 2 stages x 4 blocks an SM 176 us, 3 x 4 178, 4 x 3 179, 2 x 5 184.  fp16, one
+// int8, 128 channels, 128 sequences up to 8192, six calls in a graph: 2 stages x 4 blocks an SM 176.6 us, 3 x 4 177.8, 4 x 3 181,
+// 2 x 5 188 (within 0.2 each); of 2048 positions each 92.5, 94.4, 104 and 106; 64 up to 4000 55.3, 57.1, 58.8 and 61.  fp16, one
 // of 131071: 3 x 2 84.9 us, 2 x 3 85.9, 4 x 1 102.  64 sequences up to 4000: 256 channels int8 2 x 2 96 us, 3 x 2 100, 4 x 1
 // 134; 64 channels fp16 3 x 4 48.1, 4 x 3 49.2, 3 x 5 59; int8 2 x 4 37.2, 3 or 4 x 4 38.1, 2 x 5 38.0, 2 x 6 42.  Stages of 32
 // positions cost 5 to 50% more in all of them.
