@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(128, (Ring<D, !std::is_void<Widen>::value, (kB
                     }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e2 = top > 0.f && top <= 3e38f ? max(-110, min(126, (int)(__float_as_uint(top) >> 23) - 127)) : 13;
+                const int e2 = top > 0.f && top <= FLT_MAX ? max(-110, min(126, (int)(__float_as_uint(top) >> 23) - 127)) : 13;
                 const float up = __uint_as_float((uint32_t)(127 + 13 - e2) << 23);
                 const float back = p.scale_log2 * __uint_as_float((uint32_t)(127 - 13 + e2) << 23);
                 unit[r] = make_float2(__shfl_sync(0xffffffffu, back, 8 * t), __shfl_sync(0xffffffffu, back, 8 * t + 4));

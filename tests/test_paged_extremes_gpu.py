@@ -184,6 +184,21 @@ def test_small_weights_over_fp16_rows_beside_a_large_one(h, hkv, gap):
     assert ((got[0].view(hkv, h, 64).double() - ref[:, None]).abs() <= tol[:, None]).all()
 
 
+@pytest.mark.parametrize('kv', [I8, E4M3])
+@pytest.mark.parametrize('largest', [2.9e38, 3.2e38, torch.finfo(torch.bfloat16).max])
+def test_queries_up_to_the_largest_bf16(kv, largest):
+    """Over codes, where the queries are brought into range before the product.  (Over bf16 rows the product itself would pass
+    fp32: 3e38 times a key of 2.)"""
+    from kairos_b200 import ops
+    lens = [200, 33]
+    c, q, table, n = attention_case(BF16, kv, lens, 8, 2, 64, 16, seed=4)
+    q = (q.float() * 2.0 ** 125).to(BF16)
+    q[:, ::2, 5] = largest
+    q[:, 1::2, 5] = -largest
+    got, lse = ops.paged_attention(q, c, table, n, scale=2.0 ** -127, return_lse=True)
+    check_attention(c, q, table, lens, got, lse, scale=2.0 ** -127)
+
+
 def test_rotary_refuses_results_that_overlap():
     import kairos_b200 as kb
     from kairos_b200 import ops
