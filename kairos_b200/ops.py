@@ -334,11 +334,13 @@ def _disjoint(shape, a, b, offset):
     if offset > ends[0] or -offset > ends[1]:
         return True
     dims = sorted((step, n) for step, n in zip(a, shape) if n > 1)
-    if dims and dims == sorted((step, n) for step, n in zip(b, shape) if n > 1):
-        # slices of one activation: both stay within a part of each step of the largest dimension
-        step, reach = dims[-1][0], sum((n - 1) * step for step, n in dims[:-1])
-        if step and reach < offset % step < step - reach:
-            return True
+    if dims == sorted((step, n) for step, n in zip(b, shape) if n > 1):
+        # slices of one activation: modulo a step that divides the larger ones both stay within a part of it
+        reach = 0
+        for i, (step, n) in enumerate(dims):
+            if step and all(larger % step == 0 for larger, _ in dims[i:]) and reach < offset % step < step - reach:
+                return True
+            reach += (n - 1) * step
     first, second = _rows(shape, a), _rows(shape, b) + offset
     near = torch.searchsorted(first, second)                  # the rows of `a` on either side of each row of `b`
     behind = first[near.clamp(max=len(first) - 1)] - second
@@ -364,7 +366,7 @@ def rotary(x, positions, rotary, transpose=False, out=None):
         if out.stride(-1) != 1:                 # overlapping windows: another dimension came out as the dense one
             out = x.new_empty(shape)
     elif out.shape != shape or out.dtype != x.dtype or out.get_device() != index or out.stride(-1) != 1 or \
-            not _distinct(shape, out.stride()):
+            not (out.is_contiguous() or _distinct(shape, out.stride())):
         raise _bad(out, 'out', f'{x.dtype} {tuple(shape)} with a dense last dimension and a place for every element', index)
     elif out is not x and not (out.data_ptr() == x.data_ptr() and
                                all(a == b or n == 1 for a, b, n in zip(out.stride(), strides, shape))) and \

@@ -283,3 +283,14 @@ def test_steps_are_rounded_once(rot, theta, scaling):
             off = (step - f / two_pi() * (1 << 64)) % (1 << 64)
             assert min(off, (1 << 64) - off) <= Decimal('0.5000001')
             assert abs(Decimal(kept) - f) <= f * Decimal(2) ** -53
+
+
+def test_slices_of_one_activation_are_told_apart_at_once(monkeypatch):
+    """The usual neighbours -- heads of another kind in the same rows, batched or not -- without a look at every row."""
+    monkeypatch.setattr(ops, '_rows', None)
+    row, heads = 40 * 64, 8
+    for shape, strides in (((4096, heads, 64), (row, 64, 1)), ((32, 4096, heads, 64), (4096 * row, row, 64, 1)),
+                           ((heads, 4096, 64), (64, row, 1)), ((1, 4096, heads, 64), (7, row, 64, 1))):
+        assert ops._distinct(shape, strides)
+        for offset in (heads * 64, -heads * 64, 20 * 64, 4096 * row * 40):
+            assert ops._disjoint(shape, strides, strides, offset)
