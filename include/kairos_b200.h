@@ -286,7 +286,7 @@ int kairos_paged_kv_read(const kairos_kv_layer* kv, const void* slots, void* K_o
  * Scores, softmax sums and outputs are accumulated in fp32.  The weight that multiplies a row of V is held in two 16-bit
  * numbers: to 2^-16 of itself over BF16 rows; to 2^-22 of itself or 2^-37 of the head's largest weight, whichever is more,
  * over F16 rows; over codes weight times V scale is, to 2^-22 of itself or 2^-33 of the largest such product.  BF16 queries
- * over codes are held to 2^-38 of the head's largest value.
+ * over codes are held to 2^-38 of the head's largest value.  Weights below 2^-102 of the head's largest may count as 0.
  * `workspace` of kairos_paged_attention_workspace_bytes() is scratch of this call alone (contents need no
  * initialisation): calls that may overlap need workspaces of their own. */
 size_t kairos_paged_attention_workspace_bytes(const kairos_kv_layer* kv, int B, int H, int table_width);

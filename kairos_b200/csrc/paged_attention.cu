@@ -32,8 +32,9 @@
 //     would add an error as large as the output's own rounding.  Over bf16 rows they are off by 2^-16 of each weight; over fp16 rows
 //     2^-22 of each, but no less than 2^-37 of the head's largest; over codes the same with 2^-33 of the largest product;
 //   * bf16 queries over codes become fp16 times a power of two per head: exact to 2^-38 of the head's largest value.
-// Exponentials are ex2.approx (2 U); an argument below -126 gives 0.  The reference need not be the maximum: it moves (and o and
-// l are rescaled) only when a score passes it by 2^slack, so most stages need neither a reduction over lanes nor a rescaling.
+// Exponentials are ex2.approx (2 U); an argument below -126 gives 0: weights of less than 2^-110 of the reference (fp16 rows:
+// 2^-138).  The reference need not be the maximum: it moves (and o and l are rescaled) only when a score passes it by 2^slack, so
+// most stages need neither a reduction over lanes nor a rescaling.
 #include <cfloat>
 #include <type_traits>
 

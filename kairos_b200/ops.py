@@ -352,7 +352,8 @@ def _disjoint(shape, a, b, offset):
 def rotary(x, positions, rotary, transpose=False, out=None):
     """Heads [T, H, D] or [B, S, H, D] (fp16, bf16 or fp32; dense last dimension, any other strides) turned by their
     int64 positions, [T] or broadcastable to [B, S], with the plan of a :class:`Rotary`.  ``transpose`` turns back with the same
-    magnitude: the gradient of x from that of the result.  ``out`` may be x, and must not overlap it otherwise."""
+    magnitude: the gradient of x from that of the result.  ``out`` may be x, and must not overlap it otherwise.
+    Like the other operators here it records no autograd graph."""
     shape, strides, code, index = x.shape, x.stride(), _FLOATS.get(x.dtype), x.get_device()
     dims = len(shape)
     if code is None or not 3 <= dims <= 4 or shape[-1] != rotary.head_dim or strides[-1] != 1:
