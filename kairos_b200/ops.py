@@ -308,9 +308,9 @@ def _bad(t, name, want, index):
 
 def _rows(shape, strides):
     """Where the rows of a tensor with a dense last dimension begin, in elements, in ascending order."""
-    at = torch.zeros(1, dtype=_int64)
+    at = torch.zeros(1, dtype=_int64, device='cpu')
     for n, step in zip(shape[:-1], strides[:-1]):
-        at = (at[:, None] + torch.arange(n) * step).flatten()
+        at = (at[:, None] + torch.arange(n, device='cpu') * step).flatten()
     return at.sort().values
 
 
